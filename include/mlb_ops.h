@@ -53,7 +53,10 @@ enum {
 enum {
   MLB_STATUS_BAD_TOKEN = 1,    /* embedding: token id < 0 or >= vocab      */
   MLB_STATUS_BAD_POSITION = 2, /* rope: position < 0 or >= table rows     */
-  MLB_STATUS_BAD_LENGTH = 4    /* softmax: valid length outside [1, cols] */
+  MLB_STATUS_BAD_LENGTH = 4,   /* softmax: valid length outside [1, cols];
+                                  batched entries: a sequence's length or
+                                  row range outside its tensors          */
+  MLB_STATUS_BAD_BLOCK = 8     /* 8-bit cache: block id < 0 or >= n_blocks */
 };
 
 /* Table formats; same order as the reference's QuantType
@@ -385,6 +388,174 @@ int mlb_attention_decode_noalloc_f32(const float* q, const float* keys,
                                      int64_t position, int64_t max_seq,
                                      int n_heads, int n_kv_heads, int head_dim,
                                      void* stream);
+
+/*
+ * ---------------------------------------------------------------------------
+ * Several sequences at once.  No counterpart in the reference, whose context
+ * holds one sequence: these entries take the rows of n_seqs sequences of
+ * different lengths in one call.
+ *
+ * Packed rows: the rows of all sequences stand one behind another, sequence i
+ * at rows [offsets[i], offsets[i + 1]) with offsets a DEVICE array of
+ * n_seqs + 1 int32 (0 <= offsets[0] <= offsets[1] <= ... <= the tensor's
+ * rows).  Rows outside every sequence are not read and not written.  A
+ * sequence whose range is not inside the tensor (or runs backwards) raises
+ * MLB_STATUS_BAD_LENGTH and is left out as if it were empty.
+ */
+
+/* Floats of scratch mlb_attention_packed_f32 needs (-1 for bad arguments). */
+int64_t mlb_attention_packed_scratch_floats(int64_t q_rows, int64_t k_rows,
+                                            int64_t n_seqs, int n_heads,
+                                            int n_kv_heads, int head_dim);
+
+/*
+ * Causal attention over packed sequences: whole prompts, or new rows after
+ * earlier tokens.  Sequence i has Q = q_offsets[i + 1] - q_offsets[i] query
+ * rows and K = k_offsets[i + 1] - k_offsets[i] keys; its last query row sees
+ * all K keys, the row before it K - 1, and so on: row r sees keys
+ * 0 .. K - Q + r of its own sequence.  For a whole prompt k_offsets is
+ * q_offsets.  A row that sees no key (K < Q) is written as zeros.
+ *   out[r][h] = softmax_t(q[r][h] . k_t / sqrt(head_dim)) . v_t
+ * with kv head h / (n_heads / n_kv_heads) for query head h, as
+ * mlb_attention_rows_f32, which it equals for one sequence.
+ *   q, out: [q_rows, n_heads, head_dim]; k, v: [k_rows, n_kv_heads,
+ *   head_dim]; group n_heads / n_kv_heads <= 8; head_dim % 4 == 0, <= 256;
+ *   q, k, v, out 16-byte aligned; q_rows, k_rows, n_seqs < 2^31 / 8.
+ *   scratch: caller-owned device memory of at least
+ *   mlb_attention_packed_scratch_floats(...) floats, 16-byte aligned.
+ * Within 1e-5 * sum_t w_t |v_t| of the exact result for scores of ordinary
+ * spread.  out must not overlap q, k or v.
+ */
+int mlb_attention_packed_f32(const float* q, const float* k, const float* v,
+                             float* out, const int32_t* q_offsets,
+                             const int32_t* k_offsets, int64_t n_seqs,
+                             int64_t q_rows, int64_t k_rows, int n_heads,
+                             int n_kv_heads, int head_dim, float* scratch,
+                             int64_t scratch_floats, int32_t* status,
+                             void* stream);
+
+/*
+ * 8-bit KV cache in blocks.  A pool of n_blocks blocks, each holding
+ * block_tokens (32, 64 or 128) consecutive tokens of one sequence for every
+ * kv head, serves all sequences of a layer:
+ *   k_codes  int8  [n_blocks, n_kv_heads, block_tokens, head_dim]
+ *   v_codes  int8  [n_blocks, n_kv_heads, head_dim, block_tokens]
+ *   k_scales, v_scales  float [n_blocks, n_kv_heads]
+ *   value = code * scale, codes in [-127, 127];
+ * (V is transposed inside a block, so that in both products of the attention
+ * the codes that are summed over lie side by side).  head_dim % 32 == 0,
+ * <= 256; code pointers 16-byte aligned.  Sequence i's tokens
+ * [c * block_tokens, (c + 1) * block_tokens) are in block
+ * table[i * table_cols + c]; table is a DEVICE array [n_seqs, table_cols].
+ * Two sequences may share blocks that are only read.  A block id outside
+ * [0, n_blocks) raises MLB_STATUS_BAD_BLOCK and is never used as an address.
+ */
+
+/*
+ * Writes packed rows' k and v ([rows, n_kv_heads, head_dim] fp32, 16-byte
+ * aligned) into the cache: row offsets[i] + r of sequence i becomes its token
+ * positions[i] + r (positions: DEVICE [n_seqs] int32, the tokens that the
+ * sequence already holds).  Per block and kv head, for K and V alike:
+ *   scale' = max(amax(new rows) / 127, scale if the block holds earlier
+ *            tokens of the sequence)
+ *   new code     = round(x / scale')               (half to even, clamped
+ *   earlier code = round(code * scale / scale')     to [-127, 127])
+ * the quotients taken exactly; a scale of 0 gives codes 0.  Codes of the
+ * block's places behind the last written token become 0.  A block that
+ * receives Inf or NaN gets an infinite or NaN scale: all its values read as
+ * NaN.  A sequence whose positions leave the table (position < 0, or token
+ * >= table_cols * block_tokens) raises MLB_STATUS_BAD_POSITION, a bad block id
+ * MLB_STATUS_BAD_BLOCK; those blocks are skipped, the others written.  A
+ * block that receives rows must belong to one sequence only.  The call is
+ * idempotent: repeated with the same arguments it leaves the same cache.
+ */
+int mlb_kv8_write_f32(int8_t* k_codes, int8_t* v_codes, float* k_scales,
+                      float* v_scales, int64_t n_blocks, int block_tokens,
+                      const int32_t* table, int64_t table_cols, int64_t n_seqs,
+                      const float* k, const float* v, const int32_t* offsets,
+                      const int32_t* positions, int64_t rows, int n_kv_heads,
+                      int head_dim, int32_t* status, void* stream);
+
+/*
+ * Reads tokens back as values: token positions[i] + r of sequence i to row
+ * offsets[i] + r of k and v, [rows, n_kv_heads, head_dim] fp32 (for example
+ * the earlier tokens of a sequence, as keys of mlb_attention_packed_f32).
+ * k or v may be NULL.  Tokens outside the table or in a block with a bad id
+ * raise the status bits as in mlb_kv8_write_f32 and their rows are written
+ * as zeros.
+ */
+int mlb_kv8_read_f32(const int8_t* k_codes, const int8_t* v_codes,
+                     const float* k_scales, const float* v_scales,
+                     int64_t n_blocks, int block_tokens, const int32_t* table,
+                     int64_t table_cols, int64_t n_seqs, float* k, float* v,
+                     const int32_t* offsets, const int32_t* positions,
+                     int64_t rows, int n_kv_heads, int head_dim,
+                     int32_t* status, void* stream);
+
+/* Floats of scratch mlb_attention_kv8_f32 needs (-1 for bad arguments);
+ * with_mass: whether mass_out will be given. */
+int64_t mlb_attention_kv8_scratch_floats(int64_t n_seqs, int64_t table_cols,
+                                         int block_tokens, int n_heads,
+                                         int n_kv_heads, int head_dim,
+                                         int with_mass);
+
+/*
+ * Decode attention of one token of each of n_seqs sequences over the 8-bit
+ * cache: sequence i's query sees its first lengths[i] tokens (lengths: DEVICE
+ * [n_seqs] int32; the current token's K and V are written first).
+ *   out[i][h] = softmax_t(q[i][h] . k_t / sqrt(head_dim)) . v_t
+ * q, out: [n_seqs, n_heads, head_dim] fp32, 16-byte aligned; grouped heads as
+ * mlb_attention_decode_f32 (group <= 8).  A sequence of length 0 gets zeros.
+ * A length outside [0, table_cols * block_tokens] raises
+ * MLB_STATUS_BAD_LENGTH, a bad block id among the sequence's blocks
+ * MLB_STATUS_BAD_BLOCK; that sequence's out is zeros.
+ * mass_out (or NULL): [n_seqs, table_cols] fp32, the attention weight that
+ * each block collects, for mlb_kv8_evict:
+ *   mass_out[i][c] = mass_in[i][c] + sum over query heads and the tokens of
+ *                    block c of the softmax weights
+ * (mass_in NULL reads as zeros and may be mass_out itself; sequences with an
+ * error and places behind the last block get mass_in unchanged).
+ * scratch: at least mlb_attention_kv8_scratch_floats(...) floats, 16-byte
+ * aligned.  Deterministic.  Queries are taken in 22 bits, the weights in 22
+ * bits, all sums in fp32: within 1e-5 * sum_t w_t |v_t| of the exact result
+ * over the cache's values for scores of ordinary spread.
+ */
+int mlb_attention_kv8_f32(const float* q, const int8_t* k_codes,
+                          const int8_t* v_codes, const float* k_scales,
+                          const float* v_scales, int64_t n_blocks,
+                          int block_tokens, const int32_t* table,
+                          int64_t table_cols, const int32_t* lengths,
+                          int64_t n_seqs, int n_heads, int n_kv_heads,
+                          int head_dim, float* out, const float* mass_in,
+                          float* mass_out, float* scratch,
+                          int64_t scratch_floats, int32_t* status,
+                          void* stream);
+
+/*
+ * Eviction of whole blocks by collected attention weight.  A sequence of
+ * B = ceil(lengths[i] / block_tokens) > keep_blocks blocks gives up
+ * B - keep_blocks of them: its first sink_blocks and last recent_blocks stay
+ * (sink_blocks >= 0, recent_blocks >= 1, sink_blocks + recent_blocks <=
+ * keep_blocks), of the others those with the least mass leave, of equal
+ * masses the earlier block (NaN counts as largest, -0 as 0).  No cached
+ * token moves: the surviving blocks' ids and masses close up in order.
+ *   table_out   [n_seqs, table_cols]  surviving ids, then -1
+ *   lengths_out [n_seqs]              length - block_tokens * blocks left
+ *   mass_out    [n_seqs, table_cols]  surviving masses, then 0
+ *   freed       [n_seqs, table_cols]  ids of the blocks that left, in order,
+ *                                     then -1 (or NULL)
+ * table_out, lengths_out and mass_out may be table, lengths and mass; freed
+ * overlaps none of them.  A length outside [0, table_cols * block_tokens]
+ * raises MLB_STATUS_BAD_LENGTH; that sequence's table, length and mass are
+ * copied unchanged and nothing is freed.  Keys keep the positions they were
+ * rotated for; the next token's position is the caller's to count.
+ */
+int mlb_kv8_evict(const int32_t* table, int64_t table_cols,
+                  const int32_t* lengths, const float* mass, int64_t n_seqs,
+                  int block_tokens, int64_t keep_blocks, int64_t sink_blocks,
+                  int64_t recent_blocks, int32_t* table_out,
+                  int32_t* lengths_out, float* mass_out, int32_t* freed,
+                  int32_t* status, void* stream);
 
 /*
  * Helper for synchronous callers: waits for `stream`, copies the device

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from collections import namedtuple
 from ctypes import c_float, c_int, c_int64, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -22,6 +23,7 @@ LIB_PATH = os.path.join(HERE, "libmlb.so")
 F32, Q8_0, Q4_0, Q4_1 = 0, 1, 2, 3
 QTYPE_NAMES = {"F32": F32, "Q8_0": Q8_0, "Q4_0": Q4_0, "Q4_1": Q4_1}
 STATUS_BAD_TOKEN, STATUS_BAD_POSITION, STATUS_BAD_LENGTH = 1, 2, 4
+STATUS_BAD_BLOCK = 8
 
 # Every symbol include/mlb_ops.h declares, with (restype, argtypes).
 SIGNATURES = {
@@ -79,6 +81,24 @@ SIGNATURES = {
     "mlb_attention_decode_noalloc_f32": (c_int, [c_void_p, c_void_p, c_void_p,
                                                  c_void_p, c_int64, c_int64, c_int,
                                                  c_int, c_int, c_void_p]),
+    "mlb_attention_packed_scratch_floats": (c_int64, [c_int64, c_int64, c_int64, c_int,
+                                                      c_int, c_int]),
+    "mlb_attention_packed_f32": (c_int, [c_void_p] * 6 + [c_int64] * 3 + [c_int] * 3 +
+                                 [c_void_p, c_int64, c_void_p, c_void_p]),
+    "mlb_kv8_write_f32": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_void_p, c_int64,
+                                                   c_int64] + [c_void_p] * 4 +
+                          [c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "mlb_kv8_read_f32": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_void_p, c_int64,
+                                                  c_int64] + [c_void_p] * 4 +
+                         [c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "mlb_attention_kv8_scratch_floats": (c_int64, [c_int64, c_int64, c_int, c_int, c_int,
+                                                   c_int, c_int]),
+    "mlb_attention_kv8_f32": (c_int, [c_void_p] * 5 + [c_int64, c_int, c_void_p, c_int64,
+                                                       c_void_p, c_int64, c_int, c_int,
+                                                       c_int] + [c_void_p] * 4 +
+                              [c_int64, c_void_p, c_void_p]),
+    "mlb_kv8_evict": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int,
+                              c_int64, c_int64, c_int64] + [c_void_p] * 6),
 }
 
 _lib = None
@@ -462,6 +482,240 @@ def linear_rows_group(weights, qtype: int, ns, k: int, x, scratch=None, stream=N
                                             _ptr(scratch), scratch.numel(), _stream(stream)),
            op)
     return outs
+
+
+# ---------------------------------------------------------------------------
+# Several sequences at once.  Every tensor of a call is on one device, and the
+# call runs there whichever device is current.  Scratch and results that a
+# call allocates belong to the stream it runs on.
+
+class _On:
+    """The device of `tensor` current and, if given, `stream` too."""
+
+    def __init__(self, tensor, stream):
+        import torch
+        self.device = torch.cuda.device(tensor.device)
+        self.stream = None if stream is None else torch.cuda.stream(stream)
+
+    def __enter__(self):
+        self.device.__enter__()
+        if self.stream is not None:
+            self.stream.__enter__()
+        return _stream(None)
+
+    def __exit__(self, *exc):
+        if self.stream is not None:
+            self.stream.__exit__(*exc)
+        self.device.__exit__(*exc)
+
+
+def _like(t, dtype, device, op, name, shape=None):
+    if not (t.dtype == dtype and t.device == device and t.is_contiguous()):
+        raise ValueError(f"{op}: {name} must be a contiguous {dtype} tensor on {device}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{op}: {name} must be {list(shape)}, got {list(t.shape)}")
+
+
+def _status_word(status, device, op):
+    import torch
+    if status is not None:
+        _require(status.dtype == torch.int32 and status.device == device and
+                 status.numel() >= 1, op, f"status must be int32 on {device}")
+
+
+def attention_packed(q, k, v, q_offsets, k_offsets=None, out=None, scratch=None, status=None,
+                     stream=None):
+    """Causal attention over packed sequences: q [rows, n_heads, hd], k and v
+    [keys, kv_heads, hd], sequence i at q_offsets[i]:q_offsets[i + 1] and
+    k_offsets[i]:k_offsets[i + 1] (int32 [n_seqs + 1]; k_offsets None: whole
+    prompts, keys where the rows are).  The last row of a sequence sees all
+    of its keys.  Returns [rows, n_heads, hd]; rows outside every sequence
+    are not written."""
+    import torch
+    op = "attention_packed"
+    device = q.device
+    _require(q.is_cuda and q.dim() == 3 and k.dim() == 3, op,
+             "q must be [rows, heads, head_dim], k [keys, kv_heads, head_dim]")
+    _like(q, torch.float32, device, op, "q")
+    _like(k, torch.float32, device, op, "k")
+    _like(v, torch.float32, device, op, "v", k.shape)
+    rows, nh, hd = q.shape
+    keys, kvh, khd = k.shape
+    _require(khd == hd, op, "q and k differ in head_dim")
+    _require(q_offsets.dim() == 1 and q_offsets.numel() >= 1, op, "q_offsets must be [n_seqs + 1]")
+    _like(q_offsets, torch.int32, device, op, "q_offsets")
+    if k_offsets is None:
+        _require(keys == rows, op, "k_offsets is needed when k has other rows than q")
+        k_offsets = q_offsets
+    else:
+        _like(k_offsets, torch.int32, device, op, "k_offsets", q_offsets.shape)
+    n_seqs = q_offsets.numel() - 1
+    _status_word(status, device, op)
+    if out is not None:
+        _like(out, torch.float32, device, op, "out", q.shape)
+    lib = load()
+    with _On(q, stream) as on:
+        if out is None:
+            out = torch.empty_like(q)
+        if scratch is None:
+            need = lib.mlb_attention_packed_scratch_floats(rows, keys, n_seqs, nh, kvh, hd)
+            scratch = torch.empty(max(need, 1), dtype=torch.float32, device=device)
+        else:
+            _like(scratch, torch.float32, device, op, "scratch")
+        _check(lib.mlb_attention_packed_f32(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_offsets.data_ptr(),
+            k_offsets.data_ptr(), n_seqs, rows, keys, nh, kvh, hd, scratch.data_ptr(),
+            scratch.numel(), _ptr(status), on), op)
+    return out
+
+
+# The 8-bit KV cache's pool: codes int8 (k [blocks, kv_heads, block, hd], v
+# [blocks, kv_heads, hd, block]) and scales float32 [blocks, kv_heads].
+Kv8Cache = namedtuple("Kv8Cache", "k_codes v_codes k_scales v_scales")
+
+
+def kv8_cache(n_blocks: int, n_kv_heads: int, block_tokens: int, head_dim: int, device):
+    """An empty pool (all zeros)."""
+    import torch
+    _require(block_tokens in (32, 64, 128) and head_dim % 32 == 0 and 0 < head_dim <= 256,
+             "kv8_cache", "block_tokens 32, 64 or 128; head_dim % 32 == 0, <= 256")
+    codes = [torch.zeros(shape, dtype=torch.int8, device=device)
+             for shape in ((n_blocks, n_kv_heads, block_tokens, head_dim),
+                           (n_blocks, n_kv_heads, head_dim, block_tokens))]
+    scales = [torch.zeros((n_blocks, n_kv_heads), dtype=torch.float32, device=device)
+              for _ in range(2)]
+    return Kv8Cache(*codes, *scales)
+
+
+def _pool(cache, device, op):
+    """(n_blocks, kv_heads, block_tokens, head_dim) of a pool."""
+    import torch
+    k = cache.k_codes
+    _require(k.is_cuda and k.dim() == 4, op, "k_codes must be [blocks, kv_heads, block, head_dim]")
+    n, kvh, block, hd = k.shape
+    _like(k, torch.int8, device, op, "k_codes")
+    _like(cache.v_codes, torch.int8, device, op, "v_codes", (n, kvh, hd, block))
+    _like(cache.k_scales, torch.float32, device, op, "k_scales", (n, kvh))
+    _like(cache.v_scales, torch.float32, device, op, "v_scales", (n, kvh))
+    return n, kvh, block, hd
+
+
+def _table(table, device, op):
+    import torch
+    _require(table.dim() == 2, op, "table must be [n_seqs, columns]")
+    _like(table, torch.int32, device, op, "table")
+    return table.shape
+
+
+def kv8_write(cache, table, k, v, offsets, positions, status=None, stream=None):
+    """Writes packed rows k, v [rows, kv_heads, hd] into the 8-bit cache: rows
+    offsets[i]:offsets[i + 1] become the tokens of sequence i from
+    positions[i] on (int32 [n_seqs + 1] and [n_seqs])."""
+    import torch
+    op = "kv8_write"
+    device = cache.k_codes.device
+    n_blocks, kvh, block, hd = _pool(cache, device, op)
+    n_seqs, cols = _table(table, device, op)
+    _require(k.dim() == 3 and k.shape[1:] == (kvh, hd), op, "k must be [rows, kv_heads, head_dim]")
+    _like(k, torch.float32, device, op, "k")
+    _like(v, torch.float32, device, op, "v", k.shape)
+    _like(offsets, torch.int32, device, op, "offsets", (n_seqs + 1,))
+    _like(positions, torch.int32, device, op, "positions", (n_seqs,))
+    _status_word(status, device, op)
+    with _On(k, stream) as on:
+        _check(load().mlb_kv8_write_f32(
+            cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scales.data_ptr(),
+            cache.v_scales.data_ptr(), n_blocks, block, table.data_ptr(), cols, n_seqs,
+            k.data_ptr(), v.data_ptr(), offsets.data_ptr(), positions.data_ptr(), k.shape[0],
+            kvh, hd, _ptr(status), on), op)
+
+
+def kv8_read(cache, table, offsets, positions, rows: int, status=None, stream=None):
+    """Reads tokens back: (k, v) [rows, kv_heads, hd] with token positions[i] + r
+    of sequence i at row offsets[i] + r; rows outside every sequence are not
+    written."""
+    import torch
+    op = "kv8_read"
+    device = cache.k_codes.device
+    n_blocks, kvh, block, hd = _pool(cache, device, op)
+    n_seqs, cols = _table(table, device, op)
+    _like(offsets, torch.int32, device, op, "offsets", (n_seqs + 1,))
+    _like(positions, torch.int32, device, op, "positions", (n_seqs,))
+    _status_word(status, device, op)
+    with _On(table, stream) as on:
+        k = torch.empty((rows, kvh, hd), dtype=torch.float32, device=device)
+        v = torch.empty((rows, kvh, hd), dtype=torch.float32, device=device)
+        _check(load().mlb_kv8_read_f32(
+            cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scales.data_ptr(),
+            cache.v_scales.data_ptr(), n_blocks, block, table.data_ptr(), cols, n_seqs,
+            k.data_ptr(), v.data_ptr(), offsets.data_ptr(), positions.data_ptr(), rows, kvh, hd,
+            _ptr(status), on), op)
+    return k, v
+
+
+def attention_kv8(q, cache, table, lengths, out=None, mass_in=None, mass_out=None, scratch=None,
+                  status=None, stream=None):
+    """Decode attention of q [n_seqs, n_heads, hd] over the 8-bit cache: sequence
+    i sees its first lengths[i] tokens (int32 [n_seqs]) -> [n_seqs, n_heads,
+    hd].  With mass_out [n_seqs, columns], the attention weight each block
+    collected, added to mass_in (None: zeros; may be mass_out)."""
+    import torch
+    op = "attention_kv8"
+    device = q.device
+    n_blocks, kvh, block, hd = _pool(cache, device, op)
+    n_seqs, cols = _table(table, device, op)
+    _require(q.dim() == 3 and q.shape[0] == n_seqs and q.shape[2] == hd, op,
+             "q must be [n_seqs, heads, head_dim]")
+    _like(q, torch.float32, device, op, "q")
+    _like(lengths, torch.int32, device, op, "lengths", (n_seqs,))
+    nh = q.shape[1]
+    for m, name in ((mass_in, "mass_in"), (mass_out, "mass_out")):
+        if m is not None:
+            _like(m, torch.float32, device, op, name, table.shape)
+    _status_word(status, device, op)
+    if out is not None:
+        _like(out, torch.float32, device, op, "out", q.shape)
+    lib = load()
+    with _On(q, stream) as on:
+        if out is None:
+            out = torch.empty_like(q)
+        if scratch is None:
+            need = lib.mlb_attention_kv8_scratch_floats(n_seqs, cols, block, nh, kvh, hd,
+                                                        0 if mass_out is None else 1)
+            scratch = torch.empty(max(need, 1), dtype=torch.float32, device=device)
+        else:
+            _like(scratch, torch.float32, device, op, "scratch")
+        _check(lib.mlb_attention_kv8_f32(
+            q.data_ptr(), cache.k_codes.data_ptr(), cache.v_codes.data_ptr(),
+            cache.k_scales.data_ptr(), cache.v_scales.data_ptr(), n_blocks, block,
+            table.data_ptr(), cols, lengths.data_ptr(), n_seqs, nh, kvh, hd, out.data_ptr(),
+            _ptr(mass_in), _ptr(mass_out), scratch.data_ptr(), scratch.numel(), _ptr(status),
+            on), op)
+    return out
+
+
+def kv8_evict(table, lengths, mass, block_tokens: int, keep_blocks: int, sink_blocks: int = 1,
+              recent_blocks: int = 1, status=None, stream=None):
+    """Shrinks every sequence to at most keep_blocks blocks: the first
+    sink_blocks and last recent_blocks stay, of the others those with the
+    least mass leave.  Returns new (table, lengths, mass, freed); freed lists
+    the ids of the blocks that left, -1 behind them."""
+    import torch
+    op = "kv8_evict"
+    device = table.device
+    _require(table.is_cuda, op, "table must be a CUDA tensor")
+    n_seqs, cols = _table(table, device, op)
+    _like(lengths, torch.int32, device, op, "lengths", (n_seqs,))
+    _like(mass, torch.float32, device, op, "mass", table.shape)
+    _status_word(status, device, op)
+    with _On(table, stream) as on:
+        table_out, freed = torch.empty_like(table), torch.empty_like(table)
+        lengths_out, mass_out = torch.empty_like(lengths), torch.empty_like(mass)
+        _check(load().mlb_kv8_evict(
+            table.data_ptr(), cols, lengths.data_ptr(), mass.data_ptr(), n_seqs, block_tokens,
+            keep_blocks, sink_blocks, recent_blocks, table_out.data_ptr(),
+            lengths_out.data_ptr(), mass_out.data_ptr(), freed.data_ptr(), _ptr(status), on), op)
+    return table_out, lengths_out, mass_out, freed
 
 
 def status_check(status, stream=None) -> int:

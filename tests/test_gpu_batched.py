@@ -1,0 +1,792 @@
+"""Operators over several sequences at once, against plain evaluations in 64
+bits: packed prompt attention, the 8-bit KV cache (write, read, decode
+attention, collected weights) and eviction.
+
+Tolerances.  q, k, v and the weights p are taken in two fp16 pieces of the
+value times a power of two that brings the row's largest one (p: 1) to 2^14
+or more: a piece pair is off by at most 2^-22 of the value, or, where the
+second piece is below fp16's normal range, by half of its smallest step,
+2^-25 / 2^14 = 2^-39 of the row's largest value.  A score is then off by at most
+  delta = ((2^-21 + hd 2^-23) sum_d |q_d k_d| + 2^-38 hd max|q| max|k|) / sqrt(hd),
+of hd additions each by one whole fp32 step (2^-23; the tensor cores may cut
+off instead of rounding), a weight by a factor e^(2 delta), and an output by
+  (2 delta + 2^-20 + steps 2^-23) sum_t w_t |v_t| + 2^-37 sum_t max_d |v_t|
+with 2^-20 for exp (2 steps), the pieces of p and v (2^-22 each) and the
+division, and one step for each addition in a row: at most n / 4 + 64 (a warp
+adds every fourth key; partial sums of tiles and slices are fewer).  The last
+term is p's 2^-39 with each key's value and v's 2^-39 with a weight of at most
+1; it also covers weights and products below fp32's range (2^-126).  Codes,
+scales, tables and lengths are exact.
+"""
+import ctypes
+
+import numpy as np
+import pytest
+
+import mlb
+
+pytestmark = pytest.mark.gpu
+
+
+def dev(a, device):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a)).to(device)
+
+
+def offsets_of(lens):
+    return np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+
+
+def delta_of(q, k):
+    """How far a score of q against the keys k may be off."""
+    hd = len(q)
+    near = (2.0 ** -21 + hd * 2.0 ** -23) * (np.abs(k) @ np.abs(q)).max()
+    return (near + 2.0 ** -38 * hd * np.abs(q).max() * np.abs(k).max()) / np.sqrt(hd)
+
+
+def attend(q, k, v, sees):
+    """One head in 64 bits: q [n, hd], k, v [t, hd]; row r sees keys < sees[r].
+    Returns (out, tolerance, weights)."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    hd, t = q.shape[1], k.shape[0]
+    out, tol, w = np.zeros_like(q), np.zeros_like(q), np.zeros((len(q), t))
+    for r, n in enumerate(sees):
+        n = min(int(n), t)
+        if n <= 0:
+            continue
+        s = k[:n] @ q[r] / np.sqrt(hd)
+        delta = delta_of(q[r], k[:n])
+        e = np.exp(s - s.max())
+        e /= e.sum()
+        w[r, :n] = e
+        out[r] = e @ v[:n]
+        tol[r] = (2 * delta + 2.0 ** -20 + (n / 4 + 64) * 2.0 ** -23) * (e @ np.abs(v[:n]))
+        tol[r] += 2.0 ** -37 * np.abs(v[:n]).max(1).sum()
+    return out, tol, w
+
+
+def check(got, want, tol, what=""):
+    got = np.asarray(got, np.float64)
+    assert got.shape == want.shape, what
+    off = np.abs(got - want) - tol
+    assert np.all(off <= 0), f"{what}: {off.max():.2e} beyond a tolerance of {tol.flat[off.argmax()]:.2e}"
+
+
+# --- packed prompt attention ------------------------------------------------------------------
+
+def packed_reference(q, k, v, qo, ko):
+    rows, nh, hd = q.shape
+    group = nh // k.shape[1]
+    out, tol = np.zeros((rows, nh, hd)), np.zeros((rows, nh, hd))
+    for i in range(len(qo) - 1):
+        n, t = qo[i + 1] - qo[i], ko[i + 1] - ko[i]
+        for h in range(nh):
+            a, b, _ = attend(q[qo[i]:qo[i + 1], h], k[ko[i]:ko[i + 1], h // group],
+                             v[ko[i]:ko[i + 1], h // group], t - n + 1 + np.arange(n))
+            out[qo[i]:qo[i + 1], h], tol[qo[i]:qo[i + 1], h] = a, b
+    return out, tol
+
+
+def packed_inputs(rng, lens, keys, nh, nkv, hd, spread=1.0):
+    qo, ko = offsets_of(lens), offsets_of(keys)
+    q = (rng.standard_normal((qo[-1], nh, hd)) * spread).astype(np.float32)
+    k = rng.standard_normal((ko[-1], nkv, hd)).astype(np.float32)
+    v = rng.standard_normal((ko[-1], nkv, hd)).astype(np.float32)
+    return q, k, v, qo, ko
+
+
+PACKED = [
+    # heads, kv heads, head size, query rows, keys (None: the same)
+    (4, 2, 64, [1], None),
+    (14, 2, 64, [1, 40, 0, 17], None),
+    (32, 8, 128, [33, 1, 127, 128, 129], None),
+    (28, 4, 128, [100, 5, 64], [300, 5, 1000]),       # after earlier tokens
+    (8, 1, 64, [257, 3], [257, 514]),                  # group 8
+    (6, 2, 128, [50, 21], None),                       # group 3
+    (10, 2, 64, [60, 0, 1], [61, 7, 200]),             # group 5, an empty sequence with keys
+    (12, 2, 128, [40, 30], None),                      # group 6
+    (4, 4, 128, [300], None),                          # group 1
+    (8, 4, 32, [40, 70], [44, 70]),                    # head sizes without a special form
+    (8, 2, 96, [20, 1], None),
+    (2, 1, 4, [5, 9], None),
+    (4, 2, 256, [30, 2], [30, 90]),
+    (8, 2, 64, [20, 9], [10, 9]),                      # rows that see no key
+    (8, 2, 128, [5, 200, 3], [0, 150, 3]),
+]
+
+
+@pytest.mark.parametrize("nh,nkv,hd,lens,keys", PACKED)
+def test_packed_attention(cuda, nh, nkv, hd, lens, keys):
+    rng = np.random.default_rng(nh * 100 + hd)
+    q, k, v, qo, ko = packed_inputs(rng, lens, lens if keys is None else keys, nh, nkv, hd)
+    want, tol = packed_reference(q, k, v, qo, ko)
+    got = mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(qo, cuda),
+                               None if keys is None else dev(ko, cuda))
+    check(got.cpu().numpy(), want, tol)
+    assert mlb.wait_timeouts() == 0
+
+
+@pytest.mark.parametrize("spread", [0.0, 6.0, 12.0])
+@pytest.mark.parametrize("scale", [1.0, 1e-18, 1e12])
+def test_packed_attention_wide_values(cuda, spread, scale):
+    """Peaked softmax rows, and values far from 1 (q small where k is large:
+    the scores stay, the pieces' scales do not)."""
+    rng = np.random.default_rng(int(spread) + 5)
+    q, k, v, qo, ko = packed_inputs(rng, [150, 70], [150, 400], 8, 2, 128, spread)
+    k[:, :, :4] *= np.linspace(0.1, 3.0, len(k), dtype=np.float32)[:, None, None]
+    q, k, v = q / np.float32(scale), k * np.float32(scale), v * np.float32(scale)
+    want, tol = packed_reference(q, k, v, qo, ko)
+    got = mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(qo, cuda),
+                               dev(ko, cuda))
+    check(got.cpu().numpy(), want, tol)
+
+
+def test_packed_attention_values_of_different_size(cuda):
+    """Neighbouring keys whose values differ by powers of ten: an output's
+    tolerance follows the weights, so no key may be lost beside a larger one."""
+    rng = np.random.default_rng(3)
+    q, k, v, qo, ko = packed_inputs(rng, [200, 40], [200, 90], 8, 2, 128)
+    v *= (10.0 ** rng.uniform(-3, 3, v.shape[0])).astype(np.float32)[:, None, None]
+    v[:, :, ::7] = 0
+    want, tol = packed_reference(q, k, v, qo, ko)
+    got = mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(qo, cuda),
+                               dev(ko, cuda))
+    check(got.cpu().numpy(), want, tol)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 96])
+def test_packed_attention_does_not_look_past_its_keys(cuda, hd):
+    """NaN and Inf in later keys, in other sequences' keys and in rows between
+    the sequences reach no row that does not see them; rows outside every
+    sequence stay as they were."""
+    import torch
+    rng = np.random.default_rng(8)
+    nh, nkv = 8, 2
+    qo, ko = np.array([3, 150, 150, 190], np.int32), np.array([5, 152, 160, 200], np.int32)
+    q = rng.standard_normal((200, nh, hd)).astype(np.float32)
+    k = rng.standard_normal((220, nkv, hd)).astype(np.float32)
+    v = rng.standard_normal((220, nkv, hd)).astype(np.float32)
+    want, tol = packed_reference(q, k, v, qo, ko)
+    for x in (k, v):
+        x[:5] = np.nan
+        x[152:160] = np.inf
+        x[200:] = np.nan
+        x[151] = np.nan       # seen by the last row of sequence 0 only
+    q[:3], q[190:] = np.nan, np.inf
+    out = torch.full((200, nh, hd), 7.0, device=cuda)
+    mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(qo, cuda), dev(ko, cuda),
+                         out=out)
+    got = out.cpu().numpy()
+    assert np.all(got[:3] == 7.0) and np.all(got[190:] == 7.0)
+    assert np.isnan(got[149]).all()
+    keep = np.r_[3:149, 150:190]
+    check(got[keep], want[keep], tol[keep])
+
+
+def test_packed_attention_equals_rows_of_one_sequence(cuda):
+    """One sequence is mlb_attention_rows_f32 over its cache."""
+    rng = np.random.default_rng(9)
+    q, k, v, qo, ko = packed_inputs(rng, [160], [400], 16, 4, 128)
+    one = mlb.attention_rows(dev(q, cuda), dev(k, cuda), dev(v, cuda), 240).cpu().numpy()
+    got = mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(qo, cuda),
+                               dev(ko, cuda)).cpu().numpy()
+    _, tol = packed_reference(q, k, v, qo, ko)
+    check(got, one.astype(np.float64), 2 * tol)
+
+
+@pytest.mark.parametrize("qo,ko", [
+    ([0, 50, 40, 60], [0, 50, 60, 60]),      # runs backwards
+    ([0, 20, 70, 60], [0, 20, 60, 60]),      # leaves the rows
+    ([-4, 20, 40, 60], [0, 20, 40, 60]),
+    ([0, 20, 40, 60], [0, 20, 90, 60])])     # leaves the keys
+def test_packed_attention_bad_ranges(cuda, qo, ko):
+    """Sequences with a bad range are left out and reported; the others are
+    computed.  (Ranges that run backwards let two sequences claim a row: what
+    such a row gets is not said.)"""
+    import torch
+    rng = np.random.default_rng(10)
+    nh, nkv, hd, rows = 8, 2, 64, 60
+    q = rng.standard_normal((rows, nh, hd)).astype(np.float32)
+    k = rng.standard_normal((rows, nkv, hd)).astype(np.float32)
+    qo, ko = np.array(qo, np.int32), np.array(ko, np.int32)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = torch.full((rows, nh, hd), 7.0, device=cuda)
+    mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(k, cuda), dev(qo, cuda), dev(ko, cuda),
+                         out=out, status=status)
+    assert mlb.status_check(status) == mlb.STATUS_BAD_LENGTH
+    got = out.cpu().numpy()
+    good = [i for i in range(3)
+            if 0 <= qo[i] <= qo[i + 1] <= rows and 0 <= ko[i] <= ko[i + 1] <= rows]
+    claims = np.zeros(rows, int)
+    for i in good:
+        claims[qo[i]:qo[i + 1]] += 1
+    for i in good:
+        want, tol = packed_reference(q, k, k, qo[i:i + 2], ko[i:i + 2])
+        mine = (np.arange(rows) >= qo[i]) & (np.arange(rows) < qo[i + 1]) & (claims == 1)
+        check(got[mine], want[mine], tol[mine])
+    assert np.all(got[claims == 0] == 7.0)
+
+
+# --- the 8-bit cache --------------------------------------------------------------------------
+
+def make_pool(rng, n_blocks, nkv, block, hd):
+    k = np.clip(np.round(rng.standard_normal((n_blocks, nkv, block, hd)) * 36), -127, 127)
+    v = np.clip(np.round(rng.standard_normal((n_blocks, nkv, hd, block)) * 36), -127, 127)
+    scales = [np.exp(rng.standard_normal((n_blocks, nkv)) * 0.5).astype(np.float32) * np.float32(0.03)
+              for _ in range(2)]
+    return [k.astype(np.int8), v.astype(np.int8), *scales]
+
+
+def make_table(rng, needed, n_blocks, extra=1):
+    ids = rng.permutation(n_blocks)[:sum(needed)].astype(np.int32)
+    table = np.full((len(needed), max(needed) + extra), -1, np.int32)
+    at = 0
+    for i, n in enumerate(needed):
+        table[i, :n] = ids[at:at + n]
+        at += n
+    return table
+
+
+def to_device(pool, cuda):
+    return mlb.Kv8Cache(*[dev(x, cuda) for x in pool])
+
+
+def half_even(x, by):
+    """round(x / by): the quotient of two fp32 values (or of an 8-bit code's
+    product with one) that is no tie is further from one than 2^-53 of it."""
+    with np.errstate(divide="ignore", invalid="ignore"):
+        return np.clip(np.rint(np.where(by > 0, np.asarray(x, np.float64) / by, 0.0)), -127, 127)
+
+
+def write_reference(pool, table, k, v, offsets, positions, block):
+    """The definition, block by block, on copies of the pool."""
+    pool = [x.copy() for x in pool]
+    n_blocks = len(pool[0])
+    for which, x in ((0, k), (1, v)):
+        codes = pool[which] if which == 0 else pool[which].transpose(0, 1, 3, 2)
+        scales = pool[2 + which]
+        for i in range(len(positions)):
+            at, end = int(positions[i]), int(positions[i]) + int(offsets[i + 1] - offsets[i])
+            if end == at:
+                continue
+            for c in range(at // block, (end - 1) // block + 1):
+                if c >= table.shape[1] or not 0 <= table[i, c] < n_blocks:
+                    continue
+                b = table[i, c]
+                old = max(0, at - c * block)
+                lo, hi = max(at, c * block), min(end, (c + 1) * block)
+                new = x[offsets[i] + lo - at:offsets[i] + hi - at].transpose(1, 0, 2)
+                scale = (np.abs(new).max((1, 2)).astype(np.float64) / 127).astype(np.float32)
+                had = scales[b].copy()
+                if old:
+                    scale = np.maximum(scale, had)
+                by = scale.astype(np.float64)[:, None, None]
+                moved = codes[b][:, :old].astype(np.float64) * had[:, None, None].astype(np.float64)
+                codes[b][:, :old] = half_even(moved, by)
+                codes[b][:, old:old + hi - lo] = half_even(new, by)
+                codes[b][:, old + hi - lo:] = 0
+                scales[b] = scale
+    return pool
+
+
+WRITES = [
+    # kv heads, head size, block, new rows, earlier tokens
+    (2, 64, 32, [1], [0]),
+    (8, 128, 32, [1, 1, 1, 1], [0, 31, 32, 45]),
+    (2, 128, 64, [5, 0, 130, 64], [62, 7, 3, 64]),
+    (4, 32, 128, [300, 1, 128], [0, 127, 5]),
+    (1, 256, 128, [140, 9], [100, 0]),
+    (3, 96, 32, [33, 32, 31, 95], [0, 0, 1, 20]),
+]
+
+
+@pytest.mark.parametrize("nkv,hd,block,lens,before", WRITES)
+def test_kv8_write_and_read(cuda, nkv, hd, block, lens, before):
+    import torch
+    rng = np.random.default_rng(nkv * 10 + block)
+    needed = [-(-(a + b) // block) for a, b in zip(lens, before)]
+    n_blocks = sum(needed) + 2
+    pool, table = make_pool(rng, n_blocks, nkv, block, hd), make_table(rng, needed, n_blocks)
+    offsets, positions = offsets_of(lens), np.array(before, np.int32)
+    rows = int(offsets[-1])
+    # one scale grows past the earlier tokens', another stays below
+    k = (rng.standard_normal((rows, nkv, hd)) * 4).astype(np.float32)
+    v = (rng.standard_normal((rows, nkv, hd)) * 0.5).astype(np.float32)
+    want = write_reference(pool, table, k, v, offsets, positions, block)
+    cache = to_device(pool, cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    args = (cache, dev(table, cuda), dev(k, cuda), dev(v, cuda), dev(offsets, cuda),
+            dev(positions, cuda))
+    for _ in range(2):  # the second call changes nothing
+        mlb.kv8_write(*args, status=status)
+        for got, x in zip(cache, want):
+            assert np.array_equal(got.cpu().numpy(), x)
+    # everything that the sequences hold now
+    total = [a + b for a, b in zip(lens, before)]
+    ro = offsets_of(total)
+    kr, vr = mlb.kv8_read(cache, dev(table, cuda), dev(ro, cuda),
+                          dev(np.zeros(len(lens), np.int32), cuda), int(ro[-1]), status=status)
+    assert mlb.status_check(status) == 0
+    for i, n in enumerate(total):
+        t = np.arange(n)
+        b = table[i, t // block]
+        assert np.array_equal(kr[ro[i]:ro[i + 1]].cpu().numpy(),
+                              want[0][b, :, t % block] * want[2][b][:, :, None])
+        assert np.array_equal(vr[ro[i]:ro[i + 1]].cpu().numpy(),
+                              want[1][b, :, :, t % block] * want[3][b][:, :, None])
+
+
+@pytest.mark.parametrize("with_nan", [True, False])
+def test_kv8_write_halves_zeros_and_tiny_values(cuda, with_nan):
+    """Quotients that lie on a half or next to one (or NaN where they would lie
+    on one), blocks of zeros and values so small that their scale is
+    subnormal or 0."""
+    nkv, hd, block = 4, 64, 32
+    rng = np.random.default_rng(12)
+    pool, table = make_pool(rng, 1, nkv, block, hd), np.zeros((1, 1), np.int32)
+    x = np.zeros((32, nkv, hd), np.float32)
+    scale = np.float32(0.3)
+    halves = (np.arange(32 * hd) % 253 - 126.5).astype(np.float32) * scale
+    side = np.tile(np.array([-np.inf, np.nan, np.inf], np.float32), 32 * hd)[:32 * hd]
+    if not with_nan:
+        side = np.where(np.isnan(side), halves, side)
+    x[:, 0] = np.nextafter(halves, side).reshape(32, hd)
+    x[0, 0, 0] = scale * np.float32(127)
+    x[:, 1] = 0
+    x[:, 2] = rng.integers(-300, 300, (32, hd)).astype(np.float32) * np.float32(1e-45)
+    x[:, 3] = rng.standard_normal((32, hd)).astype(np.float32) * np.float32(1e-36)
+    offsets, positions = np.array([0, 32], np.int32), np.zeros(1, np.int32)
+    want = write_reference(pool, table, x, x[::-1].copy(), offsets, positions, block)
+    cache = to_device(pool, cuda)
+    mlb.kv8_write(cache, dev(table, cuda), dev(x, cuda), dev(x[::-1].copy(), cuda),
+                  dev(offsets, cuda), dev(positions, cuda))
+    for got, w in zip(cache, want):
+        assert np.array_equal(got.cpu().numpy(), w, equal_nan=w.dtype.kind == "f")
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_kv8_write_not_finite(cuda, bad):
+    """A block that receives Inf or NaN reads as NaN, the others are untouched."""
+    rng = np.random.default_rng(13)
+    nkv, hd, block = 2, 64, 32
+    pool = make_pool(rng, 3, nkv, block, hd)
+    table = np.array([[2, 0]], np.int32)
+    k = rng.standard_normal((40, nkv, hd)).astype(np.float32)
+    v = k.copy()
+    k[5, 1, 3] = bad
+    v[39, 0, 0] = bad
+    cache = to_device(pool, cuda)
+    o, p = np.array([0, 40], np.int32), np.zeros(1, np.int32)
+    mlb.kv8_write(cache, dev(table, cuda), dev(k, cuda), dev(v, cuda), dev(o, cuda), dev(p, cuda))
+    kr, vr = (x.cpu().numpy() for x in
+              mlb.kv8_read(cache, dev(table, cuda), dev(o, cuda), dev(p, cuda), 40))
+    assert np.isnan(kr[:32, 1]).all() and np.isfinite(kr[:, 0]).all() and np.isfinite(kr[32:]).all()
+    assert np.isnan(vr[32:, 0]).all() and np.isfinite(vr[:, 1]).all() and np.isfinite(vr[:32]).all()
+
+
+def test_kv8_write_and_read_bad_places(cuda):
+    """Bad ids, positions outside the table and bad row ranges are reported and
+    skipped; the other blocks are written; reading gives zeros there."""
+    import torch
+    rng = np.random.default_rng(14)
+    nkv, hd, block, n_blocks = 2, 64, 32, 8
+    pool = make_pool(rng, n_blocks, nkv, block, hd)
+    table = np.array([[0, 99, 1], [2, -7, -1], [3, 4, 5], [6, 7, -1]], np.int32)
+    lens, before = [90, 40, 70, 5], [0, 0, 60, -3]
+    offsets, positions = offsets_of(lens), np.array(before, np.int32)
+    rows = int(offsets[-1])
+    k = rng.standard_normal((rows, nkv, hd)).astype(np.float32)
+    v = rng.standard_normal((rows, nkv, hd)).astype(np.float32)
+    want = write_reference(pool, table[:3], k, v, offsets[:4], positions[:3], block)
+    cache = to_device(pool, cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    mlb.kv8_write(cache, dev(table, cuda), dev(k, cuda), dev(v, cuda), dev(offsets, cuda),
+                  dev(positions, cuda), status=status)
+    assert mlb.status_check(status) == mlb.STATUS_BAD_BLOCK | mlb.STATUS_BAD_POSITION
+    for got, x in zip(cache, want):
+        assert np.array_equal(got.cpu().numpy(), x)
+    status.zero_()
+    kr, vr = (x.cpu().numpy() for x in
+              mlb.kv8_read(cache, dev(table, cuda), dev(offsets, cuda), dev(positions, cuda), rows,
+                           status=status))
+    assert mlb.status_check(status) == mlb.STATUS_BAD_BLOCK | mlb.STATUS_BAD_POSITION
+    for x in (kr, vr):
+        assert np.all(x[32:64] == 0) and np.any(x[64:90] != 0)        # block 99 of sequence 0
+        assert np.all(x[122:130] == 0) and np.any(x[90:122] != 0)     # block -7 of sequence 1
+        assert np.all(x[130 + 36:200] == 0) and np.any(x[130:166] != 0)
+        assert np.all(x[200:] == 0)                                   # negative positions
+    # ranges that run backwards or leave the rows
+    bad = np.array([0, 10, 5, 9999, 20], np.int32)
+    status.zero_()
+    cache = to_device(pool, cuda)
+    mlb.kv8_write(cache, dev(np.array([[0], [1], [2], [3]], np.int32), cuda), dev(k[:20], cuda),
+                  dev(v[:20], cuda), dev(bad, cuda), dev(np.zeros(4, np.int32), cuda), status=status)
+    assert mlb.status_check(status) == mlb.STATUS_BAD_LENGTH
+    want = write_reference(pool, np.array([[0]], np.int32), k[:10], v[:10], [0, 10], [0], block)
+    for got, x in zip(cache, want):
+        assert np.array_equal(got.cpu().numpy(), x)
+
+
+def decode_reference(q, pool, table, lengths, block, mass_in=None):
+    n, nh, hd = q.shape
+    nkv = pool[0].shape[1]
+    group = nh // nkv
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    mass = np.zeros(table.shape) if mass_in is None else mass_in.astype(np.float64)
+    mass_tol = np.abs(mass) * 2.0 ** -23
+    for i, length in enumerate(lengths):
+        if length <= 0:
+            continue
+        t = np.arange(length)
+        ids = table[i, t // block]
+        for h in range(nh):
+            kv = h // group
+            k = pool[0][ids, kv, t % block] * pool[2][ids, kv].astype(np.float64)[:, None]
+            v = pool[1][ids, kv, :, t % block] * pool[3][ids, kv].astype(np.float64)[:, None]
+            a, b, w = attend(q[i, h][None], k, v, [length])
+            out[i, h], tol[i, h] = a[0], b[0]
+            delta = delta_of(q[i, h].astype(np.float64), k)
+            each = np.bincount(t // block, w[0], table.shape[1])
+            mass[i] += each
+            # weights (one that underflows loses 2^-126), and one step for each
+            # of the heads' and units' sums
+            mass_tol[i] += block * 2.0 ** -126
+            mass_tol[i] += each * (2 * delta + 2.0 ** -20 + (length / 4 + 64) * 2.0 ** -23)
+            mass_tol[i] += (nh + 4) * 2.0 ** -23 * each
+    return out, tol, mass, mass_tol + np.abs(mass) * 2.0 ** -23
+
+
+DECODES = [
+    # heads, kv heads, head size, block, lengths
+    (14, 2, 64, 32, [1]),
+    (14, 2, 64, 32, [511]),
+    (32, 8, 128, 32, [0, 1, 31, 32, 33, 0, 700, 64]),
+    (32, 32, 128, 64, [100, 2047, 1]),
+    (28, 4, 128, 128, [129, 5, 1000]),
+    (8, 1, 256, 32, [77, 300]),
+    (6, 2, 96, 64, [65, 64, 200]),
+    (10, 2, 32, 32, [3000, 9]),
+    (12, 2, 192, 32, [50]),
+    (16, 2, 160, 64, [90, 12]),
+    (8, 8, 224, 32, [70]),
+    (8, 2, 128, 32, [0]),
+    (64, 8, 128, 32, [9000]),
+    (8, 2, 64, 32, [i % 70 for i in range(300)]),       # more sequences than CTA threads
+]
+
+
+@pytest.mark.parametrize("with_mass", [False, True])
+@pytest.mark.parametrize("nh,nkv,hd,block,lengths", DECODES)
+def test_attention_kv8(cuda, nh, nkv, hd, block, lengths, with_mass):
+    import torch
+    rng = np.random.default_rng(nh + hd + block)
+    needed = [-(-n // block) for n in lengths]
+    n_blocks = sum(needed) + 2
+    pool, table = make_pool(rng, n_blocks, nkv, block, hd), make_table(rng, needed, n_blocks)
+    q = rng.standard_normal((len(lengths), nh, hd)).astype(np.float32)
+    mass_in = rng.random(table.shape).astype(np.float32)
+    # what is behind a sequence's last token is never used
+    for i, n in enumerate(lengths):
+        if n % block:
+            b = table[i, n // block]
+            pool[0][b, :, n % block:], pool[1][b, :, :, n % block:] = -128, 127
+    for x in pool[2:]:
+        x[np.setdiff1d(np.arange(n_blocks), table)] = np.nan
+    want, tol, mass, mass_tol = decode_reference(q, pool, table, lengths, block, mass_in)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    cache = to_device(pool, cuda)
+    mass_out = torch.full(table.shape, 9.0, device=cuda) if with_mass else None
+    args = (dev(q, cuda), cache, dev(table, cuda), dev(np.array(lengths, np.int32), cuda))
+    got = mlb.attention_kv8(*args, mass_in=dev(mass_in, cuda) if with_mass else None,
+                            mass_out=mass_out, status=status)
+    assert mlb.status_check(status) == 0
+    check(got.cpu().numpy(), want, tol, "out")
+    if with_mass:
+        check(mass_out.cpu().numpy(), mass, mass_tol, "mass")
+        # in place, and without an input
+        again = dev(mass_in, cuda)
+        second = mlb.attention_kv8(*args, mass_in=again, mass_out=again)
+        assert torch.equal(again, mass_out) and torch.equal(second, got)
+        mlb.attention_kv8(*args, mass_out=again)
+        _, _, alone, alone_tol = decode_reference(q, pool, table, lengths, block)
+        check(again.cpu().numpy(), alone, alone_tol, "mass alone")
+    assert mlb.wait_timeouts() == 0
+
+
+@pytest.mark.parametrize("spread,vscale", [(4.0, 1.0), (10.0, 1e-12), (0.0, 1e9), (3.0, 1e30)])
+def test_attention_kv8_wide_values(cuda, spread, vscale):
+    """Peaked rows; blocks whose scales differ by orders of magnitude; queries
+    with one large dimension."""
+    rng = np.random.default_rng(21)
+    nh, nkv, hd, block, lengths = 16, 4, 128, 32, [640, 97]
+    needed = [-(-n // block) for n in lengths]
+    pool, table = make_pool(rng, 30, nkv, block, hd), make_table(rng, needed, 30)
+    pool[2] *= (10.0 ** rng.uniform(-3, 0, pool[2].shape)).astype(np.float32)
+    pool[3] *= (10.0 ** rng.uniform(-4, 0, pool[3].shape)).astype(np.float32) * np.float32(vscale)
+    q = (rng.standard_normal((2, nh, hd)) * spread).astype(np.float32)
+    q[:, :, 5] *= 100
+    q[0, 3] *= np.float32(1e-20)
+    q[0, 4] = 0
+    want, tol, mass, mass_tol = decode_reference(q, pool, table, lengths, block)
+    import torch
+    mass_out = torch.empty(table.shape, device=cuda)
+    got = mlb.attention_kv8(dev(q, cuda), to_device(pool, cuda), dev(table, cuda),
+                            dev(np.array(lengths, np.int32), cuda), mass_out=mass_out)
+    check(got.cpu().numpy(), want, tol, "out")
+    check(mass_out.cpu().numpy(), mass, mass_tol, "mass")
+
+
+def test_attention_kv8_not_finite(cuda):
+    """Inf or NaN in a seen block or a query reaches that sequence's (and
+    head's) output as NaN and no other."""
+    rng = np.random.default_rng(22)
+    nh, nkv, hd, block = 8, 2, 64, 32
+    lengths = [100, 70, 300]
+    needed = [-(-n // block) for n in lengths]
+    pool, table = make_pool(rng, 20, nkv, block, hd), make_table(rng, needed, 20)
+    q = rng.standard_normal((3, nh, hd)).astype(np.float32)
+    want, tol, _, _ = decode_reference(q, pool, table, lengths, block)
+    pool[2][table[0, 1], 1] = np.nan
+    pool[3][table[1, 0], 0] = np.inf
+    q[2, 3, 7] = np.inf
+    q[2, 5, 0] = np.nan
+    got = mlb.attention_kv8(dev(q, cuda), to_device(pool, cuda), dev(table, cuda),
+                            dev(np.array(lengths, np.int32), cuda)).cpu().numpy()
+    lost = np.zeros((3, nh), bool)
+    lost[0, 4:] = lost[1, :4] = True
+    lost[2, 3] = lost[2, 5] = True
+    assert not np.isfinite(got[lost]).any()
+    check(got[~lost], want[~lost], tol[~lost])
+
+
+def test_attention_kv8_bad_lengths_and_blocks(cuda):
+    """A sequence with a bad length or block gives zeros, collects nothing and
+    is reported; the others are computed."""
+    import torch
+    rng = np.random.default_rng(23)
+    nh, nkv, hd, block = 8, 2, 128, 32
+    lengths = [100, 2000, -1, 500, 64]
+    table = make_table(rng, [4, 4, 4, 16, 2], 40)
+    pool = make_pool(rng, 40, nkv, block, hd)
+    q = rng.standard_normal((5, nh, hd)).astype(np.float32)
+    good = [100, 0, 0, 0, 64]
+    mass_in = rng.random(table.shape).astype(np.float32)
+    want, tol, mass, mass_tol = decode_reference(q, pool, table, good, block, mass_in)
+    for bad_id in (40, -1, 2 ** 31 - 1, -2 ** 31):
+        t = table.copy()
+        t[3, 9] = bad_id
+        status = torch.zeros(1, dtype=torch.int32, device=cuda)
+        mass_out = torch.empty(table.shape, device=cuda)
+        got = mlb.attention_kv8(dev(q, cuda), to_device(pool, cuda), dev(t, cuda),
+                                dev(np.array(lengths, np.int32), cuda), mass_in=dev(mass_in, cuda),
+                                mass_out=mass_out, status=status)
+        assert mlb.status_check(status) == mlb.STATUS_BAD_LENGTH | mlb.STATUS_BAD_BLOCK
+        check(got.cpu().numpy(), want, tol)
+        check(mass_out.cpu().numpy(), mass, mass_tol)
+
+
+# --- eviction ---------------------------------------------------------------------------------
+
+def evict_reference(table, lengths, mass, block, keep, sink, recent):
+    t, m = np.full_like(table, -1), np.zeros_like(mass)
+    freed, left = np.full_like(table, -1), np.array(lengths, np.int32)
+    for i, n in enumerate(lengths):
+        blocks = -(-int(n) // block)
+        key = [(np.inf if np.isnan(x) else float(x), bool(np.isnan(x))) for x in mass[i]]
+        order = sorted(range(sink, max(sink, blocks - recent)), key=lambda c: (*key[c], c))
+        gone = sorted(order[:max(0, blocks - keep)])
+        stays = [c for c in range(blocks) if c not in set(gone)]
+        t[i, :len(stays)], m[i, :len(stays)] = table[i, stays], mass[i, stays]
+        freed[i, :len(gone)] = table[i, gone]
+        left[i] -= block * len(gone)
+    return t, left, m, freed
+
+
+EVICTS = [
+    # columns, block, lengths, keep, sink, recent
+    (1, 32, [0, 1, 32], 1, 0, 1),
+    (10, 32, [320, 300, 289, 0, 33], 4, 1, 2),
+    (10, 64, [640, 600], 10, 1, 1),
+    (90, 32, [2880, 2000], 64, 0, 1),
+    (1024, 32, [1024 * 32, 1023 * 32 + 1], 300, 2, 8),
+    (2500, 128, [2500 * 128, 1200 * 128, 5], 700, 1, 4),
+    (40, 32, [40 * 32], 2, 1, 1),
+]
+
+
+@pytest.mark.parametrize("cols,block,lengths,keep,sink,recent", EVICTS)
+@pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
+def test_evict(cuda, cols, block, lengths, keep, sink, recent, kind):
+    import torch
+    rng = np.random.default_rng(cols + keep)
+    n = len(lengths)
+    table = rng.permutation(n * cols).astype(np.int32).reshape(n, cols)
+    mass = np.exp(rng.standard_normal((n, cols)) * 3).astype(np.float32)
+    if kind == "ties":
+        mass = np.round(rng.random((n, cols)) * 3).astype(np.float32)
+        mass[rng.random((n, cols)) < 0.2] = -0.0
+    elif kind == "odd":
+        mass = rng.standard_normal((n, cols)).astype(np.float32)
+        for value in (np.nan, np.inf, -np.inf, 1e-45, -1e-45):
+            mass[rng.random((n, cols)) < 0.05] = value
+    want = evict_reference(table, lengths, mass, block, keep, sink, recent)
+    args = [dev(table, cuda), dev(np.array(lengths, np.int32), cuda), dev(mass, cuda)]
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    got = mlb.kv8_evict(*args, block, keep, sink, recent, status=status)
+    assert mlb.status_check(status) == 0
+    for g, w in zip(got, want):
+        assert np.array_equal(g.cpu().numpy(), w, equal_nan=w.dtype.kind == "f")
+    # in place, without a list of what left
+    lib = mlb.load()
+    p = [ctypes.c_void_p(x.data_ptr()) for x in args]
+    assert lib.mlb_kv8_evict(p[0], cols, p[1], p[2], n, block, keep, sink, recent, p[0], p[1],
+                             p[2], None, None,
+                             ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    for g, w in zip(args, want):
+        assert np.array_equal(g.cpu().numpy(), w, equal_nan=w.dtype.kind == "f")
+
+
+def test_evict_bad_length(cuda):
+    import torch
+    rng = np.random.default_rng(30)
+    table = rng.permutation(30).astype(np.int32).reshape(3, 10)
+    mass = rng.random((3, 10)).astype(np.float32)
+    lengths = np.array([-5, 320, 321], np.int32)
+    want = evict_reference(table, [0, 320, 0], mass, 32, 4, 1, 1)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    t, n, m, freed = (x.cpu().numpy() for x in
+                      mlb.kv8_evict(dev(table, cuda), dev(lengths, cuda), dev(mass, cuda), 32, 4,
+                                    status=status))
+    assert mlb.status_check(status) == mlb.STATUS_BAD_LENGTH
+    for i in (0, 2):
+        assert np.array_equal(t[i], table[i]) and np.array_equal(m[i], mass[i])
+        assert n[i] == lengths[i] and np.all(freed[i] == -1)
+    assert np.array_equal(t[1], want[0][1]) and n[1] == want[1][1]
+
+
+# --- together ---------------------------------------------------------------------------------
+
+def test_serving_loop(cuda):
+    """Prompts of several sequences, then decode steps with collected weights,
+    an eviction and more steps: as a server would call them, against the same
+    run in 64 bits on a cache of the same codes."""
+    import torch
+    rng = np.random.default_rng(40)
+    nh, nkv, hd, block = 8, 2, 64, 32
+    lens = [70, 1, 33, 200]
+    cols, n_blocks = 10, 40
+    table = rng.permutation(n_blocks).astype(np.int32).reshape(4, cols)
+    pool = make_pool(rng, n_blocks, nkv, block, hd)
+    cache, table_d = to_device(pool, cuda), dev(table, cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    q, k, v, offsets, _ = packed_inputs(rng, lens, lens, nh, nkv, hd)
+    zeros = np.zeros(4, np.int32)
+    out = mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(offsets, cuda),
+                               status=status)
+    want, tol = packed_reference(q, k, v, offsets, offsets)
+    check(out.cpu().numpy(), want, tol)
+    mlb.kv8_write(cache, table_d, dev(k, cuda), dev(v, cuda), dev(offsets, cuda), dev(zeros, cuda),
+                  status=status)
+    pool = write_reference(pool, table, k, v, offsets, zeros, block)
+    lengths, mass_d = np.array(lens, np.int32), torch.zeros((4, cols), device=cuda)
+    lengths_d = dev(lengths, cuda)
+    mass, mass_tol = np.zeros((4, cols), np.float32), np.zeros((4, cols))
+    one = np.arange(5, dtype=np.int32)
+    for step in range(6):
+        if step == 4:
+            before = mass_d.cpu().numpy()
+            table_d, lengths_d, mass_d, _ = mlb.kv8_evict(table_d, lengths_d, mass_d, block, 5,
+                                                          sink_blocks=1, recent_blocks=2)
+            table, lengths, mass, freed = evict_reference(table, lengths, before, block, 5, 1, 2)
+            assert np.array_equal(table_d.cpu().numpy(), table)
+            assert np.array_equal(lengths_d.cpu().numpy(), lengths)
+            assert np.array_equal(mass_d.cpu().numpy(), mass) and (freed >= 0).sum() == 2
+            mass_tol = np.zeros((4, cols))
+        q, k, v, _, _ = packed_inputs(rng, [4], [4], nh, nkv, hd)
+        mlb.kv8_write(cache, table_d, dev(k, cuda), dev(v, cuda), dev(one, cuda), lengths_d,
+                      status=status)
+        pool = write_reference(pool, table, k, v, one, lengths, block)
+        lengths_d, lengths = lengths_d + 1, lengths + 1
+        out = mlb.attention_kv8(dev(q, cuda), cache, table_d, lengths_d, mass_in=mass_d,
+                                mass_out=mass_d, status=status)
+        want, tol, mass64, one_tol = decode_reference(q, pool, table, lengths, block, mass)
+        mass_tol = mass_tol + one_tol
+        check(out.cpu().numpy(), want, tol)
+        check(mass_d.cpu().numpy(), mass64, mass_tol)
+        mass = mass64.astype(np.float32)
+        for got, x in zip(cache, pool):
+            assert np.array_equal(got.cpu().numpy(), x)
+    # the earlier tokens as keys of a later turn's packed attention
+    total = [int(n) + 8 for n in lengths]
+    qo, ko = offsets_of([8] * 4), offsets_of(total)
+    assert mlb.status_check(status) == 0
+    kr, vr = mlb.kv8_read(cache, table_d, dev(offsets_of(lengths), cuda), dev(zeros, cuda),
+                          int(sum(lengths)), status=status)
+    q, k, v, _, _ = packed_inputs(rng, [32], [32], nh, nkv, hd)
+    ro = offsets_of(lengths)
+    keys = np.concatenate([np.concatenate([kr[ro[i]:ro[i + 1]].cpu().numpy(), k[8 * i:8 * i + 8]])
+                           for i in range(4)])
+    vals = np.concatenate([np.concatenate([vr[ro[i]:ro[i + 1]].cpu().numpy(), v[8 * i:8 * i + 8]])
+                           for i in range(4)])
+    out = mlb.attention_packed(dev(q, cuda), dev(keys, cuda), dev(vals, cuda), dev(qo, cuda),
+                               dev(ko, cuda), status=status)
+    want, tol = packed_reference(q, keys, vals, qo, ko)
+    check(out.cpu().numpy(), want, tol)
+    assert mlb.status_check(status) == 0
+
+
+def test_batched_calls_on_a_stream_and_in_a_graph(cuda):
+    """Another stream than the current one; and a decode step captured once and
+    replayed with new inputs in the same buffers, beside a second graph."""
+    import torch
+    rng = np.random.default_rng(41)
+    nh, nkv, hd, block, lengths = 8, 2, 128, 32, [90, 300, 5]
+    needed = [-(-(n + 1) // block) for n in lengths]
+    pool, table = make_pool(rng, 20, nkv, block, hd), make_table(rng, needed, 20)
+    cache, table_d = to_device(pool, cuda), dev(table, cuda)
+    n_d = dev(np.array(lengths, np.int32), cuda)
+    q, k, v, _, _ = packed_inputs(rng, [3], [3], nh, nkv, hd)
+    side = torch.cuda.Stream()
+    qd, kd, vd, one = dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(np.arange(4, dtype=np.int32), cuda)
+    torch.cuda.synchronize()
+    out = mlb.attention_kv8(qd, cache, table_d, n_d, stream=side)
+    packed = mlb.attention_packed(qd, kd, vd, one, stream=side)
+    side.synchronize()
+    want, tol, _, _ = decode_reference(q, pool, table, lengths, block)
+    check(out.cpu().numpy(), want, tol)
+    want, tol = packed_reference(q, k, v, np.arange(4), np.arange(4))
+    check(packed.cpu().numpy(), want, tol)
+
+    def step(mass):
+        mlb.kv8_write(cache, table_d, kd, vd, one, n_d)
+        got = mlb.attention_kv8(qd, cache, table_d, n_d + 1, mass_in=mass, mass_out=mass)
+        return got, mlb.attention_packed(qd, kd, vd, one), mlb.kv8_evict(table_d, n_d, mass, block, 4)
+
+    masses = [torch.zeros(table.shape, device=cuda) for _ in range(2)]
+    step(masses[0])
+    torch.cuda.synchronize()
+    graphs, results = [], []
+    for m in masses:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            results.append(step(m))
+        graphs.append(g)
+    for turn in range(3):
+        q, k, v, _, _ = packed_inputs(rng, [3], [3], nh, nkv, hd)
+        for d, x in ((qd, q), (kd, k), (vd, v)):
+            d.copy_(dev(x, cuda))
+        before = [x.cpu().numpy() for x in cache]
+        masses[turn % 2].zero_()
+        graphs[turn % 2].replay()
+        torch.cuda.synchronize()
+        got, packed, evicted = results[turn % 2]
+        pool = write_reference(before, table, k, v, np.arange(4), lengths, block)
+        longer = [n + 1 for n in lengths]
+        want, tol, mass, mass_tol = decode_reference(q, pool, table, longer, block)
+        check(got.cpu().numpy(), want, tol)
+        check(masses[turn % 2].cpu().numpy(), mass, mass_tol)
+        want, tol = packed_reference(q, k, v, np.arange(4), np.arange(4))
+        check(packed.cpu().numpy(), want, tol)
+        want = evict_reference(table, lengths, masses[turn % 2].cpu().numpy(), block, 4, 1, 1)
+        for g, w in zip(evicted, want):
+            assert np.array_equal(g.cpu().numpy(), w)
