@@ -1,11 +1,38 @@
 // Decode attention of several sequences over the 8-bit KV cache.
 //
 //   out[i][h] = softmax_t(q[i][h] . k_t / sqrt(hd)) . v_t,  t < lengths[i]
-// with k_t, v_t = code * scale of the token's block (mlb_ops.h).  A unit is
-// 32 consecutive tokens; it lies in one block, so it has one scale for K and
-// one for V.  Online softmax over units; the weight that a block collects is
-// found afterwards from each unit's (sum p, reference max) and the heads'
-// final (M, L).
+// with k_t, v_t = code * scale of the token's block (mlb_ops.h).
+//
+// Work.  A unit is 32 consecutive tokens of one sequence and kv head: one
+// scale for K, one for V, 64 hd bytes of codes.  The units of all sequences
+// and kv heads, in that order, are dealt out evenly to the warps of a grid
+// that fills the GPU once; a warp walks its share and keeps an online softmax
+// for the group's heads.  A (sequence, kv head) that lies inside one warp's
+// share is finished there; otherwise each of its warps writes a partial
+// (reference max m, sum l, accumulator) and a second kernel joins them.  So
+// one long sequence and many short ones both keep every SM busy, whatever
+// the lengths, which only the device knows.
+//
+// Products.  Both run as mma.m16n8k16 (fp16 operands, fp32 sums) with the
+// 8-bit codes as exact fp16 numbers.  q, scaled per head by a power of two
+// that brings its largest value to [2^14, 2^15), and p, times 2^14, are split
+// into two fp16 pieces each (at most 2^-22 of the value is left, or 2^-39 of
+// the row's largest); the high pieces of up to 8 heads are the tile's rows
+// 0-7, the low ones its rows 8-15, so one MMA takes both and a thread holds
+// both sums of its (head, column).  The scales of a unit multiply its scores
+// and its weighted values in fp32; a unit's values are summed from zero and
+// then added to the running accumulator by one fp32 multiply-add.
+//
+// Layout.  Column n of score tile j is the unit's token 8 (n / 2) + 2 j +
+// n % 2: a thread (lane = 4 row + c) then holds the scores of tokens 8 c ..
+// 8 c + 7 of its head, which are its part of the second product's A operand as
+// they stand, and its V codes are 8 consecutive bytes of V's [hd][token]
+// rows.  K rows are stored in that column order with an odd pitch in units
+// of 32 bytes: the 8-byte reads of both products are free of bank
+// conflicts.  Codes travel by cp.async, kStages - 1 units ahead of the
+// products, each warp on its own.
+//
+// Bound: HBM reads of 2 hd bytes per token and kv head.
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -16,8 +43,10 @@ namespace mlb {
 namespace {
 
 constexpr int kUnit = 32;  // tokens
-constexpr int kA8Threads = 128;
+constexpr int kA8Warps = 4;
 constexpr int kA8MaxGroup = 8;
+constexpr int kPartHead = 4;  // a partial: m, l, bad, unused, acc[hd]
+constexpr float kPScale = 16384.0f;
 
 struct A8Args {
   const float* q;
@@ -28,101 +57,482 @@ struct A8Args {
   const int32_t* table;
   const int32_t* lengths;
   float* out;
-  float2* lse;    // [n_seqs][n_heads] (M, L); L = 0: no token or a bad sequence
-  float2* units;  // [n_seqs][unit columns][n_heads] (reference max, sum p), or null
+  float2* lse;     // [n_seqs][n_heads] (M, L), M in powers of two; L = 0: no
+                   // token or a bad sequence
+  float2* units;   // [n_seqs][unit columns][n_heads] (m, sum p), or null
+  float* partial;  // [warps of the grid][2][group][kPartHead + hd]
   int64_t n_blocks;
   int64_t table_cols;
   int n_seqs;
   int block;
+  int block_shift;  // log2
   int n_heads;
   int kv_heads;
   int hd;
-  float scale;
+  int group;
+  int workers;  // warps of the grid
+  float scale;  // log2(e) / sqrt(hd)
   int32_t* status;
 };
 
-// CTA = (kv head, sequence): unit by unit, scores by (head, token) thread,
-// weighted values by dimension thread.
-__global__ void __launch_bounds__(kA8Threads) A8Kernel(A8Args a) {
+// 2^x; results below fp32's normal range are 0.
+__device__ __forceinline__ float Exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void Mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                    uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+      " {%8, %9}, {%0, %1, %2, %3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four codes -> two fp16 pairs (codes 0, 1 and 2, 3), exact: with the sign bit
+// flipped a code is code + 128, 0x64 above it makes the fp16 number 1024 +
+// code + 128, and one packed subtraction leaves the code.
+__device__ __forceinline__ void CodePairs(uint32_t w, uint32_t& p0, uint32_t& p1) {
+  const uint32_t u = w ^ 0x80808080u;
+  const uint32_t a = __byte_perm(u, 0x64646464u, 0x5140);
+  const uint32_t b = __byte_perm(u, 0x64646464u, 0x5342);
+  asm("sub.rn.f16x2 %0, %1, %2;\n" : "=r"(p0) : "r"(a), "r"(0x64806480u));
+  asm("sub.rn.f16x2 %0, %1, %2;\n" : "=r"(p1) : "r"(b), "r"(0x64806480u));
+}
+
+// Two values -> their high fp16 pieces and what is left, again in fp16.
+__device__ __forceinline__ void SplitPair(float x, float y, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(hi) : "f"(y), "f"(x));
+  float hx, hy;
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n cvt.f32.f16 %1, b;\n}\n"
+      : "=f"(hx), "=f"(hy)
+      : "r"(hi));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(lo) : "f"(y - hy), "f"(x - hx));
+}
+
+__device__ __forceinline__ void CopyAsync4(void* smem_dst, const void* gmem_src) {
+  const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(smem_dst));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(gmem_src));
+}
+// The rest of a 128-byte line comes along into L2 (blocks of 64 and 128
+// tokens: the next units' part of V's rows).
+__device__ __forceinline__ void CopyAsync16Line(void* smem_dst, const void* gmem_src) {
+  const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(smem_dst));
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;\n" ::"r"(dst), "l"(gmem_src));
+}
+
+// Tokens of sequence i that are attended to: 0 for a bad length.
+__device__ __forceinline__ int LengthOf(const A8Args& a, int i) {
+  const int n = a.lengths[i];
+  return n < 0 || n > a.table_cols * a.block ? 0 : n;
+}
+__device__ __forceinline__ int UnitsIn(int length) {
+  return length / kUnit + (length % kUnit != 0 ? 1 : 0);
+}
+__device__ __forceinline__ int UnitsOf(const A8Args& a, int i) {
+  return UnitsIn(LengthOf(a, i));
+}
+
+// Share of worker w: units [w total / workers, (w + 1) total / workers), at
+// least one each: no more workers than units take part.
+__device__ __forceinline__ int64_t ShareBegin(int64_t total, int workers, int64_t w) {
+  return w * total / workers;
+}
+__device__ __forceinline__ int64_t WorkerOf(int64_t total, int workers, int64_t unit) {
+  return ((unit + 1) * workers - 1) / total;
+}
+
+// A place in the order of units.
+struct Place {
+  int seq;
+  int head;
+  int unit, units;
+  int length;
+};
+__device__ __forceinline__ void Next(const A8Args& a, Place& p) {
+  if (++p.unit < p.units) return;
+  p.unit = 0;
+  if (++p.head < a.kv_heads) return;
+  p.head = 0;
+  do {
+    if (++p.seq >= a.n_seqs) return;
+    p.length = LengthOf(a, p.seq);
+    p.units = UnitsIn(p.length);
+  } while (p.units == 0);
+}
+
+template <int HD>
+struct A8Smem {
+  // an odd number of 32-byte groups per K row
+  static constexpr int kKPitch = (HD / 32) % 2 == 0 ? HD + 32 : HD;
+  static constexpr int kKBytes = kUnit * kKPitch;
+  static constexpr int kStageBytes = kKBytes + HD * kUnit + 16;  // K, V, the two scales
+  static constexpr int kStages = 3;
+  static constexpr int kBytes = kA8Warps * kStages * kStageBytes;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kA8Warps * 32) A8Kernel(A8Args a) {
+  using S = A8Smem<HD>;
+  constexpr int kStages = S::kStages;
+  constexpr int DC = HD / 32;  // groups of 32 dimensions
+  constexpr int DT = HD / 8;   // output tiles
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
-  __shared__ float qs[kA8MaxGroup * 256];
-  __shared__ float p[kA8MaxGroup][kUnit];
-  __shared__ float m_of[kA8MaxGroup], l_of[kA8MaxGroup], alpha_of[kA8MaxGroup];
-  const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
-  const int group = a.n_heads / a.kv_heads, hd = a.hd;
-  const int64_t length = a.lengths[seq];
-  const int32_t* table = a.table + seq * a.table_cols;
-  bool bad = length < 0 || length > a.table_cols * a.block;
-  if (bad && tid == 0 && a.status != nullptr) atomicOr(a.status, MLB_STATUS_BAD_LENGTH);
-  const int64_t units = bad ? 0 : (length + kUnit - 1) / kUnit;
-  const int64_t q0 = (static_cast<int64_t>(seq) * a.n_heads + head * group) * hd;
-  for (int i = tid; i < group * hd; i += kA8Threads) qs[i] = a.q[q0 + i];
-  if (tid < group) {
-    m_of[tid] = -INFINITY;
-    l_of[tid] = 0.0f;
-  }
-  float acc[kA8MaxGroup][2] = {};
+  extern __shared__ __align__(16) uint8_t a8_raw[];
+  __shared__ int64_t sums[kA8Warps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = lane >> 2, c = lane & 3;  // head of the group / column; quarter
+  uint8_t* ring = a8_raw + warp * kStages * S::kStageBytes;
+
+  // all units, and the place where this warp's share begins
+  int64_t mine = 0;
+  for (int i = threadIdx.x; i < a.n_seqs; i += kA8Warps * 32) mine += UnitsOf(a, i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sums[warp] = mine;
   __syncthreads();
-  for (int64_t u = 0; u < units; ++u) {
-    const int64_t t0 = u * kUnit;
-    const int n = static_cast<int>(length - t0 < kUnit ? length - t0 : kUnit);
-    const int32_t id = table[t0 / a.block];
-    if (id < 0 || id >= a.n_blocks) {
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kA8Warps; ++w) total += sums[w];
+  total *= a.kv_heads;
+  if (total == 0) return;
+  const int workers = a.workers < total ? a.workers : static_cast<int>(total);
+  const int worker = warp * gridDim.x + blockIdx.x;  // few workers: one a CTA
+  if (worker >= workers) return;  // nothing below waits for another warp
+  const int64_t begin = ShareBegin(total, workers, worker);
+  const int count = static_cast<int>(ShareBegin(total, workers, worker + 1) - begin);
+  Place put{};  // next unit to copy
+  {
+    int64_t before = 0;
+    for (int base = 0; base < a.n_seqs; base += 32) {
+      const int i = base + lane;
+      const int64_t units = i < a.n_seqs ? static_cast<int64_t>(UnitsOf(a, i)) * a.kv_heads : 0;
+      int64_t upto = units;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+      const bool here = begin >= before + upto - units && begin < before + upto;
+      const uint32_t found = __ballot_sync(0xffffffffu, here);
+      if (found != 0) {
+        const int src = __ffs(found) - 1;
+        put.seq = base + src;
+        put.length = LengthOf(a, put.seq);
+        put.units = UnitsIn(put.length);
+        const int64_t first = __shfl_sync(0xffffffffu, before + upto - units, src);
+        put.head = static_cast<int>((begin - first) / put.units);
+        put.unit = static_cast<int>((begin - first) % put.units);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  Place get = put;  // next unit to compute
+
+  // block ids of 32 columns of the sequence that is being copied, one a lane
+  int window = -1;
+  int window_seq = -1;
+  int32_t my_id = -1;
+  uint32_t usable = 0;  // bit s: stage s holds a unit (its block id is good)
+  const auto copy = [&](int stage) {
+    const int token = put.unit * kUnit;
+    const int col = token >> a.block_shift;
+    if (put.seq != window_seq || col < window || col >= window + 32) {
+      window = col;
+      window_seq = put.seq;
+      my_id = col + lane < a.table_cols ? a.table[put.seq * a.table_cols + col + lane] : -1;
+    }
+    const int32_t id = __shfl_sync(0xffffffffu, my_id, col - window);
+    uint8_t* to = ring + stage * S::kStageBytes;
+    if (id >= 0 && id < a.n_blocks) {
+      const int64_t at = static_cast<int64_t>(id) * a.kv_heads + put.head;
+      const int place = token & (a.block - 1);
+      const int8_t* k = a.k_codes + (at * a.block + place) * HD;
+      const int8_t* v = a.v_codes + at * a.block * HD + place;
+      // K: 16-byte chunks in memory order; token r goes to the row of its
+      // score column
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) {
+        const int x = 32 * i + lane, r = x / (HD / 16), ch = x % (HD / 16);
+        const int dst = 8 * ((r & 7) >> 1) + 2 * (r >> 3) + (r & 1);
+        CopyAsync16(to + dst * S::kKPitch + 16 * ch, k + r * HD + 16 * ch);
+      }
+      uint8_t* vt = to + S::kKBytes;
+      if (a.block == kUnit) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) CopyAsync16(vt + 16 * (32 * i + lane), v + 16 * (32 * i + lane));
+      } else {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          const int x = 32 * i + lane, d = x >> 1, half = x & 1;
+          CopyAsync16Line(vt + 16 * x, v + static_cast<int64_t>(d) * a.block + 16 * half);
+        }
+      }
+      if (lane == 0) CopyAsync4(vt + HD * kUnit, a.k_scales + at);
+      if (lane == 1) CopyAsync4(vt + HD * kUnit + 4, a.v_scales + at);
+      usable |= 1u << stage;
+    } else {
+      usable &= ~(1u << stage);
+    }
+    Next(a, put);
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (s < count) copy(s);
+    CopyAsyncCommit();
+  }
+
+  const int64_t unit_cols = a.table_cols * a.block / kUnit;
+  uint32_t qf[2 * DC][4];  // A operand of the scores, two k16 steps per 32 dimensions
+  float acc[DT][2];
+  float m = 0.0f, l = 0.0f, factor = 0.0f;
+  bool bad = false, fresh = true;
+  int first_unit = get.unit;  // of this warp's part of the sequence
+  for (int n = 0, stage = 0; n < count; ++n) {
+    __syncwarp();  // every lane is done with the stage that is filled next
+    const int ahead = stage == 0 ? kStages - 1 : stage - 1;
+    if (n + kStages - 1 < count) copy(ahead);
+    CopyAsyncCommit();
+    if (fresh) {  // q of a new (sequence, kv head): scaled and split
+      fresh = false;
+      bad = false;
+      first_unit = get.unit;
+      m = -INFINITY;
+      l = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) acc[i][0] = acc[i][1] = 0.0f;
+      float x[DC][8];
+      float top = 0.0f;
+      const float4* q = reinterpret_cast<const float4*>(
+          a.q + (static_cast<int64_t>(get.seq) * a.n_heads + get.head * a.group + row) * HD);
+#pragma unroll
+      for (int j = 0; j < DC; ++j) {
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
+        if (row < a.group) {
+          u = q[8 * j + 2 * c];
+          w = q[8 * j + 2 * c + 1];
+        }
+        x[j][0] = u.x; x[j][1] = u.y; x[j][2] = u.z; x[j][3] = u.w;
+        x[j][4] = w.x; x[j][5] = w.y; x[j][6] = w.z; x[j][7] = w.w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[j][e]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^(14 - e) for a largest value in [2^e, 2^(e + 1)); 1 for a row of
+      // zeros or with an infinity, whose outputs are NaN whatever it is
+      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+      e = top == 0.0f || e == 128 ? 14 : max(e, -100);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
+      factor = a.scale * __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+#pragma unroll
+      for (int j = 0; j < DC; ++j)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          SplitPair(x[j][4 * s] * up, x[j][4 * s + 1] * up, qf[2 * j + s][0], qf[2 * j + s][1]);
+          SplitPair(x[j][4 * s + 2] * up, x[j][4 * s + 3] * up, qf[2 * j + s][2],
+                    qf[2 * j + s][3]);
+        }
+    }
+    CopyAsyncWait<kStages - 1>();
+    __syncwarp();  // all lanes' copies of this unit have landed
+    if ((usable >> stage & 1u) != 0) {
+      const uint8_t* kt = ring + stage * S::kStageBytes;
+      const uint8_t* vt = kt + S::kKBytes;
+      const float ks = *reinterpret_cast<const float*>(vt + HD * kUnit) * factor;
+      const float vs = *reinterpret_cast<const float*>(vt + HD * kUnit + 4) * (1.0f / kPScale);
+      // scores of the 4 column tiles
+      float sc[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int g = 0; g < DC; ++g) {
+          const uint2 w =
+              *reinterpret_cast<const uint2*>(kt + (8 * j + row) * S::kKPitch + 32 * g + 8 * c);
+          uint32_t b0, b1;
+          CodePairs(w.x, b0, b1);
+          Mma(d, qf[2 * g][0], qf[2 * g][1], qf[2 * g][2], qf[2 * g][3], b0, b1);
+          CodePairs(w.y, b0, b1);
+          Mma(d, qf[2 * g + 1][0], qf[2 * g + 1][1], qf[2 * g + 1][2], qf[2 * g + 1][3], b0, b1);
+        }
+        sc[2 * j] = (d[0] + d[2]) * ks;
+        sc[2 * j + 1] = (d[1] + d[3]) * ks;
+      }
+      const int left = get.length - get.unit * kUnit;  // tokens of the unit, if < 32
+      if (left < kUnit) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (8 * c + j >= left) sc[j] = -INFINITY;
+      }
+      float top = sc[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float m_new = fmaxf(m, top);
+      const float alpha = Exp2(m - m_new);  // 0 for the first unit
+      m = m_new;
+      float sum = 0.0f;
+      uint32_t ph[4], pl[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float p0 = Exp2(sc[2 * j] - m), p1 = Exp2(sc[2 * j + 1] - m);
+        if (left < kUnit) {  // also where m is NaN or -inf
+          if (8 * c + 2 * j >= left) p0 = 0.0f;
+          if (8 * c + 2 * j + 1 >= left) p1 = 0.0f;
+        }
+        sum += p0 + p1;
+        SplitPair(p0 * kPScale, p1 * kPScale, ph[j], pl[j]);
+      }
+      l = fmaf(l, alpha, sum);
+      if (a.units != nullptr) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (c == 0 && row < a.group)
+          a.units[(get.seq * unit_cols + get.unit) * a.n_heads + get.head * a.group + row] =
+              make_float2(m, sum);
+      }
+      // weighted values, 8 dimensions a tile
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        const uint2 w = *reinterpret_cast<const uint2*>(vt + (8 * i + row) * kUnit + 8 * c);
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t b0, b1;
+        CodePairs(w.x, b0, b1);
+        Mma(d, ph[0], pl[0], ph[1], pl[1], b0, b1);
+        CodePairs(w.y, b0, b1);
+        Mma(d, ph[2], pl[2], ph[3], pl[3], b0, b1);
+        acc[i][0] = fmaf(acc[i][0], alpha, (d[0] + d[2]) * vs);
+        acc[i][1] = fmaf(acc[i][1], alpha, (d[1] + d[3]) * vs);
+      }
+    } else {
       bad = true;
-      if (tid == 0 && a.status != nullptr) atomicOr(a.status, MLB_STATUS_BAD_BLOCK);
-      break;  // the same for every thread
     }
-    const int64_t at = static_cast<int64_t>(id) * a.kv_heads + head;
-    const int place = static_cast<int>(t0 % a.block);
-    const int8_t* k = a.k_codes + (at * a.block + place) * hd;
-    const int8_t* v = a.v_codes + at * a.block * hd + place;
-    const float ks = a.k_scales[at] * a.scale, vs = a.v_scales[at];
-    for (int i = tid; i < group * kUnit; i += kA8Threads) {
-      const int g = i / kUnit, t = i % kUnit;
-      float dot = 0.0f;
-      for (int d = 0; d < hd; ++d) dot = fmaf(qs[g * hd + d], static_cast<float>(k[t * hd + d]), dot);
-      p[g][t] = t < n ? dot * ks : -INFINITY;
-    }
-    __syncthreads();
-    for (int g = tid >> 5; g < group; g += kA8Threads / 32) {
-      const int lane = tid & 31;
-      const float s = p[g][lane];
-      const float m_new = fmaxf(m_of[g], WarpMax(s));
-      const float e = lane < n ? expf(s - m_new) : 0.0f;
-      const float sum = WarpSum(e);
-      p[g][lane] = e;
-      if (lane == 0) {
-        alpha_of[g] = expf(m_of[g] - m_new);
-        l_of[g] = fmaf(l_of[g], alpha_of[g], sum);
-        m_of[g] = m_new;
-        if (a.units != nullptr)
-          a.units[(seq * (a.table_cols * a.block / kUnit) + u) * a.n_heads + head * group + g] =
-              make_float2(m_new, sum);
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+    const bool ends = get.unit + 1 == get.units;
+    if (ends || n + 1 == count) {
+      if (bad && lane == 0 && a.status != nullptr) atomicOr(a.status, MLB_STATUS_BAD_BLOCK);
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (row < a.group) {
+        if (ends && first_unit == 0) {  // all of it was here
+          const int64_t at = static_cast<int64_t>(get.seq) * a.n_heads + get.head * a.group + row;
+          if (c == 0) a.lse[at] = bad ? make_float2(0.0f, 0.0f) : make_float2(m, l);
+          const float inv = bad ? 0.0f : 1.0f / l;
+#pragma unroll
+          for (int i = 0; i < DT; ++i)
+            *reinterpret_cast<float2*>(a.out + at * HD + 8 * i + 2 * c) =
+                bad ? make_float2(0.0f, 0.0f) : make_float2(acc[i][0] * inv, acc[i][1] * inv);
+        } else {
+          float* part = a.partial +
+                        ((static_cast<int64_t>(worker) * 2 + (first_unit == 0 ? 1 : 0)) * a.group +
+                         row) * (HD + kPartHead);
+          if (c == 0) *reinterpret_cast<float4*>(part) = make_float4(m, l, bad ? 1.0f : 0.0f, 0.0f);
+#pragma unroll
+          for (int i = 0; i < DT; ++i)
+            *reinterpret_cast<float2*>(part + kPartHead + 8 * i + 2 * c) =
+                make_float2(acc[i][0], acc[i][1]);
+        }
       }
+      fresh = true;
     }
-    __syncthreads();
-    for (int j = 0; j < 2; ++j) {
-      const int d = tid + j * kA8Threads;
-      if (d >= hd) break;
-      for (int g = 0; g < group; ++g) {
-        float sum = 0.0f;
-        for (int t = 0; t < n; ++t)
-          sum = fmaf(p[g][t], static_cast<float>(v[static_cast<int64_t>(d) * a.block + t]), sum);
-        acc[g][j] = fmaf(acc[g][j], alpha_of[g], sum * vs);
-      }
-    }
-    __syncthreads();
+    Next(a, get);
   }
-  const bool none = bad || units == 0;
-  if (tid < group)
-    a.lse[static_cast<int64_t>(seq) * a.n_heads + head * group + tid] =
-        none ? make_float2(0.0f, 0.0f) : make_float2(m_of[tid], l_of[tid]);
-  for (int j = 0; j < 2; ++j) {
-    const int d = tid + j * kA8Threads;
-    if (d >= hd) break;
-    for (int g = 0; g < group; ++g) a.out[q0 + g * hd + d] = none ? 0.0f : acc[g][j] / l_of[g];
+}
+
+// Joins the partials of a (sequence, query head): out = sum_w acc_w f_w / sum_w
+// l_w f_w, f_w = 2^(m_w - M).  Warps take partials in turn, lanes dimensions.
+constexpr int kJoinThreads = 256;
+
+__global__ void __launch_bounds__(kJoinThreads) A8JoinKernel(A8Args a) {
+  LaunchWait();  // the previous kernel on the stream has completed
+  LaunchNext();
+  __shared__ int64_t sums[2][kJoinThreads / 32];
+  __shared__ float red[3][32];
+  __shared__ float accs[kJoinThreads / 32][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int h = blockIdx.x, seq = blockIdx.y;
+  int64_t before = 0, total = 0;
+  for (int i = threadIdx.x; i < a.n_seqs; i += kJoinThreads) {
+    const int64_t u = UnitsOf(a, i);
+    total += u;
+    if (i < seq) before += u;
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  if (lane == 0) {
+    sums[0][warp] = total;
+    sums[1][warp] = before;
+  }
+  __syncthreads();
+  total = before = 0;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    total += sums[0][w];
+    before += sums[1][w];
+  }
+  total *= a.kv_heads;
+  const int64_t units = UnitsOf(a, seq);
+  const int64_t at = static_cast<int64_t>(seq) * a.n_heads + h;
+  const int kv = h / a.group;
+  if (units == 0) {
+    if (h == 0 && threadIdx.x == 0 && a.lengths[seq] != 0 && a.status != nullptr)
+      atomicOr(a.status, MLB_STATUS_BAD_LENGTH);
+    for (int d = threadIdx.x; d < a.hd; d += kJoinThreads) a.out[at * a.hd + d] = 0.0f;
+    if (threadIdx.x == 0) a.lse[at] = make_float2(0.0f, 0.0f);
+    return;
+  }
+  const int64_t first = before * a.kv_heads + kv * units;
+  const int workers = a.workers < total ? a.workers : static_cast<int>(total);
+  const int64_t w0 = WorkerOf(total, workers, first);
+  const int64_t w1 = WorkerOf(total, workers, first + units - 1);
+  if (w0 == w1) return;  // finished by its warp
+  const int n = static_cast<int>(w1 - w0) + 1;
+  const int stride = a.hd + kPartHead;
+  // worker w0 found the sequence's beginning (its slot 1), the others its rest
+  const auto part = [&](int i) {
+    return a.partial + (((w0 + i) * 2 + (i == 0 ? 1 : 0)) * a.group + h % a.group) * stride;
+  };
+  float m = -INFINITY, bad = 0.0f;
+  for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+    const float4 x = *reinterpret_cast<const float4*>(part(i));
+    m = fmaxf(m, x.x);
+    bad = fmaxf(bad, x.z);
+  }
+  m = BlockMax(m, red[0]);
+  bad = BlockMax(bad, red[1]);
+  float l = 0.0f;
+  for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+    const float4 x = *reinterpret_cast<const float4*>(part(i));
+    l += x.x == -INFINITY ? x.y : x.y * Exp2(x.x - m);
+  }
+  l = BlockSum(l, red[2]);
+  float acc[8] = {};
+  for (int i = warp; i < n; i += kJoinThreads / 32) {
+    const float* x = part(i);
+    const float f = Exp2(x[0] - m);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (32 * j < a.hd) acc[j] = fmaf(x[kPartHead + 32 * j + lane], f, acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (32 * j < a.hd) accs[warp][32 * j + lane] = acc[j];
+  __syncthreads();
+  if (threadIdx.x < a.hd) {
+    float o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) o += accs[w][threadIdx.x];
+    a.out[at * a.hd + threadIdx.x] = bad != 0.0f ? 0.0f : o / l;
+  }
+  if (threadIdx.x == 0) a.lse[at] = bad != 0.0f ? make_float2(0.0f, 0.0f) : make_float2(m, l);
 }
 
 // mass_out[i][c] = mass_in[i][c] + sum over heads and the block's units of
@@ -148,7 +558,7 @@ __global__ void __launch_bounds__(256) A8MassKernel(A8Args a, const float* mass_
       for (int h = lane; h < a.n_heads; h += 32) {
         const float2 total = lse[h];  // L = 0: a bad block, nothing was collected
         const float2 x = a.units[(seq * unit_cols + u) * a.n_heads + h];
-        if (total.y != 0.0f) sum += x.y * expf(x.x - total.x) / total.y;
+        if (total.y != 0.0f) sum += x.y * Exp2(x.x - total.x) / total.y;
       }
   }
   sum = WarpSum(sum);
@@ -169,16 +579,62 @@ const char* A8Shape(int64_t n_seqs, int64_t table_cols, int block, int n_heads, 
   return nullptr;
 }
 
+// Warps of the grid: as many as run at once, but not more than there can be
+// units.
+constexpr int kA8MaxSmem = 227 * 1024;
+template <int HD>
+int CtasPerSm() {
+  constexpr int by_smem = kA8MaxSmem / (A8Smem<HD>::kBytes + 2048);
+  return by_smem < 1 ? 1 : by_smem;
+}
+int Workers(int64_t n_seqs, int64_t unit_cols, int kv_heads, int hd) {
+  int per_sm = 1;
+  switch (hd / 32) {
+    case 1: per_sm = CtasPerSm<32>(); break;
+    case 2: per_sm = CtasPerSm<64>(); break;
+    case 3: per_sm = CtasPerSm<96>(); break;
+    case 4: per_sm = CtasPerSm<128>(); break;
+    case 5: per_sm = CtasPerSm<160>(); break;
+    case 6: per_sm = CtasPerSm<192>(); break;
+    case 7: per_sm = CtasPerSm<224>(); break;
+    default: per_sm = CtasPerSm<256>(); break;
+  }
+  if (per_sm > 4) per_sm = 4;
+  const int64_t ctas = static_cast<int64_t>(per_sm) * SmCount();
+  const int64_t most = n_seqs * unit_cols * kv_heads;
+  const int64_t need = (most + kA8Warps - 1) / kA8Warps;
+  return static_cast<int>(need < ctas ? need : ctas) * kA8Warps;
+}
+
 struct A8Scratch {
-  int64_t lse, units, total;  // floats: offsets and the sum
+  int64_t lse, units, partial, total;  // floats: offsets and the sum
+  int workers;
 };
 
-A8Scratch ScratchOf(int64_t n_seqs, int64_t table_cols, int block, int n_heads, bool with_mass) {
+A8Scratch ScratchOf(int64_t n_seqs, int64_t table_cols, int block, int n_heads, int kv_heads,
+                    int hd, bool with_mass) {
   A8Scratch s;
+  const int64_t unit_cols = table_cols * block / kUnit;
+  s.workers = Workers(n_seqs, unit_cols, kv_heads, hd);
   s.lse = 0;
   s.units = (2 * n_seqs * n_heads + 3) & ~int64_t{3};
-  s.total = s.units + (with_mass ? 2 * n_seqs * (table_cols * block / kUnit) * n_heads : 0);
+  s.partial = s.units + (with_mass ? (2 * n_seqs * unit_cols * n_heads + 3) & ~int64_t{3} : 0);
+  s.total = s.partial + int64_t{2} * s.workers * (n_heads / kv_heads) * (hd + kPartHead);
   return s;
+}
+
+template <int HD>
+int LaunchA8(const A8Args& a, cudaStream_t s) {
+  constexpr int shm = A8Smem<HD>::kBytes;
+  if (shm > 48 * 1024 &&
+      cudaFuncSetAttribute(A8Kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, shm) !=
+          cudaSuccess) {
+    cudaGetLastError();
+    return Fail(MLB_ERR_CUDA, "mlb_attention_kv8_f32: shared memory opt-in");
+  }
+  Launch(A8Kernel<HD>, dim3(static_cast<unsigned>(a.workers / kA8Warps)), kA8Warps * 32,
+         static_cast<size_t>(shm), s, a);
+  return MLB_OK;
 }
 
 }  // namespace
@@ -190,7 +646,9 @@ extern "C" int64_t mlb_attention_kv8_scratch_floats(int64_t n_seqs, int64_t tabl
   using namespace mlb;
   if (A8Shape(n_seqs, table_cols, block_tokens, n_heads, n_kv_heads, head_dim) != nullptr)
     return -1;
-  return ScratchOf(n_seqs, table_cols, block_tokens, n_heads, with_mass != 0).total;
+  return ScratchOf(n_seqs, table_cols, block_tokens, n_heads, n_kv_heads, head_dim,
+                   with_mass != 0)
+      .total;
 }
 
 extern "C" int mlb_attention_kv8_f32(const float* q, const int8_t* k_codes, const int8_t* v_codes,
@@ -217,17 +675,34 @@ extern "C" int mlb_attention_kv8_f32(const float* q, const int8_t* k_codes, cons
   if (!Aligned16(q) || !Aligned16(out) || !Aligned16(k_codes) || !Aligned16(v_codes) ||
       !Aligned16(scratch))
     return Fail(MLB_ERR_ARG, op + "q, out, codes and scratch must be 16-byte aligned");
-  const A8Scratch need = ScratchOf(n_seqs, table_cols, block_tokens, n_heads, mass_out != nullptr);
+  const A8Scratch need = ScratchOf(n_seqs, table_cols, block_tokens, n_heads, n_kv_heads,
+                                   head_dim, mass_out != nullptr);
   if (scratch == nullptr || scratch_floats < need.total)
     return Fail(MLB_ERR_ARG, op + "scratch too small");
+  const double log2e = 1.4426950408889634;
   A8Args a{q, k_codes, v_codes, k_scales, v_scales, table, lengths, out,
            reinterpret_cast<float2*>(scratch + need.lse),
            mass_out != nullptr ? reinterpret_cast<float2*>(scratch + need.units) : nullptr,
-           n_blocks, table_cols, static_cast<int>(n_seqs), block_tokens, n_heads, n_kv_heads,
-           head_dim, 1.0f / std::sqrt(static_cast<float>(head_dim)), status};
+           scratch + need.partial, n_blocks, table_cols, static_cast<int>(n_seqs), block_tokens,
+           block_tokens == 32 ? 5 : block_tokens == 64 ? 6 : 7, n_heads, n_kv_heads, head_dim, n_heads / n_kv_heads, need.workers,
+           static_cast<float>(log2e / std::sqrt(static_cast<double>(head_dim))), status};
   cudaStream_t s = AsStream(stream);
-  Launch(A8Kernel, dim3(static_cast<unsigned>(n_kv_heads), static_cast<unsigned>(n_seqs)),
-         kA8Threads, 0, s, a);
+  if (need.workers > 0) {
+    int rc = MLB_OK;
+    switch (head_dim / 32) {
+      case 1: rc = LaunchA8<32>(a, s); break;
+      case 2: rc = LaunchA8<64>(a, s); break;
+      case 3: rc = LaunchA8<96>(a, s); break;
+      case 4: rc = LaunchA8<128>(a, s); break;
+      case 5: rc = LaunchA8<160>(a, s); break;
+      case 6: rc = LaunchA8<192>(a, s); break;
+      case 7: rc = LaunchA8<224>(a, s); break;
+      default: rc = LaunchA8<256>(a, s); break;
+    }
+    if (rc != MLB_OK) return rc;
+  }
+  Launch(A8JoinKernel, dim3(static_cast<unsigned>(n_heads), static_cast<unsigned>(n_seqs)),
+         kJoinThreads, 0, s, a);
   if (mass_out != nullptr && table_cols > 0)
     Launch(A8MassKernel, dim3(static_cast<unsigned>((table_cols + 7) / 8),
                               static_cast<unsigned>(n_seqs)),
