@@ -61,6 +61,7 @@ struct A8Args {
                    // token or a bad sequence
   float2* units;   // [n_seqs][unit columns][n_heads] (m, sum p), or null
   float* partial;  // [warps of the grid][2][group][kPartHead + hd]
+  int2* spans;     // [n_seqs][kv_heads] first worker and number of workers
   int64_t n_blocks;
   int64_t table_cols;
   int n_seqs;
@@ -168,12 +169,15 @@ struct A8Smem {
   static constexpr int kKPitch = (HD / 32) % 2 == 0 ? HD + 32 : HD;
   static constexpr int kKBytes = kUnit * kKPitch;
   static constexpr int kStageBytes = kKBytes + HD * kUnit + 16;  // K, V, the two scales
-  static constexpr int kStages = 3;
+  static constexpr int kStages = 2;
   static constexpr int kBytes = kA8Warps * kStages * kStageBytes;
+  // CTAs that fit an SM's shared memory (1 KB of each is the system's)
+  static constexpr int kFit = 228 * 1024 / (kBytes + 1024 + 256);
+  static constexpr int kCtasPerSm = kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kA8Warps * 32) A8Kernel(A8Args a) {
+__global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kernel(A8Args a) {
   using S = A8Smem<HD>;
   constexpr int kStages = S::kStages;
   constexpr int DC = HD / 32;  // groups of 32 dimensions
@@ -293,7 +297,7 @@ __global__ void __launch_bounds__(kA8Warps * 32) A8Kernel(A8Args a) {
   int first_unit = get.unit;  // of this warp's part of the sequence
   for (int n = 0, stage = 0; n < count; ++n) {
     __syncwarp();  // every lane is done with the stage that is filled next
-    const int ahead = stage == 0 ? kStages - 1 : stage - 1;
+    const int ahead = (stage + kStages - 1) % kStages;
     if (n + kStages - 1 < count) copy(ahead);
     CopyAsyncCommit();
     if (fresh) {  // q of a new (sequence, kv head): scaled and split
@@ -346,21 +350,30 @@ __global__ void __launch_bounds__(kA8Warps * 32) A8Kernel(A8Args a) {
       const float vs = *reinterpret_cast<const float*>(vt + HD * kUnit + 4) * (1.0f / kPScale);
       // scores of the 4 column tiles
       float sc[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      {
+        float d[4][4] = {};
 #pragma unroll
         for (int g = 0; g < DC; ++g) {
-          const uint2 w =
-              *reinterpret_cast<const uint2*>(kt + (8 * j + row) * S::kKPitch + 32 * g + 8 * c);
-          uint32_t b0, b1;
-          CodePairs(w.x, b0, b1);
-          Mma(d, qf[2 * g][0], qf[2 * g][1], qf[2 * g][2], qf[2 * g][3], b0, b1);
-          CodePairs(w.y, b0, b1);
-          Mma(d, qf[2 * g + 1][0], qf[2 * g + 1][1], qf[2 * g + 1][2], qf[2 * g + 1][3], b0, b1);
+          uint2 w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            w[j] = *reinterpret_cast<const uint2*>(kt + (8 * j + row) * S::kKPitch + 32 * g +
+                                                   8 * c);
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t b0, b1;
+              CodePairs(s == 0 ? w[j].x : w[j].y, b0, b1);
+              const uint32_t(&q)[4] = qf[2 * g + s];
+              Mma(d[j], q[0], q[1], q[2], q[3], b0, b1);
+            }
         }
-        sc[2 * j] = (d[0] + d[2]) * ks;
-        sc[2 * j + 1] = (d[1] + d[3]) * ks;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sc[2 * j] = (d[j][0] + d[j][2]) * ks;
+          sc[2 * j + 1] = (d[j][1] + d[j][3]) * ks;
+        }
       }
       const int left = get.length - get.unit * kUnit;  // tokens of the unit, if < 32
       if (left < kUnit) {
@@ -398,26 +411,40 @@ __global__ void __launch_bounds__(kA8Warps * 32) A8Kernel(A8Args a) {
       }
       // weighted values, 8 dimensions a tile
 #pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        const uint2 w = *reinterpret_cast<const uint2*>(vt + (8 * i + row) * kUnit + 8 * c);
-        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        uint32_t b0, b1;
-        CodePairs(w.x, b0, b1);
-        Mma(d, ph[0], pl[0], ph[1], pl[1], b0, b1);
-        CodePairs(w.y, b0, b1);
-        Mma(d, ph[2], pl[2], ph[3], pl[3], b0, b1);
-        acc[i][0] = fmaf(acc[i][0], alpha, (d[0] + d[2]) * vs);
-        acc[i][1] = fmaf(acc[i][1], alpha, (d[1] + d[3]) * vs);
+      for (int i = 0; i < DT; i += 4) {
+        uint2 w[4];
+        float d[4][4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] = *reinterpret_cast<const uint2*>(vt + (8 * (i + j) + row) * kUnit + 8 * c);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t b0, b1;
+            CodePairs(s == 0 ? w[j].x : w[j].y, b0, b1);
+            Mma(d[j], ph[2 * s], pl[2 * s], ph[2 * s + 1], pl[2 * s + 1], b0, b1);
+          }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[i + j][0] = fmaf(acc[i + j][0], alpha, (d[j][0] + d[j][2]) * vs);
+          acc[i + j][1] = fmaf(acc[i + j][1], alpha, (d[j][1] + d[j][3]) * vs);
+        }
       }
     } else {
       bad = true;
     }
-    stage = stage == kStages - 1 ? 0 : stage + 1;
+    stage = (stage + 1) % kStages;
     const bool ends = get.unit + 1 == get.units;
     if (ends || n + 1 == count) {
       if (bad && lane == 0 && a.status != nullptr) atomicOr(a.status, MLB_STATUS_BAD_BLOCK);
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (first_unit == 0 && lane == 0) {  // who else has a part of it
+        const int64_t last = begin + n + (get.units - 1 - get.unit);
+        a.spans[static_cast<int64_t>(get.seq) * a.kv_heads + get.head] = make_int2(
+            worker, ends ? 1 : static_cast<int>(WorkerOf(total, workers, last)) - worker + 1);
+      }
       if (row < a.group) {
         if (ends && first_unit == 0) {  // all of it was here
           const int64_t at = static_cast<int64_t>(get.seq) * a.n_heads + get.head * a.group + row;
@@ -451,50 +478,23 @@ constexpr int kJoinThreads = 256;
 __global__ void __launch_bounds__(kJoinThreads) A8JoinKernel(A8Args a) {
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
-  __shared__ int64_t sums[2][kJoinThreads / 32];
   __shared__ float red[3][32];
   __shared__ float accs[kJoinThreads / 32][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int h = blockIdx.x, seq = blockIdx.y;
-  int64_t before = 0, total = 0;
-  for (int i = threadIdx.x; i < a.n_seqs; i += kJoinThreads) {
-    const int64_t u = UnitsOf(a, i);
-    total += u;
-    if (i < seq) before += u;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
-  if (lane == 0) {
-    sums[0][warp] = total;
-    sums[1][warp] = before;
-  }
-  __syncthreads();
-  total = before = 0;
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) {
-    total += sums[0][w];
-    before += sums[1][w];
-  }
-  total *= a.kv_heads;
-  const int64_t units = UnitsOf(a, seq);
   const int64_t at = static_cast<int64_t>(seq) * a.n_heads + h;
   const int kv = h / a.group;
-  if (units == 0) {
+  const int2 span = a.spans[static_cast<int64_t>(seq) * a.kv_heads + kv];
+  if (LengthOf(a, seq) == 0) {  // its span was not written
     if (h == 0 && threadIdx.x == 0 && a.lengths[seq] != 0 && a.status != nullptr)
       atomicOr(a.status, MLB_STATUS_BAD_LENGTH);
     for (int d = threadIdx.x; d < a.hd; d += kJoinThreads) a.out[at * a.hd + d] = 0.0f;
     if (threadIdx.x == 0) a.lse[at] = make_float2(0.0f, 0.0f);
     return;
   }
-  const int64_t first = before * a.kv_heads + kv * units;
-  const int workers = a.workers < total ? a.workers : static_cast<int>(total);
-  const int64_t w0 = WorkerOf(total, workers, first);
-  const int64_t w1 = WorkerOf(total, workers, first + units - 1);
-  if (w0 == w1) return;  // finished by its warp
-  const int n = static_cast<int>(w1 - w0) + 1;
+  if (span.y == 1) return;  // finished by its warp
+  const int64_t w0 = span.x;
+  const int n = span.y;
   const int stride = a.hd + kPartHead;
   // worker w0 found the sequence's beginning (its slot 1), the others its rest
   const auto part = [&](int i) {
@@ -515,6 +515,7 @@ __global__ void __launch_bounds__(kJoinThreads) A8JoinKernel(A8Args a) {
   }
   l = BlockSum(l, red[2]);
   float acc[8] = {};
+#pragma unroll 4
   for (int i = warp; i < n; i += kJoinThreads / 32) {
     const float* x = part(i);
     const float f = Exp2(x[0] - m);
@@ -581,25 +582,18 @@ const char* A8Shape(int64_t n_seqs, int64_t table_cols, int block, int n_heads, 
 
 // Warps of the grid: as many as run at once, but not more than there can be
 // units.
-constexpr int kA8MaxSmem = 227 * 1024;
-template <int HD>
-int CtasPerSm() {
-  constexpr int by_smem = kA8MaxSmem / (A8Smem<HD>::kBytes + 2048);
-  return by_smem < 1 ? 1 : by_smem;
-}
 int Workers(int64_t n_seqs, int64_t unit_cols, int kv_heads, int hd) {
   int per_sm = 1;
   switch (hd / 32) {
-    case 1: per_sm = CtasPerSm<32>(); break;
-    case 2: per_sm = CtasPerSm<64>(); break;
-    case 3: per_sm = CtasPerSm<96>(); break;
-    case 4: per_sm = CtasPerSm<128>(); break;
-    case 5: per_sm = CtasPerSm<160>(); break;
-    case 6: per_sm = CtasPerSm<192>(); break;
-    case 7: per_sm = CtasPerSm<224>(); break;
-    default: per_sm = CtasPerSm<256>(); break;
+    case 1: per_sm = A8Smem<32>::kCtasPerSm; break;
+    case 2: per_sm = A8Smem<64>::kCtasPerSm; break;
+    case 3: per_sm = A8Smem<96>::kCtasPerSm; break;
+    case 4: per_sm = A8Smem<128>::kCtasPerSm; break;
+    case 5: per_sm = A8Smem<160>::kCtasPerSm; break;
+    case 6: per_sm = A8Smem<192>::kCtasPerSm; break;
+    case 7: per_sm = A8Smem<224>::kCtasPerSm; break;
+    default: per_sm = A8Smem<256>::kCtasPerSm; break;
   }
-  if (per_sm > 4) per_sm = 4;
   const int64_t ctas = static_cast<int64_t>(per_sm) * SmCount();
   const int64_t most = n_seqs * unit_cols * kv_heads;
   const int64_t need = (most + kA8Warps - 1) / kA8Warps;
@@ -607,7 +601,7 @@ int Workers(int64_t n_seqs, int64_t unit_cols, int kv_heads, int hd) {
 }
 
 struct A8Scratch {
-  int64_t lse, units, partial, total;  // floats: offsets and the sum
+  int64_t lse, units, spans, partial, total;  // floats: offsets and the sum
   int workers;
 };
 
@@ -618,7 +612,8 @@ A8Scratch ScratchOf(int64_t n_seqs, int64_t table_cols, int block, int n_heads, 
   s.workers = Workers(n_seqs, unit_cols, kv_heads, hd);
   s.lse = 0;
   s.units = (2 * n_seqs * n_heads + 3) & ~int64_t{3};
-  s.partial = s.units + (with_mass ? (2 * n_seqs * unit_cols * n_heads + 3) & ~int64_t{3} : 0);
+  s.spans = s.units + (with_mass ? (2 * n_seqs * unit_cols * n_heads + 3) & ~int64_t{3} : 0);
+  s.partial = s.spans + ((2 * n_seqs * kv_heads + 3) & ~int64_t{3});
   s.total = s.partial + int64_t{2} * s.workers * (n_heads / kv_heads) * (hd + kPartHead);
   return s;
 }
@@ -683,7 +678,7 @@ extern "C" int mlb_attention_kv8_f32(const float* q, const int8_t* k_codes, cons
   A8Args a{q, k_codes, v_codes, k_scales, v_scales, table, lengths, out,
            reinterpret_cast<float2*>(scratch + need.lse),
            mass_out != nullptr ? reinterpret_cast<float2*>(scratch + need.units) : nullptr,
-           scratch + need.partial, n_blocks, table_cols, static_cast<int>(n_seqs), block_tokens,
+           scratch + need.partial, reinterpret_cast<int2*>(scratch + need.spans), n_blocks, table_cols, static_cast<int>(n_seqs), block_tokens,
            block_tokens == 32 ? 5 : block_tokens == 64 ? 6 : 7, n_heads, n_kv_heads, head_dim, n_heads / n_kv_heads, need.workers,
            static_cast<float>(log2e / std::sqrt(static_cast<double>(head_dim))), status};
   cudaStream_t s = AsStream(stream);

@@ -490,27 +490,31 @@ def linear_rows_group(weights, qtype: int, ns, k: int, x, scratch=None, stream=N
 # call allocates belong to the stream it runs on.
 
 class _On:
-    """The device of `tensor` current and, if given, `stream` too."""
+    """Makes the device of `tensor` current, and `stream` if given; enters with
+    the raw stream.  Where both are so already, as in a decode loop, it costs
+    two look-ups (torch's stream objects cost a microsecond or more each)."""
+    __slots__ = ("device", "stream", "guards")
 
     def __init__(self, tensor, stream):
-        import torch
-        self.device = torch.cuda.device(tensor.device)
-        self.stream = None if stream is None else torch.cuda.stream(stream)
+        self.device, self.stream, self.guards = tensor.get_device(), stream, None
 
     def __enter__(self):
-        self.device.__enter__()
-        if self.stream is not None:
-            self.stream.__enter__()
-        return _stream(None)
+        import torch
+        if self.stream is not None or torch.cuda.current_device() != self.device:
+            self.guards = [torch.cuda.device(self.device)]
+            if self.stream is not None:
+                self.guards.append(torch.cuda.stream(self.stream))
+            for g in self.guards:
+                g.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.device)
 
     def __exit__(self, *exc):
-        if self.stream is not None:
-            self.stream.__exit__(*exc)
-        self.device.__exit__(*exc)
+        for g in reversed(self.guards or ()):
+            g.__exit__(*exc)
 
 
 def _like(t, dtype, device, op, name, shape=None):
-    if not (t.dtype == dtype and t.device == device and t.is_contiguous()):
+    if t.dtype is not dtype or t.device != device or not t.is_contiguous():
         raise ValueError(f"{op}: {name} must be a contiguous {dtype} tensor on {device}")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{op}: {name} must be {list(shape)}, got {list(t.shape)}")
