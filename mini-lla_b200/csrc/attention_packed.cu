@@ -188,6 +188,843 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
     Launch(PkRowKernel<G, 2>, grid, kPkWarps * 32, 0, s, a);
 }
 
+// ---------------------------------------------------------------------------
+// Prompts on the tensor cores (head sizes 64 and 128).
+//
+// Operands.  q, k, v and p are split into two fp16 pieces each, x 2^s = hi + lo
+// + r, |r| <= 2^-22 |x 2^s| or 2^-25, with 2^s bringing the largest magnitude
+// (of a query vector, of a block of 128 keys, of p's 1) to [2^14, 2^15).  Each
+// product runs as hi lo + lo hi and then hi hi into one fp32 accumulator
+// (tcgen05.mma kind::f16): the small terms are added while the sum is small,
+// so the large ones see one rounding per 16 values; lo lo is below 2^-22 of
+// each term and left out.  Both S = Q K^T and O_b = P_b V_b start from zero
+// for every block of 128 keys; O_b is added to the running output in fp32
+// registers, so no sum longer than 128 lives in the tensor core.
+//
+// First launch (PkSplitKernel).  One CTA per (block of 128 keys of a sequence,
+// kv head, K or V) writes the block's pieces as the images that the products
+// read from shared memory (128-byte swizzled, K-major, V transposed, keys
+// past the sequence's end as zeros), so that the second launch brings a
+// block in with one bulk copy and no tensor map, wherever the sequence
+// begins.  One more CTA lists the query tiles, those with the most key blocks
+// first.
+//
+// Second launch (PkTcKernel).  CTA = (tile of 128 query vectors: 128 / G rows x
+// G heads of a kv head); 320 threads:
+//   - warps 0-3 and 4-7: thread = query vector = tensor-memory lane.  They
+//     write Q's pieces into tensor memory once.  Group b % 2 takes block b's
+//     softmax: the maximum of the block alone, rounded to a whole power of
+//     two m_b, p = 2^(s - m_b), P's pieces over S in tensor memory.  Both
+//     groups then add O_b, half of the dimensions each, to their registers:
+//     acc = acc 2^(M - M') + O_b 2^(m_b - M'), both factors exact.
+//   - warp 8: bulk copies, K_0, K_1, V_0, K_2, V_1, ... through a ring;
+//   - warp 9: tensor memory; one lane issues S_b, then O_(b - 1), so that the
+//     softmax of block b runs under the products of O_(b - 1) and S_(b + 1).
+// Tensor memory: Q hi and lo, two S / P buffers, O.  All waits are bounded; a
+// CTA whose wait gave up writes NaN and is counted (mlb_wait_timeouts).
+//
+// A V block with an Inf or NaN is marked: where not every row of a tile sees
+// all of such a block, a row that does not see it would still meet it as 0 *
+// NaN, so that tile is computed on the CUDA cores.
+//
+// Bound: 6 products of 2 * 128 * 128 * hd flops for 128 vectors and keys.
+
+constexpr int kPtKeys = 128;
+constexpr int kPtVectors = 128;
+constexpr int kPtThreads = 320;
+constexpr int kPtTmemColumns = 512;
+constexpr int kPtQCol = 0;      // Q hi, Q lo: hd / 2 columns each
+constexpr int kPtSCol = 128;    // two buffers of 128 columns
+constexpr int kPtOCol = 384;
+constexpr float kPtPScale = 16384.0f;
+
+// A query tile; rows of a tile belong to one sequence.
+struct PtTile {
+  int row0, rows;   // packed rows
+  int sees;         // keys that the first row sees (may be <= 0)
+  int block0;       // image index of the sequence's first key block
+  int64_t key0;     // packed row of its first key
+  int64_t unused;
+};
+
+struct PtPlan {
+  int64_t max_blocks, max_tiles;
+  // byte offsets in the scratch
+  int64_t images, factors, tiles, blocks, total;
+};
+
+PtPlan PlanOf(int64_t q_rows, int64_t k_rows, int64_t n_seqs, int n_heads, int kv_heads, int hd) {
+  PtPlan p;
+  const int64_t qr = kPtVectors / (n_heads / kv_heads);
+  p.max_blocks = k_rows / kPtKeys + n_seqs;
+  p.max_tiles = q_rows / qr + n_seqs;
+  p.images = 0;
+  p.factors = p.images + p.max_blocks * kv_heads * (int64_t{8} * kPtKeys * hd);
+  p.tiles = p.factors + ((p.max_blocks * kv_heads * 8 + 31) & ~int64_t{31});
+  p.blocks = p.tiles + p.max_tiles * static_cast<int64_t>(sizeof(PtTile));
+  p.total = p.blocks + ((n_seqs + 1) * 4 + 15) / 16 * 16;
+  return p;
+}
+
+struct PtArgs {
+  PkArgs in;
+  uint8_t* images;   // [max_blocks][kv_heads][K hi, K lo, V hi, V lo]
+  float2* factors;   // [max_blocks][kv_heads] (K's 2^-s, V's 2^-s; V's negative: Inf or NaN)
+  PtTile* tiles;
+  int32_t* blocks;   // [n_seqs] first image of a sequence (-1: left out); then the tile count
+  int64_t max_blocks;
+  int64_t max_tiles;
+  int group;
+};
+
+// Offset of 16-byte chunk c of row r in a tile of 128-byte rows.
+__device__ __forceinline__ uint32_t PtSwz(int r, int c) {
+  return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4));
+}
+
+// The power of two that brings a largest magnitude in [2^e, 2^(e + 1)) to
+// [2^14, 2^15), and its inverse; 1 for 0.
+__device__ __forceinline__ float PtUp(float top, float& down) {
+  int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+  e = top == 0.0f ? 14 : max(e, -100);
+  down = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+  return __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
+}
+
+__device__ __forceinline__ float PtExp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two values -> their high fp16 pieces and what is left, again in fp16.
+__device__ __forceinline__ void PtSplit(float x, float y, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(hi) : "f"(y), "f"(x));
+  float hx, hy;
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n cvt.f32.f16 %1, b;\n}\n"
+      : "=f"(hx), "=f"(hy)
+      : "r"(hi));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(lo) : "f"(y - hy), "f"(x - hx));
+}
+
+constexpr int kPtSplitThreads = 256;
+
+// First image of every sequence, scanned kPtSplitThreads at a time; calls
+// each(i, range, first image, blocks) for the sequences that take part.  All
+// threads of the CTA call it; each thread sees its own sequences.
+template <typename Each>
+__device__ int64_t PtScan(const PtArgs& a, bool report, Each each) {
+  __shared__ int64_t warp_sum[kPtSplitThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t before = 0;
+  for (int base = 0; base < a.in.n_seqs; base += kPtSplitThreads) {
+    const int i = base + static_cast<int>(threadIdx.x);
+    PkSeq s{};
+    int64_t blocks = 0;
+    bool good = false;
+    if (i < a.in.n_seqs) {
+      good = PkRange(a.in, i, s);
+      if (!good && report && a.in.status != nullptr) atomicOr(a.in.status, MLB_STATUS_BAD_LENGTH);
+      if (good) blocks = (s.k1 - s.k0 + kPtKeys - 1) / kPtKeys;
+    }
+    int64_t upto = blocks;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kPtSplitThreads / 32; ++w) {
+      if (w < warp) upto += warp_sum[w];
+      total += warp_sum[w];
+    }
+    // ranges that run backwards can let others overlap and claim more blocks
+    // than there are: those are left out too (the status is raised already)
+    const int64_t first = before + upto - blocks;
+    if (i < a.in.n_seqs) each(i, s, good && first + blocks <= a.max_blocks ? first : -1, blocks);
+    before += total;
+    __syncthreads();
+  }
+  return before;
+}
+
+// The list of query tiles, in falling order of their key blocks (counting
+// sort over 1024 bins).
+__device__ void PtListTiles(const PtArgs& a) {
+  __shared__ int bins[1024];
+  __shared__ int bin_sum[kPtSplitThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int qr = kPtVectors / a.group;
+  for (int i = threadIdx.x; i < 1024; i += kPtSplitThreads) bins[i] = 0;
+  PtScan(a, true, [&](int i, const PkSeq&, int64_t first, int64_t) {
+    a.blocks[i] = static_cast<int32_t>(first);
+  });
+  __syncthreads();  // also the block's own global writes
+  int shift = 0;
+  while ((a.in.k_rows / kPtKeys + 1) >> shift >= 1024) ++shift;
+  const auto tiles = [&](auto&& take) {
+    for (int i = warp; i < a.in.n_seqs; i += kPtSplitThreads / 32) {
+      if (a.blocks[i] < 0) continue;
+      PkSeq s;
+      PkRange(a.in, i, s);
+      const int64_t rows = s.q1 - s.q0, keys = s.k1 - s.k0;
+      for (int64_t t = lane; t * qr < rows; t += 32) {
+        PtTile tile;
+        tile.row0 = static_cast<int>(s.q0 + t * qr);
+        tile.rows = static_cast<int>(rows - t * qr < qr ? rows - t * qr : qr);
+        tile.sees = static_cast<int>(keys - rows + t * qr + 1);
+        tile.block0 = a.blocks[i];
+        tile.key0 = s.k0;
+        tile.unused = 0;
+        const int last = tile.sees + tile.rows - 1;  // keys of the last row
+        const int nb = last <= 0 ? 0 : (last + kPtKeys - 1) / kPtKeys;
+        take(tile, 1023 - (nb >> shift));
+      }
+    }
+  };
+  tiles([&](const PtTile&, int bin) { atomicAdd(&bins[bin], 1); });
+  __syncthreads();
+  // exclusive scan: 4 bins a thread
+  int each[4], sum = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum += each[j] = bins[4 * threadIdx.x + j];
+  int upto = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += up;
+  }
+  if (lane == 31) bin_sum[warp] = upto;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) upto += bin_sum[w];
+  int at = upto - sum;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    bins[4 * threadIdx.x + j] = at;
+    at += each[j];
+  }
+  if (threadIdx.x == kPtSplitThreads - 1)
+    a.blocks[a.in.n_seqs] = static_cast<int32_t>(min(static_cast<int64_t>(upto), a.max_tiles));
+  __syncthreads();
+  tiles([&](const PtTile& tile, int bin) {
+    const int n = atomicAdd(&bins[bin], 1);
+    if (n < a.max_tiles) a.tiles[n] = tile;
+  });
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kPtSplitThreads) PkSplitKernel(PtArgs a) {
+  LaunchWait();  // the previous kernel on the stream has completed
+  LaunchNext();
+  if (static_cast<int64_t>(blockIdx.x) == a.max_blocks) {
+    if (blockIdx.y == 0 && blockIdx.z == 0) PtListTiles(a);
+    return;
+  }
+  __shared__ int64_t key0_of;
+  __shared__ int keys_of;
+  __shared__ float top_of[kPtSplitThreads / 32];
+  __shared__ int odd_of[kPtSplitThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t image = blockIdx.x;
+  const int head = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
+  if (threadIdx.x == 0) keys_of = 0;
+  __syncthreads();
+  PtScan(a, false, [&](int, const PkSeq& s, int64_t first, int64_t blocks) {
+    if (first >= 0 && image >= first && image < first + blocks) {
+      key0_of = s.k0 + (image - first) * kPtKeys;
+      keys_of = static_cast<int>(min(s.k1 - key0_of, static_cast<int64_t>(kPtKeys)));
+    }
+  });
+  __syncthreads();
+  const int keys = keys_of;
+  if (keys == 0) return;
+  const int64_t stride = static_cast<int64_t>(a.in.kv_heads) * HD;
+  const float* x = (is_v ? a.in.v : a.in.k) + key0_of * stride + head * HD;
+  uint8_t* hi = a.images + (image * a.in.kv_heads + head) * (int64_t{8} * kPtKeys * HD) +
+                (is_v ? 4 * kPtKeys * HD : 0);
+  uint8_t* lo = hi + 2 * kPtKeys * HD;
+  // 8 values a step: of one key (K) or of one dimension (V)
+  constexpr int kSteps = kPtKeys * HD / 8 / kPtSplitThreads;
+  float val[kSteps][8];
+  float top = 0.0f;
+  int odd = 0;  // Inf or NaN
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int n = i * kPtSplitThreads + threadIdx.x;
+    if (!is_v) {
+      const int key = n / (HD / 8), c = n % (HD / 8);
+      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
+      if (key < keys) {
+        u = *reinterpret_cast<const float4*>(x + key * stride + 8 * c);
+        w = *reinterpret_cast<const float4*>(x + key * stride + 8 * c + 4);
+      }
+      val[i][0] = u.x; val[i][1] = u.y; val[i][2] = u.z; val[i][3] = u.w;
+      val[i][4] = w.x; val[i][5] = w.y; val[i][6] = w.z; val[i][7] = w.w;
+    } else {
+      const int d = n % HD, k0 = n / HD * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) val[i][e] = k0 + e < keys ? x[(k0 + e) * stride + d] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float m = fabsf(val[i][e]);
+      if (m < INFINITY) top = fmaxf(top, m);  // finite values set the scale
+      else odd = 1;
+    }
+  }
+  top = WarpMax(top);
+  odd = __any_sync(0xffffffffu, odd);
+  if (lane == 0) {
+    top_of[warp] = top;
+    odd_of[warp] = odd;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPtSplitThreads / 32; ++w) {
+    top = fmaxf(top, top_of[w]);
+    odd |= odd_of[w];
+  }
+  float down;
+  const float up = PtUp(top, down);
+  if (threadIdx.x == 0) {
+    float* f = reinterpret_cast<float*>(a.factors + image * a.in.kv_heads + head);
+    f[is_v ? 1 : 0] = is_v && odd ? -down : down;
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int n = i * kPtSplitThreads + threadIdx.x;
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) PtSplit(val[i][2 * e] * up, val[i][2 * e + 1] * up, h[e], l[e]);
+    uint32_t at;
+    if (!is_v) {
+      const int key = n / (HD / 8), c = n % (HD / 8);
+      at = static_cast<uint32_t>(c >> 3) * (kPtKeys * 128) + PtSwz(key, c & 7);
+    } else {
+      const int d = n % HD, c = n / HD;
+      at = static_cast<uint32_t>(c >> 3) * (HD * 128) + PtSwz(d, c & 7);
+    }
+    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+}
+
+__device__ __forceinline__ uint32_t PtSmem(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void PtBarInit(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void PtArrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void PtExpect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+// ~2 s at most (each poll suspends for at most ~1 us)
+__device__ __forceinline__ bool PtWait(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < (1 << 21); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "n"(1000)
+        : "memory");
+    if (ok != 0) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void PtBulk(uint32_t dst, const void* src, uint32_t bytes,
+                                       uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::
+          "r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void PtCommit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar)
+      : "memory");
+}
+// K-major operand, 128-byte swizzle, 8-row atoms 1024 bytes apart.
+__device__ __forceinline__ uint64_t PtDesc(uint32_t addr) {
+  uint64_t d = static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(1) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+// D fp32, A and B fp16, both K-major, M = 128, N = n.
+__host__ __device__ constexpr uint32_t PtInstr(int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kPtVectors >> 4) << 24);
+}
+// D[tmem] (+)= A[a_tmem] . B[b]^T.
+__device__ __forceinline__ void PtMma(uint32_t d, uint32_t a, uint64_t b, uint32_t instr,
+                                      uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(instr), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void PtLd32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32"
+      " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+      " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31},"
+      " [%32];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+        "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+        "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
+        "=r"(v[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void PtSt32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0],"
+      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16,"
+      " %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+      "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+// Shared memory from a 1024-byte aligned base: the ring of images (hi and lo
+// of one block's K or V each), barriers, block statistics.
+template <int HD>
+struct PtLayout {
+  static constexpr int kItemBytes = 4 * kPtKeys * HD;  // hi and lo
+  static constexpr int kStages = HD == 128 ? 3 : 6;
+  static constexpr int kStat = kStages * kItemBytes;          // float2 [4][128]
+  static constexpr int kBars = kStat + 4 * kPtVectors * 8;
+  // full / empty per stage, q_full, s_full[2], p_full[4], o_full, o_empty, done
+  static constexpr int kBarriers = 2 * kStages + 10;
+  static constexpr int kSmemBytes = kBars + 8 * kBarriers + 16 + 1024;
+};
+
+}  // namespace
+
+// Bounded waits of this file's kernel that gave up.
+__device__ unsigned int g_pt_wait_timeouts;
+
+namespace {
+
+// A tile on the CUDA cores: a warp a vector, keys one after another.
+template <int HD>
+__device__ void PtSlowTile(const PtArgs& a, const PtTile& tile, int head) {
+  constexpr int E = HD / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t stride = static_cast<int64_t>(a.in.kv_heads) * HD;
+  const float* k = a.in.k + tile.key0 * stride + head * HD;
+  const float* v = a.in.v + tile.key0 * stride + head * HD;
+  for (int i = warp; i < tile.rows * a.group; i += kPtThreads / 32) {
+    const int sees = tile.sees + i / a.group;
+    const int64_t at =
+        ((tile.row0 + i / a.group) * static_cast<int64_t>(a.in.n_heads) + head * a.group +
+         i % a.group) * HD;
+    float q[E], acc[E], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      q[e] = a.in.q[at + 32 * e + lane];
+      acc[e] = 0.0f;
+    }
+    for (int t = 0; t < sees; ++t) {
+      float dot = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) dot = fmaf(q[e], k[t * stride + 32 * e + lane], dot);
+      const float s = WarpSum(dot) * a.in.scale;
+      const float m_new = fmaxf(m, s);
+      const float alpha = m == -INFINITY ? 0.0f : expf(m - m_new);
+      const float p = expf(s - m_new);
+      l = fmaf(l, alpha, p);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(acc[e], alpha, p * v[t * stride + 32 * e + lane]);
+      m = m_new;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) a.in.out[at + 32 * e + lane] = sees > 0 ? acc[e] / l : 0.0f;
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
+  using L = PtLayout<HD>;
+  constexpr int kStages = L::kStages;
+  constexpr int HH = HD / 2;  // dimensions of the output a group holds
+  LaunchWait();  // the previous kernel on the stream has completed
+  LaunchNext();
+  extern __shared__ __align__(16) uint8_t pt_raw[];
+  const int head = static_cast<int>(blockIdx.x % a.in.kv_heads);
+  const int64_t number = blockIdx.x / a.in.kv_heads;
+  if (number >= a.blocks[a.in.n_seqs]) return;
+  const PtTile tile = a.tiles[number];
+  const int last = tile.sees + tile.rows - 1;  // keys that the last row sees
+  const int nb = last <= 0 ? 0 : (last + kPtKeys - 1) / kPtKeys;
+  const float2* factors = a.factors + static_cast<int64_t>(tile.block0) * a.in.kv_heads + head;
+  // blocks that not every row sees whole
+  const int partial0 = tile.sees <= 0 ? 0 : tile.sees / kPtKeys;
+  {
+    bool slow = false;
+    for (int b = partial0; b < nb; ++b)
+      slow |= factors[static_cast<int64_t>(b) * a.in.kv_heads].y < 0.0f;
+    if (nb == 0 || slow) {
+      PtSlowTile<HD>(a, tile, head);
+      return;
+    }
+  }
+
+  const uint32_t raw_addr = PtSmem(pt_raw);
+  uint8_t* base = pt_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+  const uint32_t sbase = PtSmem(base);
+  float2* stat = reinterpret_cast<float2*>(base + L::kStat);
+  const uint32_t bars = sbase + L::kBars;
+  const auto full = [&](int s) { return bars + 8 * s; };
+  const auto empty = [&](int s) { return bars + 8 * (kStages + s); };
+  const uint32_t q_full = bars + 8 * (2 * kStages);
+  const auto s_full = [&](int s) { return bars + 8 * (2 * kStages + 1 + s); };
+  // four: the other group may wait for block b's while b + 2's is written
+  const auto p_full = [&](int s) { return bars + 8 * (2 * kStages + 3 + s); };
+  const uint32_t o_full = bars + 8 * (2 * kStages + 7);
+  const uint32_t o_empty = bars + 8 * (2 * kStages + 8);
+  const uint32_t all_done = bars + 8 * (2 * kStages + 9);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kBars + 8 * L::kBarriers);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      PtBarInit(full(s), 1);
+      PtBarInit(empty(s), 1);
+    }
+    PtBarInit(q_full, 256);
+    for (int s = 0; s < 2; ++s) PtBarInit(s_full(s), 1);
+    for (int s = 0; s < 4; ++s) PtBarInit(p_full(s), 128);
+    PtBarInit(o_full, 1);
+    PtBarInit(o_empty, 256);
+    PtBarInit(all_done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
+                     PtSmem(tmem_slot)),
+                 "r"(kPtTmemColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  const auto give_up = [&]() {
+    if (!*abort_flag) atomicAdd(&g_pt_wait_timeouts, 1u);
+    *abort_flag = 1;
+  };
+  const auto wait = [&](uint32_t bar, uint32_t parity) {
+    return PtWait(bar, parity) && !*abort_flag;
+  };
+  // whose outcome every lane of the warp shares
+  const auto warp_wait = [&](uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
+  };
+
+  if (warp == 8) {
+    // --------------------------------------------------------------- copies
+    if (lane == 0) {
+      int put = 0;
+      bool ok = true;
+      const auto copy = [&](int b, bool is_v) {
+        const int s = put % kStages;
+        if (put >= kStages && !wait(empty(s), (put / kStages - 1) & 1)) {
+          give_up();
+          ok = false;
+          return;
+        }
+        const uint8_t* src =
+            a.images +
+            ((static_cast<int64_t>(tile.block0) + b) * a.in.kv_heads + head) * (2 * L::kItemBytes) +
+            (is_v ? L::kItemBytes : 0);
+        PtExpect(full(s), L::kItemBytes);
+        PtBulk(sbase + s * L::kItemBytes, src, L::kItemBytes, full(s));
+        ++put;
+      };
+      for (int b = 0; ok && b <= nb; ++b) {
+        if (b < nb) copy(b, false);
+        if (ok && b >= 1) copy(b - 1, true);
+      }
+      if (!ok)  // what is in flight lands before the CTA ends
+        for (int i = put > kStages ? put - kStages : 0; i < put; ++i)
+          PtWait(full(i % kStages), (i / kStages) & 1);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------- products
+    if (lane == 0) {
+      bool ok = wait(q_full, 0);
+      if (!ok) give_up();
+      int get = 0;
+      for (int b = 0; ok && b <= nb; ++b) {
+        if (b < nb) {  // S_b = Q K_b^T
+          const int s = get % kStages;
+          if (!wait(full(s), (get / kStages) & 1)) {
+            give_up();
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          const uint32_t d = tmem + kPtSCol + 128 * (b & 1);
+          const uint32_t kh = sbase + s * L::kItemBytes, kl = kh + L::kItemBytes / 2;
+          const uint32_t qh = tmem + kPtQCol, ql = qh + HD / 2;
+#pragma unroll
+          for (int j = 0; j < HD / 16; ++j) {
+            const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
+            PtMma(d, qh + 8 * j, PtDesc(kl + off), PtInstr(kPtKeys), j != 0 ? 1u : 0u);
+            PtMma(d, ql + 8 * j, PtDesc(kh + off), PtInstr(kPtKeys), 1u);
+          }
+#pragma unroll
+          for (int j = 0; j < HD / 16; ++j) {
+            const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
+            PtMma(d, qh + 8 * j, PtDesc(kh + off), PtInstr(kPtKeys), 1u);
+          }
+          PtCommit(empty(s));
+          PtCommit(s_full(b & 1));
+          ++get;
+        }
+        if (b >= 1) {  // O_(b - 1) = P V
+          const int j0 = b - 1, s = get % kStages;
+          if (!wait(full(s), (get / kStages) & 1) || !wait(p_full(j0 & 3), (j0 >> 2) & 1) ||
+              (j0 >= 1 && !wait(o_empty, (j0 - 1) & 1))) {
+            give_up();
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          const uint32_t d = tmem + kPtOCol, p = tmem + kPtSCol + 128 * (j0 & 1);
+          const uint32_t vh = sbase + s * L::kItemBytes, vl = vh + L::kItemBytes / 2;
+          // 16 keys a step; P's pieces of 32 keys: 16 columns hi, 16 lo
+#pragma unroll
+          for (int j = 0; j < kPtKeys / 16; ++j) {
+            const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
+            const uint32_t ph = p + 32 * (j >> 1) + 8 * (j & 1), pl = ph + 16;
+            PtMma(d, ph, PtDesc(vl + off), PtInstr(HD), j != 0 ? 1u : 0u);
+            PtMma(d, pl, PtDesc(vh + off), PtInstr(HD), 1u);
+          }
+#pragma unroll
+          for (int j = 0; j < kPtKeys / 16; ++j) {
+            const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
+            PtMma(d, p + 32 * (j >> 1) + 8 * (j & 1), PtDesc(vh + off), PtInstr(HD), 1u);
+          }
+          PtCommit(empty(s));
+          PtCommit(o_full);
+          ++get;
+        }
+      }
+      PtCommit(all_done);
+      // what was issued has read its operands before tensor memory goes back
+      if (!PtWait(all_done, 0)) give_up();
+    }
+  } else {
+    // -------------------------------------------------- softmax and output
+    const int group = warp >> 2;                       // 0: warps 0-3, 1: 4-7
+    const int v = (warp & 3) * 32 + lane;              // query vector
+    const int row = v / a.group;
+    const bool live = row < tile.rows && v < (kPtVectors / a.group) * a.group;
+    const int sees = live ? tile.sees + row : 0;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const int64_t at = ((tile.row0 + row) * static_cast<int64_t>(a.in.n_heads) + head * a.group +
+                        v % a.group) * HD;
+    float scale;  // of raw scores, to powers of two; without the key block's factor
+    {
+      const float4* q = reinterpret_cast<const float4*>(a.in.q + at);
+      float top = 0.0f;
+      if (live) {
+#pragma unroll 8
+        for (int i = 0; i < HD / 4; ++i) {
+          const float4 x = q[i];
+          const float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+          // a vector with Inf (or NaN) has NaN outputs whatever its scale
+          top = fmaxf(top, m < INFINITY ? m : 0.0f);
+        }
+      }
+      float down;
+      const float up = PtUp(top, down);
+      scale = a.in.scale * 1.4426950408889634f * down;
+#pragma unroll
+      for (int c = 0; c < HH / 32; ++c) {  // 32 dimensions: 16 columns of each piece
+        uint32_t out[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 x =
+              live ? q[group * (HH / 4) + 8 * c + i] : make_float4(0.f, 0.f, 0.f, 0.f);
+          PtSplit(x.x * up, x.y * up, out[2 * i], out[16 + 2 * i]);
+          PtSplit(x.z * up, x.w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
+        }
+        const uint32_t to = lanes + kPtQCol + group * (HH / 2) + 16 * c;
+#define PT_ST16(addr, o)                                                                        \
+  asm volatile(                                                                                 \
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"                                            \
+      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(addr), \
+      "r"(out[o]), "r"(out[o + 1]), "r"(out[o + 2]), "r"(out[o + 3]), "r"(out[o + 4]),           \
+      "r"(out[o + 5]), "r"(out[o + 6]), "r"(out[o + 7]), "r"(out[o + 8]), "r"(out[o + 9]),       \
+      "r"(out[o + 10]), "r"(out[o + 11]), "r"(out[o + 12]), "r"(out[o + 13]), "r"(out[o + 14]),  \
+      "r"(out[o + 15])                                                                          \
+      : "memory")
+        PT_ST16(to, 0);
+        PT_ST16(to + HD / 2, 16);
+#undef PT_ST16
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      PtArrive(q_full);
+    }
+    float acc[HH];
+#pragma unroll
+    for (int i = 0; i < HH; ++i) acc[i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int b = 0; b <= nb; ++b) {
+      if (b < nb && (b & 1) == group) {
+        const float f = scale * factors[static_cast<int64_t>(b) * a.in.kv_heads].x;
+        if (!warp_wait(s_full(b & 1), (b >> 1) & 1)) {
+          give_up();
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const uint32_t s_at = lanes + kPtSCol + 128 * (b & 1);
+        const int seen = sees - b * kPtKeys;  // keys of the block that the row sees
+        const bool whole = b < partial0;      // the same for every thread
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t s[32];
+          PtLd32(s_at + 32 * c, s);
+          if (whole) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(s[j]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              top = fmaxf(top, 32 * c + j < seen ? __uint_as_float(s[j]) : -INFINITY);
+          }
+        }
+        // the reference is a whole power of two: 2^(m_b - M) is exact, and so
+        // is the subtraction's operand
+        const float mb = rintf(top * f);
+        const float minus = mb == -INFINITY ? 0.0f : -mb;  // nothing seen: p is 0
+        float sum = 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t s[32];
+          PtLd32(s_at + 32 * c, s);
+          uint32_t out[32];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            float p0 = PtExp2(fmaf(__uint_as_float(s[2 * j]), f, minus));
+            float p1 = PtExp2(fmaf(__uint_as_float(s[2 * j + 1]), f, minus));
+            if (!whole) {
+              if (32 * c + 2 * j >= seen) p0 = 0.0f;
+              if (32 * c + 2 * j + 1 >= seen) p1 = 0.0f;
+            }
+            sum += p0 + p1;
+            PtSplit(p0 * kPtPScale, p1 * kPtPScale, out[j], out[16 + j]);
+          }
+          PtSt32(s_at + 32 * c, out);
+        }
+        stat[(b & 3) * kPtVectors + v] = make_float2(mb, sum);
+        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        PtArrive(p_full(b & 3));
+      }
+      if (b >= 1) {
+        const int j = b - 1;
+        const float fv = fabsf(factors[static_cast<int64_t>(j) * a.in.kv_heads].y);
+        if (!warp_wait(p_full(j & 3), (j >> 2) & 1) || !warp_wait(o_full, j & 1)) {
+          give_up();
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const float2 st = stat[(j & 3) * kPtVectors + v];
+        const float m_new = fmaxf(m, st.x);
+        const float keep = m == m_new ? 1.0f : PtExp2(m - m_new);
+        const float weight = st.x == -INFINITY ? 0.0f : PtExp2(st.x - m_new);
+        const float add = weight * (fv * (1.0f / kPtPScale));
+        l = st.x == -INFINITY ? l + st.y : fmaf(l, keep, st.y * weight);
+        m = m_new;
+#pragma unroll
+        for (int c = 0; c < HH / 32; ++c) {
+          uint32_t o[32];
+          PtLd32(lanes + kPtOCol + group * HH + 32 * c, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            acc[32 * c + i] = fmaf(acc[32 * c + i], keep, __uint_as_float(o[i]) * add);
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        PtArrive(o_empty);
+      }
+    }
+    if (live) {
+      float4* o = reinterpret_cast<float4*>(a.in.out + at + group * HH);
+      const float inv = 1.0f / l;
+#pragma unroll
+      for (int i = 0; i < HH / 4; ++i) {
+        float4 y = make_float4(acc[4 * i] * inv, acc[4 * i + 1] * inv, acc[4 * i + 2] * inv,
+                               acc[4 * i + 3] * inv);
+        if (sees <= 0) y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!ok) y = make_float4(NAN, NAN, NAN, NAN);
+        o[i] = y;
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  if (warp == 9) {
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
+                 "r"(kPtTmemColumns)
+                 : "memory");
+  }
+}
+
+template <int HD>
+int LaunchPkTc(const PtArgs& a, cudaStream_t s) {
+  constexpr int smem = PtLayout<HD>::kSmemBytes;
+  if (cudaFuncSetAttribute(PkTcKernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+      cudaSuccess) {
+    cudaGetLastError();
+    return Fail(MLB_ERR_CUDA, "mlb_attention_packed_f32: shared memory opt-in");
+  }
+  Launch(PkSplitKernel<HD>,
+         dim3(static_cast<unsigned>(a.max_blocks + 1), static_cast<unsigned>(a.in.kv_heads), 2),
+         kPtSplitThreads, 0, s, a);
+  Launch(PkTcKernel<HD>, dim3(static_cast<unsigned>(a.max_tiles * a.in.kv_heads)), kPtThreads,
+         static_cast<size_t>(smem), s, a);
+  return MLB_OK;
+}
+
+// Whether the tensor cores take a call.
+bool TakesTc(int64_t q_rows, int64_t k_rows, int64_t n_seqs, int n_heads, int kv_heads, int hd) {
+  (void)n_heads;
+  if (hd != 64 && hd != 128) return false;
+  const int64_t tiles = q_rows / (kPtVectors / (n_heads / kv_heads)) + n_seqs;
+  return k_rows >= 64 * n_seqs && tiles * kv_heads <= INT_MAX;
+}
+
 const char* PkShape(int64_t q_rows, int64_t k_rows, int64_t n_seqs, int n_heads, int kv_heads,
                     int hd) {
   if (n_heads <= 0 || kv_heads <= 0 || n_heads % kv_heads != 0 ||
@@ -200,6 +1037,16 @@ const char* PkShape(int64_t q_rows, int64_t k_rows, int64_t n_seqs, int n_heads,
 }
 
 }  // namespace
+
+unsigned int PackedWaitTimeouts() {
+  unsigned int count = 0;
+  if (cudaMemcpyFromSymbol(&count, g_pt_wait_timeouts, sizeof(count)) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return count;
+}
+
 }  // namespace mlb
 
 extern "C" int64_t mlb_attention_packed_scratch_floats(int64_t q_rows, int64_t k_rows,
@@ -207,7 +1054,8 @@ extern "C" int64_t mlb_attention_packed_scratch_floats(int64_t q_rows, int64_t k
                                                        int n_kv_heads, int head_dim) {
   using namespace mlb;
   if (PkShape(q_rows, k_rows, n_seqs, n_heads, n_kv_heads, head_dim) != nullptr) return -1;
-  return 0;
+  if (!TakesTc(q_rows, k_rows, n_seqs, n_heads, n_kv_heads, head_dim)) return 0;
+  return PlanOf(q_rows, k_rows, n_seqs, n_heads, n_kv_heads, head_dim).total / 4;
 }
 
 extern "C" int mlb_attention_packed_f32(const float* q, const float* k, const float* v, float* out,
@@ -233,6 +1081,16 @@ extern "C" int mlb_attention_packed_f32(const float* q, const float* k, const fl
                  n_heads, n_kv_heads, head_dim, 1.0f / std::sqrt(static_cast<float>(head_dim)),
                  status};
   cudaStream_t s = AsStream(stream);
+  if (TakesTc(q_rows, k_rows, n_seqs, n_heads, n_kv_heads, head_dim)) {
+    const PtPlan p = PlanOf(q_rows, k_rows, n_seqs, n_heads, n_kv_heads, head_dim);
+    uint8_t* at = reinterpret_cast<uint8_t*>(scratch);
+    const PtArgs t{a, at + p.images, reinterpret_cast<float2*>(at + p.factors),
+                   reinterpret_cast<PtTile*>(at + p.tiles),
+                   reinterpret_cast<int32_t*>(at + p.blocks), p.max_blocks, p.max_tiles,
+                   n_heads / n_kv_heads};
+    const int rc = head_dim == 64 ? LaunchPkTc<64>(t, s) : LaunchPkTc<128>(t, s);
+    return rc != MLB_OK ? rc : CheckLaunch("mlb_attention_packed_f32");
+  }
   switch (n_heads / n_kv_heads) {
     case 1: LaunchPkRows<1>(a, s); break;
     case 2: LaunchPkRows<2>(a, s); break;

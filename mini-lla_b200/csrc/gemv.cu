@@ -685,6 +685,7 @@ int GemvTc(int qtype, int count, const void* const* w, const int64_t* n, int64_t
 unsigned int GemvTcWaitTimeouts();
 unsigned int LinearF16WaitTimeouts();  // linear_f16.cu
 unsigned int AttnTcWaitTimeouts();     // attention_tc.cu
+unsigned int PackedWaitTimeouts();     // attention_packed.cu
 }  // namespace mlb
 
 namespace {
@@ -759,7 +760,7 @@ extern "C" int mlb_wait_timeouts(unsigned int* count) {
       cudaMemcpyFromSymbol(&abandoned, g_wait_abandoned, sizeof(unsigned int)) != cudaSuccess)
     return Fail(MLB_ERR_CUDA, "mlb_wait_timeouts: read failed");
   *count += TcWaitTimeouts() + GemvTcWaitTimeouts() + LinearF16WaitTimeouts() +
-            AttnTcWaitTimeouts();
+            AttnTcWaitTimeouts() + PackedWaitTimeouts();
   if (abandoned != 0)
     return Fail(MLB_ERR_CUDA, "mlb_wait_timeouts: " + std::to_string(abandoned) +
                                   " warp(s) gave up with bulk copies still pending into "
