@@ -209,17 +209,20 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
 // begins.  One more CTA lists the query tiles, those with the most key blocks
 // first.
 //
-// Second launch (PkTcKernel).  CTA = (tile of 128 query vectors: 128 / G rows x
-// G heads of a kv head); 320 threads:
-//   - warps 0-3 and 4-7: thread = query vector = tensor-memory lane.  They
-//     write Q's pieces into tensor memory once.  Group b % 2 takes block b's
-//     softmax: the maximum of the block alone, rounded to a whole power of
-//     two m_b, p = 2^(s - m_b), P's pieces over S in tensor memory.  Both
-//     groups then add O_b, half of the dimensions each, to their registers:
-//     acc = acc 2^(M - M') + O_b 2^(m_b - M'), both factors exact.
-//   - warp 8: bulk copies, K_0, K_1, V_0, K_2, V_1, ... through a ring;
-//   - warp 9: tensor memory; one lane issues S_b, then O_(b - 1), so that the
-//     softmax of block b runs under the products of O_(b - 1) and S_(b + 1).
+// Second launch (PkTcKernel).  One CTA per SM takes tiles of 128 query vectors
+// (128 / G rows x G heads of a kv head) from the list; 320 threads:
+//   - warps 0-3 and 4-7: thread = (query vector = tensor-memory lane, half).
+//     They write the tile's Q pieces into tensor memory; per block each takes
+//     64 keys of its vector's scores, the two halves exchange their maxima
+//     through shared memory, and p = 2^(s - m_b) goes back over S as pieces,
+//     with the block's own reference m_b, rounded to a whole power of two.
+//     Then O_(b - 1), half of the dimensions each, joins the registers: acc =
+//     acc 2^(M - M') + O 2^(m - M'), both factors exact.  The next tile's Q
+//     is written before the last block's output is taken.
+//   - warp 8: bulk copies, K_0, K_1, V_0, K_2, V_1, ... through a ring, on into
+//     the next tile;
+//   - warp 9: tensor memory; one lane issues S_(b + 1), then O_b, so that the
+//     softmax of a block runs under the products of its neighbours.
 // Tensor memory: Q hi and lo, two S / P buffers, O.  All waits are bounded; a
 // CTA whose wait gave up writes NaN and is counted (mlb_wait_timeouts).
 //
@@ -243,8 +246,8 @@ struct PtTile {
   int row0, rows;   // packed rows
   int sees;         // keys that the first row sees (may be <= 0)
   int block0;       // image index of the sequence's first key block
-  int64_t key0;     // packed row of its first key
-  int64_t unused;
+  int key0;         // packed row of its first key
+  int unused[3];
 };
 
 struct PtPlan {
@@ -305,6 +308,36 @@ __device__ __forceinline__ void PtSplit(float x, float y, uint32_t& hi, uint32_t
       : "=f"(hx), "=f"(hy)
       : "r"(hi));
   asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(lo) : "f"(y - hy), "f"(x - hx));
+}
+
+// Packed pairs of fp32 (one instruction each).
+__device__ __forceinline__ uint64_t PtPair(float x, float y) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ void PtUnpair(uint64_t p, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(p));
+}
+__device__ __forceinline__ uint64_t PtFma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t PtMul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t PtAdd2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float PtMax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 constexpr int kPtSplitThreads = 256;
@@ -372,13 +405,12 @@ __device__ void PtListTiles(const PtArgs& a) {
       PkRange(a.in, i, s);
       const int64_t rows = s.q1 - s.q0, keys = s.k1 - s.k0;
       for (int64_t t = lane; t * qr < rows; t += 32) {
-        PtTile tile;
+        PtTile tile{};
         tile.row0 = static_cast<int>(s.q0 + t * qr);
         tile.rows = static_cast<int>(rows - t * qr < qr ? rows - t * qr : qr);
         tile.sees = static_cast<int>(keys - rows + t * qr + 1);
         tile.block0 = a.blocks[i];
-        tile.key0 = s.k0;
-        tile.unused = 0;
+        tile.key0 = static_cast<int>(s.k0);
         const int last = tile.sees + tile.rows - 1;  // keys of the last row
         const int nb = last <= 0 ? 0 : (last + kPtKeys - 1) / kPtKeys;
         take(tile, 1023 - (nb >> shift));
@@ -563,6 +595,11 @@ __device__ __forceinline__ uint64_t PtDesc(uint32_t addr) {
   d |= static_cast<uint64_t>(2) << 61;
   return d;
 }
+// The descriptor of an operand `bytes` further (a multiple of 16; shared
+// memory's addresses leave room in the field).
+__device__ __forceinline__ uint64_t PtAt(uint64_t desc, uint32_t bytes) {
+  return desc + (bytes >> 4);
+}
 // D fp32, A and B fp16, both K-major, M = 128, N = n.
 __host__ __device__ constexpr uint32_t PtInstr(int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) |
@@ -577,7 +614,8 @@ __device__ __forceinline__ void PtMma(uint32_t d, uint32_t a, uint64_t b, uint32
       "r"(a), "l"(b), "r"(instr), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void PtLd32(uint32_t taddr, uint32_t (&v)[32]) {
+// 32 columns of a lane, without waiting (PtLdWait).
+__device__ __forceinline__ void PtLd32(uint32_t taddr, uint32_t* v) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32"
       " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
@@ -590,9 +628,16 @@ __device__ __forceinline__ void PtLd32(uint32_t taddr, uint32_t (&v)[32]) {
         "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
         "=r"(v[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
-__device__ __forceinline__ void PtSt32(uint32_t taddr, const uint32_t (&v)[32]) {
+// Waits for the loads of N registers; they pass through so that no use of
+// them moves above the wait.
+template <int N>
+__device__ __forceinline__ void PtLdWait(uint32_t (&v)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
+__device__ __forceinline__ void PtSt32(uint32_t taddr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0],"
       " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16,"
@@ -606,16 +651,56 @@ __device__ __forceinline__ void PtSt32(uint32_t taddr, const uint32_t (&v)[32]) 
       : "memory");
 }
 
+__device__ __forceinline__ void PtSt16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15])
+      : "memory");
+}
+
+// One lane of the warp, the same each time.  (The compiler knows that code
+// behind it runs on a single thread.)
+__device__ __forceinline__ bool PtElect() {
+  uint32_t e;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(e));
+  return e != 0;
+}
+
+// Turns 16-byte chunks over between the four lanes of a quad: lane i's x[j]
+// becomes lane j's x[i].
+__device__ __forceinline__ void PtTurnPair(float4& a, float4& b, bool odd, int mask) {
+  float4 t = odd ? a : b;
+  t.x = __shfl_xor_sync(0xffffffffu, t.x, mask);
+  t.y = __shfl_xor_sync(0xffffffffu, t.y, mask);
+  t.z = __shfl_xor_sync(0xffffffffu, t.z, mask);
+  t.w = __shfl_xor_sync(0xffffffffu, t.w, mask);
+  if (odd) a = t;
+  else b = t;
+}
+__device__ __forceinline__ void PtTurn(float4& x0, float4& x1, float4& x2, float4& x3) {
+  const bool odd = (threadIdx.x & 1) != 0, high = (threadIdx.x & 2) != 0;
+  PtTurnPair(x0, x1, odd, 1);
+  PtTurnPair(x2, x3, odd, 1);
+  PtTurnPair(x0, x2, high, 2);
+  PtTurnPair(x1, x3, high, 2);
+}
+
 // Shared memory from a 1024-byte aligned base: the ring of images (hi and lo
-// of one block's K or V each), barriers, block statistics.
+// of one block's K or V each), the halves' exchange, barriers.
 template <int HD>
 struct PtLayout {
   static constexpr int kItemBytes = 4 * kPtKeys * HD;  // hi and lo
   static constexpr int kStages = HD == 128 ? 3 : 6;
-  static constexpr int kStat = kStages * kItemBytes;          // float2 [4][128]
-  static constexpr int kBars = kStat + 4 * kPtVectors * 8;
-  // full / empty per stage, q_full, s_full[2], p_full[4], o_full, o_empty, done
-  static constexpr int kBarriers = 2 * kStages + 10;
+  static constexpr int kSwap = kStages * kItemBytes;   // float [2][2][128]
+  static constexpr int kBars = kSwap + 4 * kPtVectors * 4;
+  // full / empty per stage, q_full, s_full[2], p_full[2], o_full, o_empty,
+  // swap[4], done
+  static constexpr int kBarriers = 2 * kStages + 12;
   static constexpr int kSmemBytes = kBars + 8 * kBarriers + 16 + 1024;
 };
 
@@ -663,50 +748,68 @@ __device__ void PtSlowTile(const PtArgs& a, const PtTile& tile, int head) {
   }
 }
 
+// The tiles of a CTA, in the order in which every role walks them: rounds over
+// the sorted list, every other one backwards.
+struct PtWork {
+  PtTile tile;
+  int head;
+  int nb;        // key blocks
+  int partial0;  // from this block on not every row sees the whole block
+  bool valid;    // false: no more
+  bool slow;     // computed on the CUDA cores (also: nothing to see)
+};
+
+__device__ __forceinline__ PtWork PtFetch(const PtArgs& a, int64_t total, int& round) {
+  PtWork w;
+  w.valid = false;
+  for (;; ++round) {
+    const int64_t base = static_cast<int64_t>(round) * gridDim.x;
+    if (base >= total) return w;
+    const int64_t n = base + ((round & 1) == 0 ? blockIdx.x : gridDim.x - 1 - blockIdx.x);
+    if (n >= total) continue;
+    ++round;
+    w.valid = true;
+    w.tile = a.tiles[n / a.in.kv_heads];
+    w.head = static_cast<int>(n % a.in.kv_heads);
+    const int last = w.tile.sees + w.tile.rows - 1;  // keys that the last row sees
+    w.nb = last <= 0 ? 0 : (last + kPtKeys - 1) / kPtKeys;
+    w.partial0 = w.tile.sees <= 0 ? 0 : w.tile.sees / kPtKeys;
+    w.slow = w.nb == 0;
+    for (int b = w.partial0; b < w.nb; ++b)
+      w.slow |= a.factors[(static_cast<int64_t>(w.tile.block0) + b) * a.in.kv_heads + w.head].y <
+                0.0f;
+    return w;
+  }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
   using L = PtLayout<HD>;
   constexpr int kStages = L::kStages;
-  constexpr int HH = HD / 2;  // dimensions of the output a group holds
+  constexpr int HH = HD / 2;  // dimensions of the output a thread holds
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
   extern __shared__ __align__(16) uint8_t pt_raw[];
-  const int head = static_cast<int>(blockIdx.x % a.in.kv_heads);
-  const int64_t number = blockIdx.x / a.in.kv_heads;
-  if (number >= a.blocks[a.in.n_seqs]) return;
-  const PtTile tile = a.tiles[number];
-  const int last = tile.sees + tile.rows - 1;  // keys that the last row sees
-  const int nb = last <= 0 ? 0 : (last + kPtKeys - 1) / kPtKeys;
-  const float2* factors = a.factors + static_cast<int64_t>(tile.block0) * a.in.kv_heads + head;
-  // blocks that not every row sees whole
-  const int partial0 = tile.sees <= 0 ? 0 : tile.sees / kPtKeys;
-  {
-    bool slow = false;
-    for (int b = partial0; b < nb; ++b)
-      slow |= factors[static_cast<int64_t>(b) * a.in.kv_heads].y < 0.0f;
-    if (nb == 0 || slow) {
-      PtSlowTile<HD>(a, tile, head);
-      return;
-    }
-  }
-
+  const int64_t total = static_cast<int64_t>(a.blocks[a.in.n_seqs]) * a.in.kv_heads;
   const uint32_t raw_addr = PtSmem(pt_raw);
   uint8_t* base = pt_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   const uint32_t sbase = PtSmem(base);
-  float2* stat = reinterpret_cast<float2*>(base + L::kStat);
+  float* swap = reinterpret_cast<float*>(base + L::kSwap);
   const uint32_t bars = sbase + L::kBars;
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (kStages + s); };
   const uint32_t q_full = bars + 8 * (2 * kStages);
   const auto s_full = [&](int s) { return bars + 8 * (2 * kStages + 1 + s); };
-  // four: the other group may wait for block b's while b + 2's is written
   const auto p_full = [&](int s) { return bars + 8 * (2 * kStages + 3 + s); };
-  const uint32_t o_full = bars + 8 * (2 * kStages + 7);
-  const uint32_t o_empty = bars + 8 * (2 * kStages + 8);
-  const uint32_t all_done = bars + 8 * (2 * kStages + 9);
+  const uint32_t o_full = bars + 8 * (2 * kStages + 5);
+  const uint32_t o_empty = bars + 8 * (2 * kStages + 6);
+  const auto swapped = [&](int w) { return bars + 8 * (2 * kStages + 7 + w); };
+  const uint32_t all_done = bars + 8 * (2 * kStages + 11);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kBars + 8 * L::kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* slow_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -714,12 +817,16 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
       PtBarInit(empty(s), 1);
     }
     PtBarInit(q_full, 256);
-    for (int s = 0; s < 2; ++s) PtBarInit(s_full(s), 1);
-    for (int s = 0; s < 4; ++s) PtBarInit(p_full(s), 128);
+    for (int s = 0; s < 2; ++s) {
+      PtBarInit(s_full(s), 1);
+      PtBarInit(p_full(s), 256);
+    }
     PtBarInit(o_full, 1);
     PtBarInit(o_empty, 256);
+    for (int w = 0; w < 4; ++w) PtBarInit(swapped(w), 64);
     PtBarInit(all_done, 1);
     *abort_flag = 0;
+    *slow_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 9) {
@@ -737,37 +844,43 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
     if (!*abort_flag) atomicAdd(&g_pt_wait_timeouts, 1u);
     *abort_flag = 1;
   };
-  const auto wait = [&](uint32_t bar, uint32_t parity) {
+  const auto wait = [&](uint32_t bar, uint32_t parity) __attribute__((always_inline)) {
     return PtWait(bar, parity) && !*abort_flag;
   };
   // whose outcome every lane of the warp shares
-  const auto warp_wait = [&](uint32_t bar, uint32_t parity) {
+  const auto warp_wait = [&](uint32_t bar, uint32_t parity) __attribute__((always_inline)) {
     return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
   };
 
   if (warp == 8) {
     // --------------------------------------------------------------- copies
-    if (lane == 0) {
-      int put = 0;
+    if (PtElect()) {
+      int put = 0, round = 0;
       bool ok = true;
-      const auto copy = [&](int b, bool is_v) {
-        const int s = put % kStages;
-        if (put >= kStages && !wait(empty(s), (put / kStages - 1) & 1)) {
-          give_up();
-          ok = false;
-          return;
+      for (PtWork w = PtFetch(a, total, round); ok && w.valid; w = PtFetch(a, total, round)) {
+        if (w.slow) {
+          *slow_flag = 1;
+          continue;
         }
-        const uint8_t* src =
+        const uint8_t* image =
             a.images +
-            ((static_cast<int64_t>(tile.block0) + b) * a.in.kv_heads + head) * (2 * L::kItemBytes) +
-            (is_v ? L::kItemBytes : 0);
-        PtExpect(full(s), L::kItemBytes);
-        PtBulk(sbase + s * L::kItemBytes, src, L::kItemBytes, full(s));
-        ++put;
-      };
-      for (int b = 0; ok && b <= nb; ++b) {
-        if (b < nb) copy(b, false);
-        if (ok && b >= 1) copy(b - 1, true);
+            (static_cast<int64_t>(w.tile.block0) * a.in.kv_heads + w.head) * (2 * L::kItemBytes);
+        const auto copy = [&](const uint8_t* src) {
+          const int s = put % kStages;
+          if (put >= kStages && !wait(empty(s), (put / kStages - 1) & 1)) {
+            give_up();
+            ok = false;
+            return;
+          }
+          PtExpect(full(s), L::kItemBytes);
+          PtBulk(sbase + s * L::kItemBytes, src, L::kItemBytes, full(s));
+          ++put;
+        };
+        const int64_t step = static_cast<int64_t>(a.in.kv_heads) * (2 * L::kItemBytes);
+        for (int b = 0; ok && b <= w.nb; ++b) {
+          if (b < w.nb) copy(image + b * step);
+          if (ok && b >= 1) copy(image + (b - 1) * step + L::kItemBytes);
+        }
       }
       if (!ok)  // what is in flight lands before the CTA ends
         for (int i = put > kStages ? put - kStages : 0; i < put; ++i)
@@ -775,63 +888,81 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------- products
-    if (lane == 0) {
-      bool ok = wait(q_full, 0);
-      if (!ok) give_up();
-      int get = 0;
-      for (int b = 0; ok && b <= nb; ++b) {
-        if (b < nb) {  // S_b = Q K_b^T
-          const int s = get % kStages;
-          if (!wait(full(s), (get / kStages) & 1)) {
-            give_up();
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          const uint32_t d = tmem + kPtSCol + 128 * (b & 1);
-          const uint32_t kh = sbase + s * L::kItemBytes, kl = kh + L::kItemBytes / 2;
-          const uint32_t qh = tmem + kPtQCol, ql = qh + HD / 2;
+    if (PtElect()) {
+      bool ok = true;
+      int get = 0, round = 0;
+      uint32_t s_count = 0, o_count = 0, q_count = 0;
+      for (PtWork w = PtFetch(a, total, round); ok && w.valid; w = PtFetch(a, total, round)) {
+        if (w.slow) continue;
+        ok = wait(q_full, q_count & 1);
+        ++q_count;
+        // The queue of products holds a few: the waits for what comes next are
+        // made before a group's last products are issued, so that the tensor
+        // core does not run dry meanwhile.
+        const auto k_ready = [&]() { return wait(full(get % kStages), (get / kStages) & 1); };
+        ok = ok && k_ready();
+        for (int b = 0; ok && b <= w.nb; ++b) {
+          const int s = get % kStages;  // K_b's stage, or the last V's
+          if (b < w.nb) {               // S_b = Q K_b^T
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const uint32_t d = tmem + kPtSCol + 128 * (s_count & 1);
+            const uint64_t kh = PtDesc(sbase + s * L::kItemBytes);
+            const uint64_t kl = PtAt(kh, L::kItemBytes / 2);
+            const uint32_t qh = tmem + kPtQCol, ql = qh + HD / 2;
 #pragma unroll
-          for (int j = 0; j < HD / 16; ++j) {
-            const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
-            PtMma(d, qh + 8 * j, PtDesc(kl + off), PtInstr(kPtKeys), j != 0 ? 1u : 0u);
-            PtMma(d, ql + 8 * j, PtDesc(kh + off), PtInstr(kPtKeys), 1u);
+            for (int j = 0; j < HD / 16; ++j) {
+              const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
+              PtMma(d, qh + 8 * j, PtAt(kl, off), PtInstr(kPtKeys), j != 0 ? 1u : 0u);
+              PtMma(d, ql + 8 * j, PtAt(kh, off), PtInstr(kPtKeys), 1u);
+            }
+            ++get;
           }
+          if (b >= 1)  // for O_(b - 1)
+            ok = k_ready() && wait(p_full(o_count & 1), (o_count >> 1) & 1) &&
+                 (o_count == 0 || wait(o_empty, (o_count - 1) & 1));
+          if (!ok) break;
+          if (b < w.nb) {
+            const uint32_t d = tmem + kPtSCol + 128 * (s_count & 1);
+            const uint64_t kh = PtDesc(sbase + s * L::kItemBytes);
+            const uint32_t qh = tmem + kPtQCol;
 #pragma unroll
-          for (int j = 0; j < HD / 16; ++j) {
-            const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
-            PtMma(d, qh + 8 * j, PtDesc(kh + off), PtInstr(kPtKeys), 1u);
+            for (int j = 0; j < HD / 16; ++j) {
+              const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
+              PtMma(d, qh + 8 * j, PtAt(kh, off), PtInstr(kPtKeys), 1u);
+            }
+            PtCommit(empty(s));
+            PtCommit(s_full(s_count & 1));
+            ++s_count;
           }
-          PtCommit(empty(s));
-          PtCommit(s_full(b & 1));
-          ++get;
+          if (b >= 1) {  // O_(b - 1) = P V
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const int sv = get % kStages;
+            const uint32_t d = tmem + kPtOCol, p = tmem + kPtSCol + 128 * (o_count & 1);
+            const uint64_t vh = PtDesc(sbase + sv * L::kItemBytes);
+            const uint64_t vl = PtAt(vh, L::kItemBytes / 2);
+            // 16 keys a step; P's pieces of 32 keys: 16 columns hi, 16 lo
+#pragma unroll
+            for (int j = 0; j < kPtKeys / 16; ++j) {
+              const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
+              const uint32_t ph = p + 32 * (j >> 1) + 8 * (j & 1), pl = ph + 16;
+              PtMma(d, ph, PtAt(vl, off), PtInstr(HD), j != 0 ? 1u : 0u);
+              PtMma(d, pl, PtAt(vh, off), PtInstr(HD), 1u);
+            }
+            ++get;
+            if (b + 1 < w.nb) ok = k_ready();
+#pragma unroll
+            for (int j = 0; j < kPtKeys / 16; ++j) {
+              const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
+              PtMma(d, p + 32 * (j >> 1) + 8 * (j & 1), PtAt(vh, off), PtInstr(HD), 1u);
+            }
+            PtCommit(empty(sv));
+            PtCommit(o_full);
+            ++o_count;
+          } else if (b + 1 < w.nb) {
+            ok = k_ready();
+          }
         }
-        if (b >= 1) {  // O_(b - 1) = P V
-          const int j0 = b - 1, s = get % kStages;
-          if (!wait(full(s), (get / kStages) & 1) || !wait(p_full(j0 & 3), (j0 >> 2) & 1) ||
-              (j0 >= 1 && !wait(o_empty, (j0 - 1) & 1))) {
-            give_up();
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          const uint32_t d = tmem + kPtOCol, p = tmem + kPtSCol + 128 * (j0 & 1);
-          const uint32_t vh = sbase + s * L::kItemBytes, vl = vh + L::kItemBytes / 2;
-          // 16 keys a step; P's pieces of 32 keys: 16 columns hi, 16 lo
-#pragma unroll
-          for (int j = 0; j < kPtKeys / 16; ++j) {
-            const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
-            const uint32_t ph = p + 32 * (j >> 1) + 8 * (j & 1), pl = ph + 16;
-            PtMma(d, ph, PtDesc(vl + off), PtInstr(HD), j != 0 ? 1u : 0u);
-            PtMma(d, pl, PtDesc(vh + off), PtInstr(HD), 1u);
-          }
-#pragma unroll
-          for (int j = 0; j < kPtKeys / 16; ++j) {
-            const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
-            PtMma(d, p + 32 * (j >> 1) + 8 * (j & 1), PtDesc(vh + off), PtInstr(HD), 1u);
-          }
-          PtCommit(empty(s));
-          PtCommit(o_full);
-          ++get;
-        }
+        if (!ok) give_up();
       }
       PtCommit(all_done);
       // what was issued has read its operands before tensor memory goes back
@@ -839,160 +970,260 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
     }
   } else {
     // -------------------------------------------------- softmax and output
-    const int group = warp >> 2;                       // 0: warps 0-3, 1: 4-7
-    const int v = (warp & 3) * 32 + lane;              // query vector
+    const int half = warp >> 2;
+    const int v = (warp & 3) * 32 + lane;  // query vector
     const int row = v / a.group;
-    const bool live = row < tile.rows && v < (kPtVectors / a.group) * a.group;
-    const int sees = live ? tile.sees + row : 0;
+    const bool used = v < (kPtVectors / a.group) * a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const int64_t at = ((tile.row0 + row) * static_cast<int64_t>(a.in.n_heads) + head * a.group +
-                        v % a.group) * HD;
-    float scale;  // of raw scores, to powers of two; without the key block's factor
-    {
-      const float4* q = reinterpret_cast<const float4*>(a.in.q + at);
+    // q and out are read and written by fours of lanes, 64 bytes of a vector
+    // at a time (16 bytes of 32 vectors would take four times the requests),
+    // and turned over between the four
+    int quad_row[4], quad_at[4];  // the four vectors: row of the tile, offset from its first
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int u = (v & ~3) + j;
+      quad_row[j] = u < (kPtVectors / a.group) * a.group ? u / a.group : kPtVectors;
+      quad_at[j] = (u / a.group * a.in.n_heads + u % a.group) * HD + half * HH + 4 * (lane & 3);
+    }
+    const auto first_of = [&](const PtWork& w) {  // of the tile in q and out
+      return (static_cast<int64_t>(w.tile.row0) * a.in.n_heads + w.head * a.group) * HD;
+    };
+    uint32_t swaps = 0;  // exchanges so far
+    bool ok = true;
+    // this half's value to the other half of the vector, and its value back
+    const auto exchange = [&](float x) __attribute__((always_inline)) {
+      float* at = swap + (swaps & 1) * 2 * kPtVectors + v;
+      at[half * kPtVectors] = x;
+      PtArrive(swapped(warp & 3));
+      ok = warp_wait(swapped(warp & 3), swaps & 1) && ok;
+      ++swaps;
+      return at[(1 - half) * kPtVectors];
+    };
+    // the tile's Q pieces into tensor memory; returns the factor from raw
+    // scores to powers of two, without the key block's
+    const auto write_q = [&](const PtWork& w) __attribute__((always_inline)) {
+      const float* q = a.in.q + first_of(w);
+      float4 x[HH / 4];
+#pragma unroll
+      for (int i = 0; i < HH / 4; ++i)
+        x[i] = quad_row[i & 3] < w.tile.rows
+                   ? *reinterpret_cast<const float4*>(q + quad_at[i & 3] + 16 * (i >> 2))
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
       float top = 0.0f;
-      if (live) {
-#pragma unroll 8
-        for (int i = 0; i < HD / 4; ++i) {
-          const float4 x = q[i];
-          const float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-          // a vector with Inf (or NaN) has NaN outputs whatever its scale
-          top = fmaxf(top, m < INFINITY ? m : 0.0f);
-        }
+#pragma unroll
+      for (int i = 0; i < HH / 16; ++i) PtTurn(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+#pragma unroll
+      for (int i = 0; i < HH / 4; ++i) {
+        const float m =
+            fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+        // a vector with Inf (or NaN) has NaN outputs whatever its scale
+        top = fmaxf(top, m < INFINITY ? m : 0.0f);
       }
+      top = fmaxf(top, exchange(top));
       float down;
       const float up = PtUp(top, down);
-      scale = a.in.scale * 1.4426950408889634f * down;
 #pragma unroll
       for (int c = 0; c < HH / 32; ++c) {  // 32 dimensions: 16 columns of each piece
         uint32_t out[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 x =
-              live ? q[group * (HH / 4) + 8 * c + i] : make_float4(0.f, 0.f, 0.f, 0.f);
-          PtSplit(x.x * up, x.y * up, out[2 * i], out[16 + 2 * i]);
-          PtSplit(x.z * up, x.w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
+          const float4 y = x[8 * c + i];
+          PtSplit(y.x * up, y.y * up, out[2 * i], out[16 + 2 * i]);
+          PtSplit(y.z * up, y.w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
         }
-        const uint32_t to = lanes + kPtQCol + group * (HH / 2) + 16 * c;
-#define PT_ST16(addr, o)                                                                        \
-  asm volatile(                                                                                 \
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"                                            \
-      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(addr), \
-      "r"(out[o]), "r"(out[o + 1]), "r"(out[o + 2]), "r"(out[o + 3]), "r"(out[o + 4]),           \
-      "r"(out[o + 5]), "r"(out[o + 6]), "r"(out[o + 7]), "r"(out[o + 8]), "r"(out[o + 9]),       \
-      "r"(out[o + 10]), "r"(out[o + 11]), "r"(out[o + 12]), "r"(out[o + 13]), "r"(out[o + 14]),  \
-      "r"(out[o + 15])                                                                          \
-      : "memory")
-        PT_ST16(to, 0);
-        PT_ST16(to + HD / 2, 16);
-#undef PT_ST16
+        const uint32_t to = lanes + kPtQCol + half * (HH / 2) + 16 * c;
+        PtSt16(to, out);
+        PtSt16(to + HD / 2, out + 16);
       }
       asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
       PtArrive(q_full);
-    }
-    float acc[HH];
+      return a.in.scale * 1.4426950408889634f * down;
+    };
+    int round = 0;
+    uint32_t s_count = 0, o_count = 0;
+    const auto advance = [&]() {
+      PtWork w = PtFetch(a, total, round);
+      while (w.valid && w.slow) w = PtFetch(a, total, round);
+      return w;
+    };
+    PtWork w = advance();
+    float scale = w.valid ? write_q(w) : 0.0f;
+    while (w.valid) {
+      const bool live = used && row < w.tile.rows;
+      const int sees = live ? w.tile.sees + row : 0;
+      const float2* factors =
+          a.factors + static_cast<int64_t>(w.tile.block0) * a.in.kv_heads + w.head;
+      PtWork next;
+      next.valid = false;
+      float next_scale = 0.0f;
+      uint64_t acc[HH / 2];  // pairs of dimensions
 #pragma unroll
-    for (int i = 0; i < HH; ++i) acc[i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    bool ok = true;
-    for (int b = 0; b <= nb; ++b) {
-      if (b < nb && (b & 1) == group) {
-        const float f = scale * factors[static_cast<int64_t>(b) * a.in.kv_heads].x;
-        if (!warp_wait(s_full(b & 1), (b >> 1) & 1)) {
-          give_up();
-          ok = false;
-          break;
-        }
+      for (int i = 0; i < HH / 2; ++i) acc[i] = 0;
+      float m = -INFINITY, l = 0.0f;
+      float m_of = 0.0f, sum_of = 0.0f, fv_of = 0.0f;  // of the block before
+      // O of the block before into the registers
+      const auto take = [&]() __attribute__((always_inline)) {
+        ok = ok && warp_wait(o_full, o_count & 1);
+        ++o_count;
+        if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const uint32_t s_at = lanes + kPtSCol + 128 * (b & 1);
-        const int seen = sees - b * kPtKeys;  // keys of the block that the row sees
-        const bool whole = b < partial0;      // the same for every thread
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t s[32];
-          PtLd32(s_at + 32 * c, s);
-          if (whole) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(s[j]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              top = fmaxf(top, 32 * c + j < seen ? __uint_as_float(s[j]) : -INFINITY);
-          }
-        }
-        // the reference is a whole power of two: 2^(m_b - M) is exact, and so
-        // is the subtraction's operand
-        const float mb = rintf(top * f);
-        const float minus = mb == -INFINITY ? 0.0f : -mb;  // nothing seen: p is 0
-        float sum = 0.0f;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t s[32];
-          PtLd32(s_at + 32 * c, s);
-          uint32_t out[32];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float p0 = PtExp2(fmaf(__uint_as_float(s[2 * j]), f, minus));
-            float p1 = PtExp2(fmaf(__uint_as_float(s[2 * j + 1]), f, minus));
-            if (!whole) {
-              if (32 * c + 2 * j >= seen) p0 = 0.0f;
-              if (32 * c + 2 * j + 1 >= seen) p1 = 0.0f;
-            }
-            sum += p0 + p1;
-            PtSplit(p0 * kPtPScale, p1 * kPtPScale, out[j], out[16 + j]);
-          }
-          PtSt32(s_at + 32 * c, out);
-        }
-        stat[(b & 3) * kPtVectors + v] = make_float2(mb, sum);
-        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        PtArrive(p_full(b & 3));
-      }
-      if (b >= 1) {
-        const int j = b - 1;
-        const float fv = fabsf(factors[static_cast<int64_t>(j) * a.in.kv_heads].y);
-        if (!warp_wait(p_full(j & 3), (j >> 2) & 1) || !warp_wait(o_full, j & 1)) {
-          give_up();
-          ok = false;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const float2 st = stat[(j & 3) * kPtVectors + v];
-        const float m_new = fmaxf(m, st.x);
+        const float m_new = fmaxf(m, m_of);
         const float keep = m == m_new ? 1.0f : PtExp2(m - m_new);
-        const float weight = st.x == -INFINITY ? 0.0f : PtExp2(st.x - m_new);
-        const float add = weight * (fv * (1.0f / kPtPScale));
-        l = st.x == -INFINITY ? l + st.y : fmaf(l, keep, st.y * weight);
+        const float weight = m_of == -INFINITY ? 0.0f : PtExp2(m_of - m_new);
+        const float add = weight * (fv_of * (1.0f / kPtPScale));
+        l = m_of == -INFINITY ? l + sum_of : fmaf(l, keep, sum_of * weight);
         m = m_new;
+        const uint64_t keep2 = PtPair(keep, keep), add2 = PtPair(add, add);
 #pragma unroll
         for (int c = 0; c < HH / 32; ++c) {
           uint32_t o[32];
-          PtLd32(lanes + kPtOCol + group * HH + 32 * c, o);
+          PtLd32(lanes + kPtOCol + half * HH + 32 * c, o);
+          PtLdWait(o);
+          if (c + 1 == HH / 32) {
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            PtArrive(o_empty);
+          }
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            acc[32 * c + i] = fmaf(acc[32 * c + i], keep, __uint_as_float(o[i]) * add);
+          for (int i = 0; i < 16; ++i)
+            acc[16 * c + i] = PtFma2(
+                acc[16 * c + i], keep2,
+                PtMul2(PtPair(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), add2));
         }
-        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        PtArrive(o_empty);
-      }
-    }
-    if (live) {
-      float4* o = reinterpret_cast<float4*>(a.in.out + at + group * HH);
-      const float inv = 1.0f / l;
+      };
+      float2 f_next = factors[0];
+      for (int b = 0; b < w.nb; ++b) {
+        const float2 ff = f_next;
+        if (b + 1 < w.nb) f_next = factors[static_cast<int64_t>(b + 1) * a.in.kv_heads];
+        // at least the smallest normal number: a score of -inf stays one
+        const float f = fmaxf(scale * ff.x, 1.17549435e-38f);
+        ok = ok && warp_wait(s_full(s_count & 1), (s_count >> 1) & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const uint32_t s_at = lanes + kPtSCol + 128 * (s_count & 1) + 64 * half;
+        // 32 scores; those of keys that the row does not see are -inf
+        const int seen = sees - b * kPtKeys - 64 * half;
+        const bool whole = b < w.partial0;  // the same for every thread
+        const auto scores = [&](int c, uint32_t(&s)[32]) __attribute__((always_inline)) {
+          PtLd32(s_at + 32 * c, s);
+          PtLdWait(s);
+          if (!whole) {
 #pragma unroll
-      for (int i = 0; i < HH / 4; ++i) {
-        float4 y = make_float4(acc[4 * i] * inv, acc[4 * i + 1] * inv, acc[4 * i + 2] * inv,
-                               acc[4 * i + 3] * inv);
-        if (sees <= 0) y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!ok) y = make_float4(NAN, NAN, NAN, NAN);
-        o[i] = y;
+            for (int j = 0; j < 32; ++j)
+              if (32 * c + j >= seen) s[j] = 0xff800000u;
+          }
+        };
+        float t0 = -INFINITY, t1 = t0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32];
+          scores(c, s);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            t0 = PtMax3(t0, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+            t1 = PtMax3(t1, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
+          }
+        }
+        float top = fmaxf(t0, t1);
+        top = fmaxf(top, exchange(top));
+        if (!ok) break;
+        // the reference is a whole power of two: 2^(m_b - M) is exact, and so
+        // is the summand below, which also brings p to its 2^14
+        const float mb = rintf(top * f);
+        const float plus = mb == -INFINITY ? 0.0f : 14.0f - mb;  // nothing seen: p is 0
+        const uint64_t f2 = PtPair(f, f), plus2 = PtPair(plus, plus);
+        uint64_t sum_a = PtPair(0.0f, 0.0f), sum_b = sum_a;
+        // the scores are read again: held over the exchange they would not
+        // fit the registers beside the output
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32], out[32];
+          scores(c, s);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float p0, p1;
+            PtUnpair(PtFma2(PtPair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), f2,
+                            plus2),
+                     p0, p1);
+            p0 = PtExp2(p0);
+            p1 = PtExp2(p1);
+            const uint64_t p = PtPair(p0, p1);
+            if ((i & 1) == 0) sum_a = PtAdd2(sum_a, p);
+            else sum_b = PtAdd2(sum_b, p);
+            uint32_t hi, lo;
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(hi) : "f"(p1), "f"(p0));
+            float h0, h1;
+            asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n"
+                " cvt.f32.f16 %1, b;\n}\n"
+                : "=f"(h0), "=f"(h1)
+                : "r"(hi));
+            PtUnpair(PtFma2(PtPair(h0, h1), PtPair(-1.0f, -1.0f), p), h0, h1);
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(lo) : "f"(h1), "f"(h0));
+            out[i] = hi;
+            out[16 + i] = lo;
+          }
+          PtSt32(s_at + 32 * c, out);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        PtArrive(p_full(s_count & 1));
+        ++s_count;
+        if (b >= 1) take();
+        if (b + 1 == w.nb) {  // every product with Q has run
+          next = advance();
+          if (next.valid) next_scale = write_q(next);
+        }
+        float x, y;
+        PtUnpair(PtAdd2(sum_a, sum_b), x, y);
+        m_of = mb;
+        sum_of = x + y;
+        fv_of = fabsf(ff.y);
       }
+      if (ok) take();
+      if (ok) l += exchange(l);
+      const float inv = sees > 0 ? kPtPScale / l : 0.0f;
+      if (sees <= 0)
+#pragma unroll
+        for (int i = 0; i < HH / 2; ++i) acc[i] = 0;
+      float* out = a.in.out + first_of(w);
+#pragma unroll
+      for (int i = 0; i < HH / 16; ++i) {
+        float4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          PtUnpair(PtMul2(acc[8 * i + 2 * j], PtPair(inv, inv)), x[j].x, x[j].y);
+          PtUnpair(PtMul2(acc[8 * i + 2 * j + 1], PtPair(inv, inv)), x[j].z, x[j].w);
+        }
+        PtTurn(x[0], x[1], x[2], x[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (quad_row[j] < w.tile.rows)
+            *reinterpret_cast<float4*>(out + quad_at[j] + 16 * i) = x[j];
+      }
+      if (!ok) {
+        give_up();
+        break;
+      }
+      w = next;
+      scale = next_scale;
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
+  // tiles for the CUDA cores; after a wait gave up all tiles, as NaN
+  const bool gave_up = *abort_flag != 0, some_slow = *slow_flag != 0;
+  int round = 0;
+  PtWork w;
+  while ((gave_up || some_slow) && (w = PtFetch(a, total, round)).valid) {
+    if (gave_up) {
+      const int64_t at = (w.tile.row0 * static_cast<int64_t>(a.in.n_heads) + w.head * a.group) * HD;
+      for (int i = threadIdx.x; i < w.tile.rows * a.group * HD; i += kPtThreads)
+        a.in.out[at + i / (a.group * HD) * static_cast<int64_t>(a.in.n_heads) * HD +
+                 i % (a.group * HD)] = NAN;
+    } else if (w.slow) {
+      PtSlowTile<HD>(a, w.tile, w.head);
+    }
+  }
   if (warp == 9) {
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
@@ -1012,7 +1243,8 @@ int LaunchPkTc(const PtArgs& a, cudaStream_t s) {
   Launch(PkSplitKernel<HD>,
          dim3(static_cast<unsigned>(a.max_blocks + 1), static_cast<unsigned>(a.in.kv_heads), 2),
          kPtSplitThreads, 0, s, a);
-  Launch(PkTcKernel<HD>, dim3(static_cast<unsigned>(a.max_tiles * a.in.kv_heads)), kPtThreads,
+  const int64_t most = a.max_tiles * a.in.kv_heads, sms = SmCount();
+  Launch(PkTcKernel<HD>, dim3(static_cast<unsigned>(most < sms ? most : sms)), kPtThreads,
          static_cast<size_t>(smem), s, a);
   return MLB_OK;
 }
