@@ -210,7 +210,7 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
 // first.
 //
 // Second launch (PkTcKernel).  One CTA per SM takes tiles of 128 query vectors
-// (128 / G rows x G heads of a kv head) from the list; 320 threads:
+// (128 / G rows x G heads of a kv head) from the list; 384 threads:
 //   - warps 0-3 and 4-7: thread = (query vector = tensor-memory lane, half).
 //     They write the tile's Q pieces into tensor memory; per block each takes
 //     64 keys of its vector's scores, the two halves exchange their maxima
@@ -222,7 +222,8 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
 //   - warp 8: bulk copies, K_0, K_1, V_0, K_2, V_1, ... through a ring, on into
 //     the next tile;
 //   - warp 9: tensor memory; one lane issues S_(b + 1), then O_b, so that the
-//     softmax of a block runs under the products of its neighbours.
+//     softmax of a block runs under the products of its neighbours;
+//   - warps 10-11 only complete the warpgroup that gives up registers.
 // Tensor memory: Q hi and lo, two S / P buffers, O.  All waits are bounded; a
 // CTA whose wait gave up writes NaN and is counted (mlb_wait_timeouts).
 //
@@ -234,7 +235,11 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
 
 constexpr int kPtKeys = 128;
 constexpr int kPtVectors = 128;
-constexpr int kPtThreads = 320;
+constexpr int kPtThreads = 384;
+// Registers: 168 a thread at launch (384 x 168 = 64512); the copying and
+// issuing warpgroup gives up what the other two take, 256 x 216 + 128 x 72.
+constexpr int kPtRegsMath = 216;
+constexpr int kPtRegsIssue = 72;
 constexpr int kPtTmemColumns = 512;
 constexpr int kPtQCol = 0;      // Q hi, Q lo: hd / 2 columns each
 constexpr int kPtSCol = 128;    // two buffers of 128 columns
@@ -852,11 +857,25 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
     return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
   };
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kPtRegsIssue));
   if (warp == 8) {
     // --------------------------------------------------------------- copies
     if (PtElect()) {
       int put = 0, round = 0;
       bool ok = true;
+      const uint8_t* v_due = nullptr;  // the block before's V comes after this block's K
+      const auto copy = [&](const uint8_t* src) {
+        const int s = put % kStages;
+        if (put >= kStages && !wait(empty(s), (put / kStages - 1) & 1)) {
+          give_up();
+          ok = false;
+          return;
+        }
+        PtExpect(full(s), L::kItemBytes);
+        PtBulk(sbase + s * L::kItemBytes, src, L::kItemBytes, full(s));
+        ++put;
+      };
       for (PtWork w = PtFetch(a, total, round); ok && w.valid; w = PtFetch(a, total, round)) {
         if (w.slow) {
           *slow_flag = 1;
@@ -865,23 +884,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
         const uint8_t* image =
             a.images +
             (static_cast<int64_t>(w.tile.block0) * a.in.kv_heads + w.head) * (2 * L::kItemBytes);
-        const auto copy = [&](const uint8_t* src) {
-          const int s = put % kStages;
-          if (put >= kStages && !wait(empty(s), (put / kStages - 1) & 1)) {
-            give_up();
-            ok = false;
-            return;
-          }
-          PtExpect(full(s), L::kItemBytes);
-          PtBulk(sbase + s * L::kItemBytes, src, L::kItemBytes, full(s));
-          ++put;
-        };
         const int64_t step = static_cast<int64_t>(a.in.kv_heads) * (2 * L::kItemBytes);
-        for (int b = 0; ok && b <= w.nb; ++b) {
-          if (b < w.nb) copy(image + b * step);
-          if (ok && b >= 1) copy(image + (b - 1) * step + L::kItemBytes);
+        for (int b = 0; ok && b < w.nb; ++b) {
+          copy(image + b * step);
+          if (ok && v_due != nullptr) copy(v_due);
+          v_due = image + b * step + L::kItemBytes;
         }
       }
+      if (ok && v_due != nullptr) copy(v_due);
       if (!ok)  // what is in flight lands before the CTA ends
         for (int i = put > kStages ? put - kStages : 0; i < put; ++i)
           PtWait(full(i % kStages), (i / kStages) & 1);
@@ -889,86 +899,106 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
   } else if (warp == 9) {
     // ------------------------------------------------------------- products
     if (PtElect()) {
-      bool ok = true;
+      bool ok = true, due = false;  // due: O of the block before is still to come
       int get = 0, round = 0;
       uint32_t s_count = 0, o_count = 0, q_count = 0;
-      for (PtWork w = PtFetch(a, total, round); ok && w.valid; w = PtFetch(a, total, round)) {
-        if (w.slow) continue;
-        ok = wait(q_full, q_count & 1);
-        ++q_count;
-        // The queue of products holds a few: the waits for what comes next are
-        // made before a group's last products are issued, so that the tensor
-        // core does not run dry meanwhile.
-        const auto k_ready = [&]() { return wait(full(get % kStages), (get / kStages) & 1); };
-        ok = ok && k_ready();
-        for (int b = 0; ok && b <= w.nb; ++b) {
-          const int s = get % kStages;  // K_b's stage, or the last V's
-          if (b < w.nb) {               // S_b = Q K_b^T
-            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            const uint32_t d = tmem + kPtSCol + 128 * (s_count & 1);
-            const uint64_t kh = PtDesc(sbase + s * L::kItemBytes);
-            const uint64_t kl = PtAt(kh, L::kItemBytes / 2);
-            const uint32_t qh = tmem + kPtQCol, ql = qh + HD / 2;
+      // The queue of products holds a few: waits for what comes next are made
+      // before a group's last products are issued, so that the tensor core
+      // does not run dry meanwhile.
+      const auto item_ready = [&]() { return wait(full(get % kStages), (get / kStages) & 1); };
+      const auto fast = [&]() {
+        PtWork w = PtFetch(a, total, round);
+        while (w.valid && w.slow) w = PtFetch(a, total, round);
+        return w;
+      };
+      const auto s_part = [&](int s, bool cross) __attribute__((always_inline)) {
+        const uint32_t d = tmem + kPtSCol + 128 * (s_count & 1);
+        const uint64_t kh = PtDesc(sbase + s * L::kItemBytes);
+        const uint64_t kl = PtAt(kh, L::kItemBytes / 2);
+        const uint32_t qh = tmem + kPtQCol, ql = qh + HD / 2;
 #pragma unroll
-            for (int j = 0; j < HD / 16; ++j) {
-              const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
-              PtMma(d, qh + 8 * j, PtAt(kl, off), PtInstr(kPtKeys), j != 0 ? 1u : 0u);
-              PtMma(d, ql + 8 * j, PtAt(kh, off), PtInstr(kPtKeys), 1u);
-            }
-            ++get;
-          }
-          if (b >= 1)  // for O_(b - 1)
-            ok = k_ready() && wait(p_full(o_count & 1), (o_count >> 1) & 1) &&
-                 (o_count == 0 || wait(o_empty, (o_count - 1) & 1));
-          if (!ok) break;
-          if (b < w.nb) {
-            const uint32_t d = tmem + kPtSCol + 128 * (s_count & 1);
-            const uint64_t kh = PtDesc(sbase + s * L::kItemBytes);
-            const uint32_t qh = tmem + kPtQCol;
-#pragma unroll
-            for (int j = 0; j < HD / 16; ++j) {
-              const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
-              PtMma(d, qh + 8 * j, PtAt(kh, off), PtInstr(kPtKeys), 1u);
-            }
-            PtCommit(empty(s));
-            PtCommit(s_full(s_count & 1));
-            ++s_count;
-          }
-          if (b >= 1) {  // O_(b - 1) = P V
-            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            const int sv = get % kStages;
-            const uint32_t d = tmem + kPtOCol, p = tmem + kPtSCol + 128 * (o_count & 1);
-            const uint64_t vh = PtDesc(sbase + sv * L::kItemBytes);
-            const uint64_t vl = PtAt(vh, L::kItemBytes / 2);
-            // 16 keys a step; P's pieces of 32 keys: 16 columns hi, 16 lo
-#pragma unroll
-            for (int j = 0; j < kPtKeys / 16; ++j) {
-              const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
-              const uint32_t ph = p + 32 * (j >> 1) + 8 * (j & 1), pl = ph + 16;
-              PtMma(d, ph, PtAt(vl, off), PtInstr(HD), j != 0 ? 1u : 0u);
-              PtMma(d, pl, PtAt(vh, off), PtInstr(HD), 1u);
-            }
-            ++get;
-            if (b + 1 < w.nb) ok = k_ready();
-#pragma unroll
-            for (int j = 0; j < kPtKeys / 16; ++j) {
-              const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
-              PtMma(d, p + 32 * (j >> 1) + 8 * (j & 1), PtAt(vh, off), PtInstr(HD), 1u);
-            }
-            PtCommit(empty(sv));
-            PtCommit(o_full);
-            ++o_count;
-          } else if (b + 1 < w.nb) {
-            ok = k_ready();
+        for (int j = 0; j < HD / 16; ++j) {
+          const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
+          if (cross) {
+            PtMma(d, qh + 8 * j, PtAt(kl, off), PtInstr(kPtKeys), j != 0 ? 1u : 0u);
+            PtMma(d, ql + 8 * j, PtAt(kh, off), PtInstr(kPtKeys), 1u);
+          } else {
+            PtMma(d, qh + 8 * j, PtAt(kh, off), PtInstr(kPtKeys), 1u);
           }
         }
-        if (!ok) give_up();
+      };
+      const auto o_part = [&](int s, bool cross) __attribute__((always_inline)) {
+        const uint32_t d = tmem + kPtOCol, p = tmem + kPtSCol + 128 * (o_count & 1);
+        const uint64_t vh = PtDesc(sbase + s * L::kItemBytes);
+        const uint64_t vl = PtAt(vh, L::kItemBytes / 2);
+        // 16 keys a step; P's pieces of 32 keys: 16 columns hi, 16 lo
+#pragma unroll
+        for (int j = 0; j < kPtKeys / 16; ++j) {
+          const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
+          const uint32_t ph = p + 32 * (j >> 1) + 8 * (j & 1), pl = ph + 16;
+          if (cross) {
+            PtMma(d, ph, PtAt(vl, off), PtInstr(HD), j != 0 ? 1u : 0u);
+            PtMma(d, pl, PtAt(vh, off), PtInstr(HD), 1u);
+          } else {
+            PtMma(d, ph, PtAt(vh, off), PtInstr(HD), 1u);
+          }
+        }
+      };
+      PtWork w = fast();
+      int b = 0;
+      if (w.valid) ok = wait(q_full, 0) && item_ready();
+      ++q_count;
+      while (ok && (w.valid || due)) {
+        const bool more = w.valid;  // a block whose scores are to come
+        const int sk = get % kStages;
+        if (more) {  // S = Q K^T of this block
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          s_part(sk, true);
+          ++get;
+          if (due) ok = item_ready() && wait(p_full(o_count & 1), (o_count >> 1) & 1);
+          if (!ok) break;
+          s_part(sk, false);
+          PtCommit(s_full(s_count & 1));
+          PtCommit(empty(sk));
+          ++s_count;
+          if (++b == w.nb) {
+            w = fast();
+            b = 0;
+          }
+        } else {
+          ok = item_ready() && wait(p_full(o_count & 1), (o_count >> 1) & 1);
+        }
+        const bool next_q = more && w.valid && b == 0;  // the next block is another tile's
+        if (due) {  // O = P V of the block before
+          ok = ok && (o_count == 0 || wait(o_empty, (o_count - 1) & 1));
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          const int sv = get % kStages;
+          o_part(sv, true);
+          ++get;
+          if (w.valid && !next_q) ok = item_ready();
+          if (!ok) break;
+          o_part(sv, false);
+          PtCommit(o_full);
+          PtCommit(empty(sv));
+          ++o_count;
+        } else if (w.valid && !next_q) {
+          ok = item_ready();
+        }
+        if (next_q) {
+          ok = ok && wait(q_full, q_count & 1) && item_ready();
+          ++q_count;
+        }
+        due = more;
       }
+      if (!ok) give_up();
       PtCommit(all_done);
       // what was issued has read its operands before tensor memory goes back
       if (!PtWait(all_done, 0)) give_up();
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kPtRegsMath));
     // -------------------------------------------------- softmax and output
     const int half = warp >> 2;
     const int v = (warp & 3) * 32 + lane;  // query vector
@@ -1042,108 +1072,144 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
     };
     int round = 0;
     uint32_t s_count = 0, o_count = 0;
-    const auto advance = [&]() {
+    const auto fast = [&]() {
       PtWork w = PtFetch(a, total, round);
       while (w.valid && w.slow) w = PtFetch(a, total, round);
       return w;
     };
-    PtWork w = advance();
-    float scale = w.valid ? write_q(w) : 0.0f;
-    while (w.valid) {
-      const bool live = used && row < w.tile.rows;
-      const int sees = live ? w.tile.sees + row : 0;
-      const float2* factors =
-          a.factors + static_cast<int64_t>(w.tile.block0) * a.in.kv_heads + w.head;
-      PtWork next;
-      next.valid = false;
-      float next_scale = 0.0f;
-      uint64_t acc[HH / 2];  // pairs of dimensions
+    // the output of the block before's tile, and that block's reference, sum
+    // and factor of V
+    uint64_t acc[HH / 2];  // pairs of dimensions
+#pragma unroll
+    for (int i = 0; i < HH / 2; ++i) acc[i] = 0;
+    float m = -INFINITY, l = 0.0f;
+    float m_of = 0.0f, sum_of = 0.0f, fv_of = 0.0f;
+    float* out_of = nullptr;
+    int rows_of = 0;
+    bool sees_of = false;
+    const auto take = [&]() __attribute__((always_inline)) {
+      ok = ok && warp_wait(o_full, o_count & 1);
+      ++o_count;
+      if (!ok) return;
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      uint32_t o[HH];
+#pragma unroll
+      for (int c = 0; c < HH / 32; ++c) PtLd32(lanes + kPtOCol + half * HH + 32 * c, o + 32 * c);
+      const float m_new = fmaxf(m, m_of);
+      const float keep = m == m_new ? 1.0f : PtExp2(m - m_new);
+      const float weight = m_of == -INFINITY ? 0.0f : PtExp2(m_of - m_new);
+      const float add = weight * (fv_of * (1.0f / kPtPScale));
+      l = m_of == -INFINITY ? l + sum_of : fmaf(l, keep, sum_of * weight);
+      m = m_new;
+      const uint64_t keep2 = PtPair(keep, keep), add2 = PtPair(add, add);
+      PtLdWait(o);
+      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      PtArrive(o_empty);
+#pragma unroll
+      for (int i = 0; i < HH / 2; ++i)
+        acc[i] = PtFma2(
+            acc[i], keep2,
+            PtMul2(PtPair(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), add2));
+    };
+    const auto finish = [&]() __attribute__((always_inline)) {
+      l += exchange(l);
+      if (!ok) return;
+      const float inv = sees_of ? kPtPScale / l : 0.0f;
+      if (!sees_of)
+#pragma unroll
+        for (int i = 0; i < HH / 2; ++i) acc[i] = 0;
+#pragma unroll
+      for (int i = 0; i < HH / 16; ++i) {
+        float4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          PtUnpair(PtMul2(acc[8 * i + 2 * j], PtPair(inv, inv)), x[j].x, x[j].y);
+          PtUnpair(PtMul2(acc[8 * i + 2 * j + 1], PtPair(inv, inv)), x[j].z, x[j].w);
+        }
+        PtTurn(x[0], x[1], x[2], x[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (quad_row[j] < rows_of)
+            *reinterpret_cast<float4*>(out_of + quad_at[j] + 16 * i) = x[j];
+      }
 #pragma unroll
       for (int i = 0; i < HH / 2; ++i) acc[i] = 0;
-      float m = -INFINITY, l = 0.0f;
-      float m_of = 0.0f, sum_of = 0.0f, fv_of = 0.0f;  // of the block before
-      // O of the block before into the registers
-      const auto take = [&]() __attribute__((always_inline)) {
-        ok = ok && warp_wait(o_full, o_count & 1);
-        ++o_count;
-        if (!ok) return;
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const float m_new = fmaxf(m, m_of);
-        const float keep = m == m_new ? 1.0f : PtExp2(m - m_new);
-        const float weight = m_of == -INFINITY ? 0.0f : PtExp2(m_of - m_new);
-        const float add = weight * (fv_of * (1.0f / kPtPScale));
-        l = m_of == -INFINITY ? l + sum_of : fmaf(l, keep, sum_of * weight);
-        m = m_new;
-        const uint64_t keep2 = PtPair(keep, keep), add2 = PtPair(add, add);
-#pragma unroll
-        for (int c = 0; c < HH / 32; ++c) {
-          uint32_t o[32];
-          PtLd32(lanes + kPtOCol + half * HH + 32 * c, o);
-          PtLdWait(o);
-          if (c + 1 == HH / 32) {
-            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-            PtArrive(o_empty);
+      m = -INFINITY;
+      l = 0.0f;
+    };
+    PtWork w = fast(), next;
+    next.valid = false;
+    float scale = w.valid ? write_q(w) : 0.0f;
+    const auto factor = [&](const PtWork& x, int block) {
+      return a.factors[(static_cast<int64_t>(x.tile.block0) + block) * a.in.kv_heads + x.head];
+    };
+    float2 ff_next = w.valid ? factor(w, 0) : make_float2(0.0f, 0.0f);
+    int b = 0;
+    bool due = false;  // a block whose output is still to come
+#pragma unroll 1
+    while (ok && (w.valid || due)) {
+      const bool more = w.valid;
+      float mb = 0.0f, sum = 0.0f, fv = 0.0f;
+      const bool first = b == 0;
+      if (more) {
+        const float2 ff = ff_next;
+        const int sees = used && row < w.tile.rows ? w.tile.sees + row : 0;
+        if (first) {
+          next = fast();
+          if (next.valid && used && row < next.tile.rows) {  // its q on the way to L2
+            const float* q = a.in.q + first_of(next) + row * a.in.n_heads * HD +
+                             v % a.group * HD + half * HH;
+            asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q));
+            asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + HH - 4));
           }
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            acc[16 * c + i] = PtFma2(
-                acc[16 * c + i], keep2,
-                PtMul2(PtPair(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), add2));
         }
-      };
-      float2 f_next = factors[0];
-      for (int b = 0; b < w.nb; ++b) {
-        const float2 ff = f_next;
-        if (b + 1 < w.nb) f_next = factors[static_cast<int64_t>(b + 1) * a.in.kv_heads];
         // at least the smallest normal number: a score of -inf stays one
         const float f = fmaxf(scale * ff.x, 1.17549435e-38f);
-        ok = ok && warp_wait(s_full(s_count & 1), (s_count >> 1) & 1);
+        fv = fabsf(ff.y);
+        ff_next = b + 1 < w.nb ? factor(w, b + 1) : next.valid ? factor(next, 0) : ff;
+        ok = warp_wait(s_full(s_count & 1), (s_count >> 1) & 1);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        // all products with this tile's Q have run: the next tile's, so that
+        // its first scores are computed during this block's softmax
+        if (b + 1 == w.nb && next.valid) scale = write_q(next);
         const uint32_t s_at = lanes + kPtSCol + 128 * (s_count & 1) + 64 * half;
-        // 32 scores; those of keys that the row does not see are -inf
-        const int seen = sees - b * kPtKeys - 64 * half;
-        const bool whole = b < w.partial0;  // the same for every thread
-        const auto scores = [&](int c, uint32_t(&s)[32]) __attribute__((always_inline)) {
-          PtLd32(s_at + 32 * c, s);
-          PtLdWait(s);
-          if (!whole) {
+        uint32_t s[64];
+        PtLd32(s_at, s);
+        PtLd32(s_at + 32, s + 32);
+        PtLdWait(s);
+        if (b >= w.partial0) {  // the same for every thread
+          const int seen = sees - b * kPtKeys - 64 * half;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (32 * c + j >= seen) s[j] = 0xff800000u;
-          }
-        };
-        float t0 = -INFINITY, t1 = t0;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t s[32];
-          scores(c, s);
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            t0 = PtMax3(t0, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-            t1 = PtMax3(t1, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
-          }
+          for (int j = 0; j < 64; ++j)
+            if (j >= seen) s[j] = 0xff800000u;  // keys that the row does not see: -inf
         }
-        float top = fmaxf(t0, t1);
+        float t0 = -INFINITY, t1 = t0, t2 = t0, t3 = t0;
+#pragma unroll
+        for (int j = 0; j < 64; j += 8) {
+          t0 = PtMax3(t0, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+          t1 = PtMax3(t1, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
+          t2 = PtMax3(t2, __uint_as_float(s[j + 4]), __uint_as_float(s[j + 5]));
+          t3 = PtMax3(t3, __uint_as_float(s[j + 6]), __uint_as_float(s[j + 7]));
+        }
+        float top = PtMax3(fmaxf(t0, t1), t2, t3);
         top = fmaxf(top, exchange(top));
         if (!ok) break;
         // the reference is a whole power of two: 2^(m_b - M) is exact, and so
         // is the summand below, which also brings p to its 2^14
-        const float mb = rintf(top * f);
+        mb = rintf(top * f);
         const float plus = mb == -INFINITY ? 0.0f : 14.0f - mb;  // nothing seen: p is 0
         const uint64_t f2 = PtPair(f, f), plus2 = PtPair(plus, plus);
         uint64_t sum_a = PtPair(0.0f, 0.0f), sum_b = sum_a;
-        // the scores are read again: held over the exchange they would not
-        // fit the registers beside the output
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t s[32], out[32];
-          scores(c, s);
+          uint32_t out[32];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float p0, p1;
-            PtUnpair(PtFma2(PtPair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), f2,
-                            plus2),
+            PtUnpair(PtFma2(PtPair(__uint_as_float(s[32 * c + 2 * i]),
+                                   __uint_as_float(s[32 * c + 2 * i + 1])),
+                            f2, plus2),
                      p0, p1);
             p0 = PtExp2(p0);
             p1 = PtExp2(p1);
@@ -1168,45 +1234,30 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
         PtArrive(p_full(s_count & 1));
         ++s_count;
-        if (b >= 1) take();
-        if (b + 1 == w.nb) {  // every product with Q has run
-          next = advance();
-          if (next.valid) next_scale = write_q(next);
-        }
         float x, y;
         PtUnpair(PtAdd2(sum_a, sum_b), x, y);
-        m_of = mb;
-        sum_of = x + y;
-        fv_of = fabsf(ff.y);
+        sum = x + y;
       }
-      if (ok) take();
-      if (ok) l += exchange(l);
-      const float inv = sees > 0 ? kPtPScale / l : 0.0f;
-      if (sees <= 0)
-#pragma unroll
-        for (int i = 0; i < HH / 2; ++i) acc[i] = 0;
-      float* out = a.in.out + first_of(w);
-#pragma unroll
-      for (int i = 0; i < HH / 16; ++i) {
-        float4 x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          PtUnpair(PtMul2(acc[8 * i + 2 * j], PtPair(inv, inv)), x[j].x, x[j].y);
-          PtUnpair(PtMul2(acc[8 * i + 2 * j + 1], PtPair(inv, inv)), x[j].z, x[j].w);
-        }
-        PtTurn(x[0], x[1], x[2], x[3]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (quad_row[j] < w.tile.rows)
-            *reinterpret_cast<float4*>(out + quad_at[j] + 16 * i) = x[j];
+      if (due) {
+        take();
+        if (ok && (first || !more)) finish();
       }
-      if (!ok) {
-        give_up();
-        break;
+      if (!ok) break;
+      if (more && first) {
+        out_of = a.in.out + first_of(w);
+        rows_of = w.tile.rows;
+        sees_of = used && row < w.tile.rows && w.tile.sees + row > 0;
       }
-      w = next;
-      scale = next_scale;
+      m_of = mb;
+      sum_of = sum;
+      fv_of = fv;
+      due = more;
+      if (more && ++b == w.nb) {
+        w = next;
+        b = 0;
+      }
     }
+    if (!ok) give_up();
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
