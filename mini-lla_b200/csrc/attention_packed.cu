@@ -210,20 +210,22 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
 // first.
 //
 // Second launch (PkTcKernel).  One CTA per SM takes tiles of 128 query vectors
-// (128 / G rows x G heads of a kv head) from the list; 384 threads:
-//   - warps 0-3 and 4-7: thread = (query vector = tensor-memory lane, half).
-//     They write the tile's Q pieces into tensor memory; per block each takes
-//     64 keys of its vector's scores, the two halves exchange their maxima
-//     through shared memory, and p = 2^(s - m_b) goes back over S as pieces,
-//     with the block's own reference m_b, rounded to a whole power of two.
-//     Then O_(b - 1), half of the dimensions each, joins the registers: acc =
-//     acc 2^(M - M') + O 2^(m - M'), both factors exact.  The next tile's Q
-//     is written before the last block's output is taken.
-//   - warp 8: bulk copies, K_0, K_1, V_0, K_2, V_1, ... through a ring, on into
+// (128 / G rows x G heads of a kv head) from the list; 512 threads:
+//   - warps 0-3 and 4-7: softmax.  Thread = (query vector = tensor-memory
+//     lane, half of a block's keys); the halves exchange their maxima through
+//     shared memory, and p = 2^(s - m_b) goes over S as pieces, with the
+//     block's own reference m_b, rounded to a whole power of two, so that a
+//     block's softmax needs no other's;
+//   - warps 8-11: output.  Thread = query vector: O_b joins the registers,
+//     acc = acc 2^(M - M') + O 2^(m_b - M'), both factors exact.  They also
+//     write the tiles' Q pieces into tensor memory, the next tile's while the
+//     softmax of a tile's last block runs;
+//   - warp 12: bulk copies, K_0, K_1, V_0, K_2, V_1, ... through a ring, on into
 //     the next tile;
-//   - warp 9: tensor memory; one lane issues S_(b + 1), then O_b, so that the
-//     softmax of a block runs under the products of its neighbours;
-//   - warps 10-11 only complete the warpgroup that gives up registers.
+//   - warp 13: tensor memory; one lane issues S_(b + 1), then O_b (O first where
+//     S is the next tile's), so that the softmax of a block runs under the
+//     products of its neighbours;
+//   - warps 14-15 only complete the warpgroup that gives up registers.
 // Tensor memory: Q hi and lo, two S / P buffers, O.  All waits are bounded; a
 // CTA whose wait gave up writes NaN and is counted (mlb_wait_timeouts).
 //
@@ -235,11 +237,11 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
 
 constexpr int kPtKeys = 128;
 constexpr int kPtVectors = 128;
-constexpr int kPtThreads = 384;
-// Registers: 168 a thread at launch (384 x 168 = 64512); the copying and
-// issuing warpgroup gives up what the other two take, 256 x 216 + 128 x 72.
-constexpr int kPtRegsMath = 216;
-constexpr int kPtRegsIssue = 72;
+constexpr int kPtThreads = 512;
+// Registers: 128 a thread at launch (65536); the copying and issuing
+// warpgroup gives up what the output's takes: 256 x 128 + 128 x 200 + 128 x 56.
+constexpr int kPtRegsOutput = 200;
+constexpr int kPtRegsIssue = 56;
 constexpr int kPtTmemColumns = 512;
 constexpr int kPtQCol = 0;      // Q hi, Q lo: hd / 2 columns each
 constexpr int kPtSCol = 128;    // two buffers of 128 columns
@@ -563,18 +565,24 @@ __device__ __forceinline__ void PtExpect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes)
                : "memory");
 }
-// ~2 s at most (each poll suspends for at most ~1 us)
-__device__ __forceinline__ bool PtWait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool PtPoll(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n"
+      " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "n"(1000)
+      : "memory");
+  return ok != 0;
+}
+// ~2 s at most (each poll suspends for at most ~1 us); false too once another
+// role gave up.
+__device__ __forceinline__ bool PtWait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (PtPoll(bar, parity)) return true;
   for (int i = 0; i < (1 << 21); ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n"
-        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "n"(1000)
-        : "memory");
-    if (ok != 0) return true;
+    if (PtPoll(bar, parity)) return true;
+    if (abort_flag != nullptr && *abort_flag) return false;
   }
   return false;
 }
@@ -696,16 +704,19 @@ __device__ __forceinline__ void PtTurn(float4& x0, float4& x1, float4& x2, float
 }
 
 // Shared memory from a 1024-byte aligned base: the ring of images (hi and lo
-// of one block's K or V each), the halves' exchange, barriers.
+// of one block's K or V each), blocks' references and sums, queries' scales,
+// the halves' exchange, barriers.
 template <int HD>
 struct PtLayout {
   static constexpr int kItemBytes = 4 * kPtKeys * HD;  // hi and lo
   static constexpr int kStages = HD == 128 ? 3 : 6;
-  static constexpr int kSwap = kStages * kItemBytes;   // float [2][2][128]
+  static constexpr int kStat = kStages * kItemBytes;         // float [4][3][128]
+  static constexpr int kScale = kStat + 12 * kPtVectors * 4;  // float [2][128]
+  static constexpr int kSwap = kScale + 2 * kPtVectors * 4;   // float [2][2][128]
   static constexpr int kBars = kSwap + 4 * kPtVectors * 4;
-  // full / empty per stage, q_full, s_full[2], p_full[2], o_full, o_empty,
+  // full / empty per stage, q_full[2], s_full[2], p_full[4], o_full, o_empty,
   // swap[4], done
-  static constexpr int kBarriers = 2 * kStages + 12;
+  static constexpr int kBarriers = 2 * kStages + 15;
   static constexpr int kSmemBytes = kBars + 8 * kBarriers + 16 + 1024;
 };
 
@@ -716,7 +727,8 @@ __device__ unsigned int g_pt_wait_timeouts;
 
 namespace {
 
-// A tile on the CUDA cores: a warp a vector, keys one after another.
+// A tile on the CUDA cores (warps 0-7): a warp a vector, keys one after
+// another.
 template <int HD>
 __device__ void PtSlowTile(const PtArgs& a, const PtTile& tile, int head) {
   constexpr int E = HD / 32;
@@ -724,7 +736,7 @@ __device__ void PtSlowTile(const PtArgs& a, const PtTile& tile, int head) {
   const int64_t stride = static_cast<int64_t>(a.in.kv_heads) * HD;
   const float* k = a.in.k + tile.key0 * stride + head * HD;
   const float* v = a.in.v + tile.key0 * stride + head * HD;
-  for (int i = warp; i < tile.rows * a.group; i += kPtThreads / 32) {
+  for (int i = warp; i < tile.rows * a.group; i += 8) {
     const int sees = tile.sees + i / a.group;
     const int64_t at =
         ((tile.row0 + i / a.group) * static_cast<int64_t>(a.in.n_heads) + head * a.group +
@@ -791,7 +803,6 @@ template <int HD>
 __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
   using L = PtLayout<HD>;
   constexpr int kStages = L::kStages;
-  constexpr int HH = HD / 2;  // dimensions of the output a thread holds
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
   extern __shared__ __align__(16) uint8_t pt_raw[];
@@ -799,20 +810,22 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
   const uint32_t raw_addr = PtSmem(pt_raw);
   uint8_t* base = pt_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   const uint32_t sbase = PtSmem(base);
+  float* stat = reinterpret_cast<float*>(base + L::kStat);  // m_b, the halves' sums
   float* swap = reinterpret_cast<float*>(base + L::kSwap);
+  float* scale_of = reinterpret_cast<float*>(base + L::kScale);
   const uint32_t bars = sbase + L::kBars;
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (kStages + s); };
-  const uint32_t q_full = bars + 8 * (2 * kStages);
-  const auto s_full = [&](int s) { return bars + 8 * (2 * kStages + 1 + s); };
-  const auto p_full = [&](int s) { return bars + 8 * (2 * kStages + 3 + s); };
-  const uint32_t o_full = bars + 8 * (2 * kStages + 5);
-  const uint32_t o_empty = bars + 8 * (2 * kStages + 6);
-  const auto swapped = [&](int w) { return bars + 8 * (2 * kStages + 7 + w); };
-  const uint32_t all_done = bars + 8 * (2 * kStages + 11);
+  // (two or four of a kind where a role may be that far ahead of another)
+  const auto q_full = [&](uint32_t t) { return bars + 8 * (2 * kStages + (t & 1)); };
+  const auto s_full = [&](uint32_t n) { return bars + 8 * (2 * kStages + 2 + (n & 1)); };
+  const auto p_full = [&](uint32_t n) { return bars + 8 * (2 * kStages + 4 + (n & 3)); };
+  const uint32_t o_full = bars + 8 * (2 * kStages + 8);
+  const uint32_t o_empty = bars + 8 * (2 * kStages + 9);
+  const auto swapped = [&](int i) { return bars + 8 * (2 * kStages + 10 + i); };
+  const uint32_t all_done = bars + 8 * (2 * kStages + 14);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kBars + 8 * L::kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* slow_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
 
@@ -821,20 +834,21 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
       PtBarInit(full(s), 1);
       PtBarInit(empty(s), 1);
     }
-    PtBarInit(q_full, 256);
-    for (int s = 0; s < 2; ++s) {
-      PtBarInit(s_full(s), 1);
-      PtBarInit(p_full(s), 256);
+    for (int i = 0; i < 2; ++i) {
+      PtBarInit(q_full(i), 128);
+      PtBarInit(s_full(i), 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      PtBarInit(p_full(i), 256);
+      PtBarInit(swapped(i), 64);
     }
     PtBarInit(o_full, 1);
-    PtBarInit(o_empty, 256);
-    for (int w = 0; w < 4; ++w) PtBarInit(swapped(w), 64);
+    PtBarInit(o_empty, 128);
     PtBarInit(all_done, 1);
     *abort_flag = 0;
-    *slow_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == 13) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
                      PtSmem(tmem_slot)),
                  "r"(kPtTmemColumns)
@@ -850,16 +864,16 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
     *abort_flag = 1;
   };
   const auto wait = [&](uint32_t bar, uint32_t parity) __attribute__((always_inline)) {
-    return PtWait(bar, parity) && !*abort_flag;
+    return PtWait(bar, parity, abort_flag);
   };
   // whose outcome every lane of the warp shares
   const auto warp_wait = [&](uint32_t bar, uint32_t parity) __attribute__((always_inline)) {
     return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
   };
 
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kPtRegsIssue));
-  if (warp == 8) {
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kPtRegsIssue));
+    if (warp == 12) {
     // --------------------------------------------------------------- copies
     if (PtElect()) {
       int put = 0, round = 0;
@@ -877,26 +891,24 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
         ++put;
       };
       for (PtWork w = PtFetch(a, total, round); ok && w.valid; w = PtFetch(a, total, round)) {
-        if (w.slow) {
-          *slow_flag = 1;
-          continue;
-        }
+        if (w.slow) continue;
         const uint8_t* image =
             a.images +
             (static_cast<int64_t>(w.tile.block0) * a.in.kv_heads + w.head) * (2 * L::kItemBytes);
         const int64_t step = static_cast<int64_t>(a.in.kv_heads) * (2 * L::kItemBytes);
         for (int b = 0; ok && b < w.nb; ++b) {
-          copy(image + b * step);
-          if (ok && v_due != nullptr) copy(v_due);
+          if (b == 0 && v_due != nullptr) copy(v_due);
+          if (ok) copy(image + b * step);
+          if (ok && b != 0) copy(v_due);
           v_due = image + b * step + L::kItemBytes;
         }
       }
       if (ok && v_due != nullptr) copy(v_due);
       if (!ok)  // what is in flight lands before the CTA ends
         for (int i = put > kStages ? put - kStages : 0; i < put; ++i)
-          PtWait(full(i % kStages), (i / kStages) & 1);
+          PtWait(full(i % kStages), (i / kStages) & 1, nullptr);
     }
-  } else if (warp == 9) {
+    } else if (warp == 13) {
     // ------------------------------------------------------------- products
     if (PtElect()) {
       bool ok = true, due = false;  // due: O of the block before is still to come
@@ -916,7 +928,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
         const uint64_t kh = PtDesc(sbase + s * L::kItemBytes);
         const uint64_t kl = PtAt(kh, L::kItemBytes / 2);
         const uint32_t qh = tmem + kPtQCol, ql = qh + HD / 2;
-#pragma unroll
+#pragma unroll 4
         for (int j = 0; j < HD / 16; ++j) {
           const uint32_t off = static_cast<uint32_t>((j >> 2) * (kPtKeys * 128) + (j & 3) * 32);
           if (cross) {
@@ -932,7 +944,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
         const uint64_t vh = PtDesc(sbase + s * L::kItemBytes);
         const uint64_t vl = PtAt(vh, L::kItemBytes / 2);
         // 16 keys a step; P's pieces of 32 keys: 16 columns hi, 16 lo
-#pragma unroll
+#pragma unroll 4
         for (int j = 0; j < kPtKeys / 16; ++j) {
           const uint32_t off = static_cast<uint32_t>((j >> 2) * (HD * 128) + (j & 3) * 32);
           const uint32_t ph = p + 32 * (j >> 1) + 8 * (j & 1), pl = ph + 16;
@@ -944,21 +956,28 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
           }
         }
       };
+      const auto p_ready = [&]() { return wait(p_full(o_count), (o_count >> 2) & 1); };
+      const auto q_ready = [&]() {
+        const bool ready = wait(q_full(q_count), (q_count >> 1) & 1);
+        ++q_count;
+        return ready;
+      };
       PtWork w = fast();
       int b = 0;
-      if (w.valid) ok = wait(q_full, 0) && item_ready();
-      ++q_count;
       while (ok && (w.valid || due)) {
-        const bool more = w.valid;  // a block whose scores are to come
+        // S = Q K^T of the next block, unless it is another tile's and O is due
+        const bool s_now = w.valid && (b != 0 || !due);
         const int sk = get % kStages;
-        if (more) {  // S = Q K^T of this block
+        if (s_now) {
+          if (b == 0) ok = q_ready() && item_ready();
+          if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           s_part(sk, true);
           ++get;
-          if (due) ok = item_ready() && wait(p_full(o_count & 1), (o_count >> 1) & 1);
+          if (due) ok = item_ready() && p_ready();
           if (!ok) break;
           s_part(sk, false);
-          PtCommit(s_full(s_count & 1));
+          PtCommit(s_full(s_count));
           PtCommit(empty(sk));
           ++s_count;
           if (++b == w.nb) {
@@ -966,9 +985,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
             b = 0;
           }
         } else {
-          ok = item_ready() && wait(p_full(o_count & 1), (o_count >> 1) & 1);
+          ok = item_ready() && p_ready();
         }
-        const bool next_q = more && w.valid && b == 0;  // the next block is another tile's
         if (due) {  // O = P V of the block before
           ok = ok && (o_count == 0 || wait(o_empty, (o_count - 1) & 1));
           if (!ok) break;
@@ -976,240 +994,290 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
           const int sv = get % kStages;
           o_part(sv, true);
           ++get;
-          if (w.valid && !next_q) ok = item_ready();
+          if (w.valid && b != 0) ok = item_ready();
           if (!ok) break;
           o_part(sv, false);
           PtCommit(o_full);
           PtCommit(empty(sv));
           ++o_count;
-        } else if (w.valid && !next_q) {
+        } else if (w.valid && b != 0) {
           ok = item_ready();
         }
-        if (next_q) {
-          ok = ok && wait(q_full, q_count & 1) && item_ready();
-          ++q_count;
-        }
-        due = more;
+        due = s_now;
       }
       if (!ok) give_up();
       PtCommit(all_done);
       // what was issued has read its operands before tensor memory goes back
-      if (!PtWait(all_done, 0)) give_up();
+      if (!PtWait(all_done, 0, nullptr)) give_up();
     }
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kPtRegsMath));
-    // -------------------------------------------------- softmax and output
-    const int half = warp >> 2;
+    }
+  } else if (warp >= 8) {
+    // --------------------------------------------------------------- output
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kPtRegsOutput));
     const int v = (warp & 3) * 32 + lane;  // query vector
     const int row = v / a.group;
     const bool used = v < (kPtVectors / a.group) * a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    // q and out are read and written by fours of lanes, 64 bytes of a vector
-    // at a time (16 bytes of 32 vectors would take four times the requests),
-    // and turned over between the four
+    // q is read by fours of lanes, 64 bytes of a vector at a time (16 bytes of
+    // 32 vectors would take four times the requests), and turned over between
+    // the four
+    const int at = (row * a.in.n_heads + v % a.group) * HD;  // of the vector in the tile
     int quad_row[4], quad_at[4];  // the four vectors: row of the tile, offset from its first
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int u = (v & ~3) + j;
       quad_row[j] = u < (kPtVectors / a.group) * a.group ? u / a.group : kPtVectors;
-      quad_at[j] = (u / a.group * a.in.n_heads + u % a.group) * HD + half * HH + 4 * (lane & 3);
+      quad_at[j] = (u / a.group * a.in.n_heads + u % a.group) * HD + 4 * (lane & 3);
     }
-    const auto first_of = [&](const PtWork& w) {  // of the tile in q and out
+    const auto first_of = [&](const PtWork& w) {  // the tile's first vector in q and out
       return (static_cast<int64_t>(w.tile.row0) * a.in.n_heads + w.head * a.group) * HD;
     };
-    uint32_t swaps = 0;  // exchanges so far
-    bool ok = true;
-    // this half's value to the other half of the vector, and its value back
-    const auto exchange = [&](float x) __attribute__((always_inline)) {
-      float* at = swap + (swaps & 1) * 2 * kPtVectors + v;
-      at[half * kPtVectors] = x;
-      PtArrive(swapped(warp & 3));
-      ok = warp_wait(swapped(warp & 3), swaps & 1) && ok;
-      ++swaps;
-      return at[(1 - half) * kPtVectors];
-    };
-    // the tile's Q pieces into tensor memory; returns the factor from raw
-    // scores to powers of two, without the key block's
-    const auto write_q = [&](const PtWork& w) __attribute__((always_inline)) {
+    // tile t's Q pieces into tensor memory, and the vectors' factors from raw
+    // scores to powers of two (without the key block's)
+    const auto write_q = [&](const PtWork& w, uint32_t t) __attribute__((always_inline)) {
       const float* q = a.in.q + first_of(w);
-      float4 x[HH / 4];
-#pragma unroll
-      for (int i = 0; i < HH / 4; ++i)
-        x[i] = quad_row[i & 3] < w.tile.rows
+      const auto load = [&](int i) __attribute__((always_inline)) {
+        return quad_row[i & 3] < w.tile.rows
                    ? *reinterpret_cast<const float4*>(q + quad_at[i & 3] + 16 * (i >> 2))
                    : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
       float top = 0.0f;
+      {  // of the quad's four vectors over this lane's chunks, then of this vector
+        float tops[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+        for (int c = 0; c < HD / 64; ++c) {
+          float4 x[16];
 #pragma unroll
-      for (int i = 0; i < HH / 16; ++i) PtTurn(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          for (int i = 0; i < 16; ++i) x[i] = load(16 * c + i);
 #pragma unroll
-      for (int i = 0; i < HH / 4; ++i) {
-        const float m =
-            fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-        // a vector with Inf (or NaN) has NaN outputs whatever its scale
-        top = fmaxf(top, m < INFINITY ? m : 0.0f);
+          for (int i = 0; i < 16; ++i) {
+            const float m =
+                fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+            // a vector with Inf (or NaN) has NaN outputs whatever its scale
+            tops[i & 3] = fmaxf(tops[i & 3], m < INFINITY ? m : 0.0f);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          tops[j] = fmaxf(tops[j], __shfl_xor_sync(0xffffffffu, tops[j], 1));
+          tops[j] = fmaxf(tops[j], __shfl_xor_sync(0xffffffffu, tops[j], 2));
+          if ((lane & 3) == j) top = tops[j];
+        }
       }
-      top = fmaxf(top, exchange(top));
       float down;
       const float up = PtUp(top, down);
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {  // 32 dimensions: 16 columns of each piece
+        float4 x[8];
 #pragma unroll
-      for (int c = 0; c < HH / 32; ++c) {  // 32 dimensions: 16 columns of each piece
+        for (int i = 0; i < 8; ++i) x[i] = load(8 * c + i);
+        PtTurn(x[0], x[1], x[2], x[3]);
+        PtTurn(x[4], x[5], x[6], x[7]);
         uint32_t out[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 y = x[8 * c + i];
-          PtSplit(y.x * up, y.y * up, out[2 * i], out[16 + 2 * i]);
-          PtSplit(y.z * up, y.w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
+          PtSplit(x[i].x * up, x[i].y * up, out[2 * i], out[16 + 2 * i]);
+          PtSplit(x[i].z * up, x[i].w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
         }
-        const uint32_t to = lanes + kPtQCol + half * (HH / 2) + 16 * c;
-        PtSt16(to, out);
-        PtSt16(to + HD / 2, out + 16);
+        PtSt16(lanes + kPtQCol + 16 * c, out);
+        PtSt16(lanes + kPtQCol + 16 * c + HD / 2, out + 16);
       }
+      scale_of[(t & 1) * kPtVectors + v] = a.in.scale * 1.4426950408889634f * down;
       asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-      PtArrive(q_full);
-      return a.in.scale * 1.4426950408889634f * down;
+      PtArrive(q_full(t));
     };
     int round = 0;
-    uint32_t s_count = 0, o_count = 0;
     const auto fast = [&]() {
       PtWork w = PtFetch(a, total, round);
       while (w.valid && w.slow) w = PtFetch(a, total, round);
       return w;
     };
-    // the output of the block before's tile, and that block's reference, sum
-    // and factor of V
-    uint64_t acc[HH / 2];  // pairs of dimensions
-#pragma unroll
-    for (int i = 0; i < HH / 2; ++i) acc[i] = 0;
-    float m = -INFINITY, l = 0.0f;
-    float m_of = 0.0f, sum_of = 0.0f, fv_of = 0.0f;
-    float* out_of = nullptr;
-    int rows_of = 0;
-    bool sees_of = false;
-    const auto take = [&]() __attribute__((always_inline)) {
-      ok = ok && warp_wait(o_full, o_count & 1);
-      ++o_count;
-      if (!ok) return;
-      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-      uint32_t o[HH];
-#pragma unroll
-      for (int c = 0; c < HH / 32; ++c) PtLd32(lanes + kPtOCol + half * HH + 32 * c, o + 32 * c);
-      const float m_new = fmaxf(m, m_of);
-      const float keep = m == m_new ? 1.0f : PtExp2(m - m_new);
-      const float weight = m_of == -INFINITY ? 0.0f : PtExp2(m_of - m_new);
-      const float add = weight * (fv_of * (1.0f / kPtPScale));
-      l = m_of == -INFINITY ? l + sum_of : fmaf(l, keep, sum_of * weight);
-      m = m_new;
-      const uint64_t keep2 = PtPair(keep, keep), add2 = PtPair(add, add);
-      PtLdWait(o);
-      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-      PtArrive(o_empty);
-#pragma unroll
-      for (int i = 0; i < HH / 2; ++i)
-        acc[i] = PtFma2(
-            acc[i], keep2,
-            PtMul2(PtPair(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), add2));
-    };
-    const auto finish = [&]() __attribute__((always_inline)) {
-      l += exchange(l);
-      if (!ok) return;
-      const float inv = sees_of ? kPtPScale / l : 0.0f;
-      if (!sees_of)
-#pragma unroll
-        for (int i = 0; i < HH / 2; ++i) acc[i] = 0;
-#pragma unroll
-      for (int i = 0; i < HH / 16; ++i) {
-        float4 x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          PtUnpair(PtMul2(acc[8 * i + 2 * j], PtPair(inv, inv)), x[j].x, x[j].y);
-          PtUnpair(PtMul2(acc[8 * i + 2 * j + 1], PtPair(inv, inv)), x[j].z, x[j].w);
-        }
-        PtTurn(x[0], x[1], x[2], x[3]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (quad_row[j] < rows_of)
-            *reinterpret_cast<float4*>(out_of + quad_at[j] + 16 * i) = x[j];
-      }
-#pragma unroll
-      for (int i = 0; i < HH / 2; ++i) acc[i] = 0;
-      m = -INFINITY;
-      l = 0.0f;
-    };
-    PtWork w = fast(), next;
-    next.valid = false;
-    float scale = w.valid ? write_q(w) : 0.0f;
-    const auto factor = [&](const PtWork& x, int block) {
-      return a.factors[(static_cast<int64_t>(x.tile.block0) + block) * a.in.kv_heads + x.head];
-    };
-    float2 ff_next = w.valid ? factor(w, 0) : make_float2(0.0f, 0.0f);
-    int b = 0;
-    bool due = false;  // a block whose output is still to come
+    bool ok = true;
+    uint32_t n = 0, t = 0;  // blocks and tiles so far
+    // (one pass before the first tile: only its Q)
+    PtWork w, next = fast();
+    w.valid = false;
+    w.nb = 1;
 #pragma unroll 1
-    while (ok && (w.valid || due)) {
-      const bool more = w.valid;
-      float mb = 0.0f, sum = 0.0f, fv = 0.0f;
-      const bool first = b == 0;
-      if (more) {
-        const float2 ff = ff_next;
-        const int sees = used && row < w.tile.rows ? w.tile.sees + row : 0;
-        if (first) {
-          next = fast();
-          if (next.valid && used && row < next.tile.rows) {  // its q on the way to L2
-            const float* q = a.in.q + first_of(next) + row * a.in.n_heads * HD +
-                             v % a.group * HD + half * HH;
-            asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q));
-            asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + HH - 4));
-          }
+    do {
+      if (w.valid) next = fast();
+      if (next.valid && quad_row[lane & 3] < next.tile.rows) {  // its q on the way to L2
+        const float* q = a.in.q + first_of(next) + quad_at[lane & 3] - 4 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < HD; i += 32) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + i));
+      }
+      uint64_t acc[HD / 2];  // pairs of dimensions
+#pragma unroll
+      for (int i = 0; i < HD / 2; ++i) acc[i] = 0;
+      float m = -INFINITY, l = 0.0f;
+      const float2* factors =
+          a.factors + (w.valid ? static_cast<int64_t>(w.tile.block0) * a.in.kv_heads + w.head : 0);
+#pragma unroll 1
+      for (int b = 0; b < w.nb; ++b, ++n) {
+        const float fv = w.valid ? fabsf(factors[static_cast<int64_t>(b) * a.in.kv_heads].y) : 0.0f;
+        if (b + 1 == w.nb && next.valid) {  // all products with this tile's Q have run
+          ok = !w.valid || warp_wait(s_full(n), (n >> 1) & 1);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          write_q(next, w.valid ? t + 1 : 0);
         }
-        // at least the smallest normal number: a score of -inf stays one
-        const float f = fmaxf(scale * ff.x, 1.17549435e-38f);
-        fv = fabsf(ff.y);
-        ff_next = b + 1 < w.nb ? factor(w, b + 1) : next.valid ? factor(next, 0) : ff;
-        ok = warp_wait(s_full(s_count & 1), (s_count >> 1) & 1);
+        if (!w.valid) break;
+        ok = warp_wait(p_full(n), (n >> 2) & 1);
+        const float* st = stat + (n & 3) * 3 * kPtVectors + v;
+        const float mb = st[0], sum = st[kPtVectors] + st[2 * kPtVectors];
+        const float m_new = fmaxf(m, mb);
+        const float keep = m == m_new ? 1.0f : PtExp2(m - m_new);
+        const float weight = mb == -INFINITY ? 0.0f : PtExp2(mb - m_new);
+        const float add = weight * (fv * (1.0f / kPtPScale));
+        l = mb == -INFINITY ? l + sum : fmaf(l, keep, sum * weight);
+        m = m_new;
+        const uint64_t keep2 = PtPair(keep, keep), add2 = PtPair(add, add);
+        ok = ok && warp_wait(o_full, n & 1);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        // all products with this tile's Q have run: the next tile's, so that
-        // its first scores are computed during this block's softmax
-        if (b + 1 == w.nb && next.valid) scale = write_q(next);
-        const uint32_t s_at = lanes + kPtSCol + 128 * (s_count & 1) + 64 * half;
-        uint32_t s[64];
-        PtLd32(s_at, s);
-        PtLd32(s_at + 32, s + 32);
-        PtLdWait(s);
-        if (b >= w.partial0) {  // the same for every thread
-          const int seen = sees - b * kPtKeys - 64 * half;
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (j >= seen) s[j] = 0xff800000u;  // keys that the row does not see: -inf
-        }
-        float t0 = -INFINITY, t1 = t0, t2 = t0, t3 = t0;
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          PtLd32(lanes + kPtOCol + 32 * c, o);
+          PtLdWait(o);
+          if (c + 1 == HD / 32) {
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            PtArrive(o_empty);
+          }
 #pragma unroll
-        for (int j = 0; j < 64; j += 8) {
-          t0 = PtMax3(t0, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-          t1 = PtMax3(t1, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
-          t2 = PtMax3(t2, __uint_as_float(s[j + 4]), __uint_as_float(s[j + 5]));
-          t3 = PtMax3(t3, __uint_as_float(s[j + 6]), __uint_as_float(s[j + 7]));
+          for (int i = 0; i < 16; ++i)
+            acc[16 * c + i] = PtFma2(
+                acc[16 * c + i], keep2,
+                PtMul2(PtPair(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), add2));
         }
-        float top = PtMax3(fmaxf(t0, t1), t2, t3);
-        top = fmaxf(top, exchange(top));
+      }
+      if (!ok) break;
+      if (w.valid && used && row < w.tile.rows) {
+        // 16 bytes a lane as they stand: turned over between lanes like q they
+        // would be fewer requests, but the code for it, run once a tile, takes
+        // longer to fetch than these take to drain
+        const bool sees = w.tile.sees + row > 0;
+        const float inv = sees ? kPtPScale / l : 0.0f;
+        const uint64_t inv2 = PtPair(inv, inv);
+        float4* out = reinterpret_cast<float4*>(a.in.out + first_of(w) + at);
+#pragma unroll
+        for (int i = 0; i < HD / 4; ++i) {
+          float4 x;
+          PtUnpair(PtMul2(acc[2 * i], inv2), x.x, x.y);
+          PtUnpair(PtMul2(acc[2 * i + 1], inv2), x.z, x.w);
+          out[i] = x;
+        }
+        if (!sees)
+          for (int i = 0; i < HD / 4; ++i) out[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (w.valid) ++t;
+      w = next;
+    } while (w.valid);
+    if (!ok) {
+      give_up();
+      for (int r = 0; (w = PtFetch(a, total, r)).valid;) {  // NaN for what is not finished
+        if (w.slow) continue;
+        if (t > 0) {
+          --t;
+          continue;
+        }
+        float* out = a.in.out + first_of(w);
+        for (int i = threadIdx.x - 256; i < w.tile.rows * a.group * HD; i += 128)
+          out[i / (a.group * HD) * static_cast<int64_t>(a.in.n_heads) * HD + i % (a.group * HD)] =
+              NAN;
+      }
+    }
+  } else {
+    // -------------------------------------------------------------- softmax
+    const int half = warp >> 2;
+    const int v = (warp & 3) * 32 + lane;  // query vector
+    const int row = v / a.group;
+    const bool used = v < (kPtVectors / a.group) * a.group;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kPtSCol + 64 * half;
+    int round = 0;
+    const auto factor = [&](const PtWork& x, int block) {
+      return a.factors[(static_cast<int64_t>(x.tile.block0) + block) * a.in.kv_heads + x.head].x;
+    };
+    bool ok = true, some_slow = false;
+    uint32_t n = 0, t = 0;  // blocks and tiles so far
+    const auto fast = [&]() {
+      PtWork w = PtFetch(a, total, round);
+      for (; w.valid && w.slow; w = PtFetch(a, total, round)) some_slow = true;
+      return w;
+    };
+    PtWork w = fast();
+    float f_next = w.valid ? factor(w, 0) : 0.0f;
+#pragma unroll 1
+    while (w.valid) {
+      const PtWork next = fast();
+      ok = warp_wait(q_full(t), (t >> 1) & 1);
+      const float scale = scale_of[(t & 1) * kPtVectors + v];
+      const int sees = used && row < w.tile.rows ? w.tile.sees + row : 0;
+#pragma unroll 1
+      for (int b = 0; ok && b < w.nb; ++b, ++n) {
+        // at least the smallest normal number: a score of -inf stays one
+        const float f = fmaxf(scale * f_next, 1.17549435e-38f);
+        if (b + 1 < w.nb) f_next = factor(w, b + 1);
+        else if (next.valid) f_next = factor(next, 0);
+        ok = warp_wait(s_full(n), (n >> 1) & 1);
         if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const uint32_t s_at = lanes + 128 * (n & 1);
+        const int seen = sees - b * kPtKeys - 64 * half;
+        const bool whole = b < w.partial0;  // the same for every thread
+        // 32 scores; those of keys that the row does not see are -inf
+        const auto hide = [&](int c, uint32_t* s) __attribute__((always_inline)) {
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (32 * c + j >= seen) s[j] = 0xff800000u;
+          }
+        };
+        float top;
+        {
+          uint32_t s[64];
+          PtLd32(s_at, s);
+          PtLd32(s_at + 32, s + 32);
+          PtLdWait(s);
+          hide(0, s);
+          hide(1, s + 32);
+          float t0 = -INFINITY, t1 = t0, t2 = t0, t3 = t0;
+#pragma unroll
+          for (int j = 0; j < 64; j += 8) {
+            t0 = PtMax3(t0, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+            t1 = PtMax3(t1, __uint_as_float(s[j + 2]), __uint_as_float(s[j + 3]));
+            t2 = PtMax3(t2, __uint_as_float(s[j + 4]), __uint_as_float(s[j + 5]));
+            t3 = PtMax3(t3, __uint_as_float(s[j + 6]), __uint_as_float(s[j + 7]));
+          }
+          top = PtMax3(fmaxf(t0, t1), t2, t3);
+        }
+        // the other half's maximum
+        float* sw = swap + (n & 1) * 2 * kPtVectors + v;
+        sw[half * kPtVectors] = top;
+        PtArrive(swapped(warp & 3));
+        uint32_t s[32];
+        PtLd32(s_at, s);  // the scores again: they do not fit beside the pieces
+        ok = warp_wait(swapped(warp & 3), n & 1);
+        if (!ok) break;
+        top = fmaxf(top, sw[(1 - half) * kPtVectors]);
         // the reference is a whole power of two: 2^(m_b - M) is exact, and so
         // is the summand below, which also brings p to its 2^14
-        mb = rintf(top * f);
+        const float mb = rintf(top * f);
         const float plus = mb == -INFINITY ? 0.0f : 14.0f - mb;  // nothing seen: p is 0
         const uint64_t f2 = PtPair(f, f), plus2 = PtPair(plus, plus);
         uint64_t sum_a = PtPair(0.0f, 0.0f), sum_b = sum_a;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
+          if (c != 0) PtLd32(s_at + 32, s);
+          PtLdWait(s);
+          hide(c, s);
           uint32_t out[32];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float p0, p1;
-            PtUnpair(PtFma2(PtPair(__uint_as_float(s[32 * c + 2 * i]),
-                                   __uint_as_float(s[32 * c + 2 * i + 1])),
-                            f2, plus2),
+            PtUnpair(PtFma2(PtPair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), f2,
+                            plus2),
                      p0, p1);
             p0 = PtExp2(p0);
             p1 = PtExp2(p1);
@@ -1230,52 +1298,27 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
           }
           PtSt32(s_at + 32 * c, out);
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        PtArrive(p_full(s_count & 1));
-        ++s_count;
         float x, y;
         PtUnpair(PtAdd2(sum_a, sum_b), x, y);
-        sum = x + y;
-      }
-      if (due) {
-        take();
-        if (ok && (first || !more)) finish();
+        float* st = stat + (n & 3) * 3 * kPtVectors + v;
+        if (half == 0) st[0] = mb;
+        st[(1 + half) * kPtVectors] = x + y;
+        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        PtArrive(p_full(n));
       }
       if (!ok) break;
-      if (more && first) {
-        out_of = a.in.out + first_of(w);
-        rows_of = w.tile.rows;
-        sees_of = used && row < w.tile.rows && w.tile.sees + row > 0;
-      }
-      m_of = mb;
-      sum_of = sum;
-      fv_of = fv;
-      due = more;
-      if (more && ++b == w.nb) {
-        w = next;
-        b = 0;
-      }
+      w = next;
+      ++t;
     }
     if (!ok) give_up();
+    round = 0;
+    while (some_slow && (w = PtFetch(a, total, round)).valid)  // tiles for the CUDA cores
+      if (w.slow) PtSlowTile<HD>(a, w.tile, w.head);
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
-  // tiles for the CUDA cores; after a wait gave up all tiles, as NaN
-  const bool gave_up = *abort_flag != 0, some_slow = *slow_flag != 0;
-  int round = 0;
-  PtWork w;
-  while ((gave_up || some_slow) && (w = PtFetch(a, total, round)).valid) {
-    if (gave_up) {
-      const int64_t at = (w.tile.row0 * static_cast<int64_t>(a.in.n_heads) + w.head * a.group) * HD;
-      for (int i = threadIdx.x; i < w.tile.rows * a.group * HD; i += kPtThreads)
-        a.in.out[at + i / (a.group * HD) * static_cast<int64_t>(a.in.n_heads) * HD +
-                 i % (a.group * HD)] = NAN;
-    } else if (w.slow) {
-      PtSlowTile<HD>(a, w.tile, w.head);
-    }
-  }
-  if (warp == 9) {
+  if (warp == 13) {
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
                  "r"(kPtTmemColumns)
