@@ -218,13 +218,13 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
 //     block's softmax needs no other's;
 //   - warps 8-11: output.  Thread = query vector: O_b joins the registers,
 //     acc = acc 2^(M - M') + O 2^(m_b - M'), both factors exact.  They also
-//     write the tiles' Q pieces into tensor memory, the next tile's while the
-//     softmax of a tile's last block runs;
-//   - warp 12: bulk copies, K_0, K_1, V_0, K_2, V_1, ... through a ring, on into
-//     the next tile;
-//   - warp 13: tensor memory; one lane issues S_(b + 1), then O_b (O first where
-//     S is the next tile's), so that the softmax of a block runs under the
-//     products of its neighbours;
+//     split the tiles' Q into tensor memory, the next tile's as soon as the
+//     last scores of a tile are there;
+//   - warp 12: bulk copies through a ring: for each block n of all tiles in
+//     turn Q (where n begins a tile), K_n, V_(n - 1);
+//   - warp 13: tensor memory; one lane issues S_n, then O_(n - 1), across the
+//     tiles, so that the softmax of a block runs under the products of its
+//     neighbours;
 //   - warps 14-15 only complete the warpgroup that gives up registers.
 // Tensor memory: Q hi and lo, two S / P buffers, O.  All waits are bounded; a
 // CTA whose wait gave up writes NaN and is counted (mlb_wait_timeouts).
@@ -345,6 +345,12 @@ __device__ __forceinline__ float PtMax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+
+// Index of the ring item that holds the Q of tile t, whose first block is
+// number n of all: the Qs before it, n Ks and n - 1 Vs.
+__device__ __forceinline__ uint32_t PtQItem(uint32_t t, uint32_t n) {
+  return t + n + (n == 0 ? 0 : n - 1);
 }
 
 constexpr int kPtSplitThreads = 256;
@@ -684,27 +690,8 @@ __device__ __forceinline__ bool PtElect() {
   return e != 0;
 }
 
-// Turns 16-byte chunks over between the four lanes of a quad: lane i's x[j]
-// becomes lane j's x[i].
-__device__ __forceinline__ void PtTurnPair(float4& a, float4& b, bool odd, int mask) {
-  float4 t = odd ? a : b;
-  t.x = __shfl_xor_sync(0xffffffffu, t.x, mask);
-  t.y = __shfl_xor_sync(0xffffffffu, t.y, mask);
-  t.z = __shfl_xor_sync(0xffffffffu, t.z, mask);
-  t.w = __shfl_xor_sync(0xffffffffu, t.w, mask);
-  if (odd) a = t;
-  else b = t;
-}
-__device__ __forceinline__ void PtTurn(float4& x0, float4& x1, float4& x2, float4& x3) {
-  const bool odd = (threadIdx.x & 1) != 0, high = (threadIdx.x & 2) != 0;
-  PtTurnPair(x0, x1, odd, 1);
-  PtTurnPair(x2, x3, odd, 1);
-  PtTurnPair(x0, x2, high, 2);
-  PtTurnPair(x1, x3, high, 2);
-}
-
-// Shared memory from a 1024-byte aligned base: the ring of images (hi and lo
-// of one block's K or V each), blocks' references and sums, queries' scales,
+// Shared memory from a 1024-byte aligned base: the ring (an item is the hi and
+// lo images of one block's K or V, or a tile's Q in fp32), blocks' references and sums, queries' scales,
 // the halves' exchange, barriers.
 template <int HD>
 struct PtLayout {
@@ -875,39 +862,66 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kPtRegsIssue));
     if (warp == 12) {
     // --------------------------------------------------------------- copies
-    if (PtElect()) {
+      // One warp walks the ring, item by item (a wait for a stage's release
+      // may only ever be for the release that comes next).
       int put = 0, round = 0;
       bool ok = true;
-      const uint8_t* v_due = nullptr;  // the block before's V comes after this block's K
-      const auto copy = [&](const uint8_t* src) {
+      int begun[kStages];  // last item begun in each stage
+      for (int i = 0; i < kStages; ++i) begun[i] = -1;
+      // the next item's stage, when it is free
+      const auto stage = [&]() {
         const int s = put % kStages;
-        if (put >= kStages && !wait(empty(s), (put / kStages - 1) & 1)) {
-          give_up();
-          ok = false;
-          return;
-        }
-        PtExpect(full(s), L::kItemBytes);
-        PtBulk(sbase + s * L::kItemBytes, src, L::kItemBytes, full(s));
-        ++put;
+        if (put >= kStages) ok = warp_wait(empty(s), (put / kStages - 1) & 1);
+        if (ok) begun[s] = put++;
+        return s;
       };
+      const auto copy = [&](const uint8_t* src) {
+        const int s = stage();
+        if (ok && lane == 0) {
+          PtExpect(full(s), L::kItemBytes);
+          PtBulk(sbase + s * L::kItemBytes, src, L::kItemBytes, full(s));
+        }
+        __syncwarp();
+      };
+      const uint8_t* v_due = nullptr;  // the block before's V comes after this block's K
       for (PtWork w = PtFetch(a, total, round); ok && w.valid; w = PtFetch(a, total, round)) {
         if (w.slow) continue;
+        // Q: a vector's 16-byte chunk i goes to place (i + v) mod (HD / 4) of
+        // its row, so that 8 threads that read chunk i of 8 vectors meet all
+        // banks
+        constexpr uint32_t kChunks = HD / 4;
+        const int vectors = w.tile.rows * a.group;
+        const int sq = stage();
+        if (!ok) break;
+        if (lane == 0) PtExpect(full(sq), vectors * HD * 4);
+        __syncwarp();
+        for (int v = lane; v < vectors; v += 32) {
+          const uint8_t* src = reinterpret_cast<const uint8_t*>(
+              a.in.q + ((w.tile.row0 + v / a.group) * static_cast<int64_t>(a.in.n_heads) +
+                        w.head * a.group + v % a.group) * HD);
+          const uint32_t dst = sbase + sq * L::kItemBytes + v * HD * 4;
+          const uint32_t turn = 16 * (v % kChunks);
+          PtBulk(dst + turn, src, HD * 4 - turn, full(sq));
+          if (turn != 0) PtBulk(dst, src + HD * 4 - turn, turn, full(sq));
+        }
+        __syncwarp();
         const uint8_t* image =
             a.images +
             (static_cast<int64_t>(w.tile.block0) * a.in.kv_heads + w.head) * (2 * L::kItemBytes);
         const int64_t step = static_cast<int64_t>(a.in.kv_heads) * (2 * L::kItemBytes);
         for (int b = 0; ok && b < w.nb; ++b) {
-          if (b == 0 && v_due != nullptr) copy(v_due);
-          if (ok) copy(image + b * step);
-          if (ok && b != 0) copy(v_due);
+          copy(image + b * step);
+          if (ok && v_due != nullptr) copy(v_due);
           v_due = image + b * step + L::kItemBytes;
         }
       }
       if (ok && v_due != nullptr) copy(v_due);
-      if (!ok)  // what is in flight lands before the CTA ends
-        for (int i = put > kStages ? put - kStages : 0; i < put; ++i)
-          PtWait(full(i % kStages), (i / kStages) & 1, nullptr);
-    }
+      // after a wait that gave up, what is in flight lands before the CTA ends
+      if (!ok) {
+        give_up();
+        for (int i = 0; i < kStages; ++i)
+          if (begun[i] >= 0) PtWait(full(i), (begun[i] / kStages) & 1, nullptr);
+      }
     } else if (warp == 13) {
     // ------------------------------------------------------------- products
     if (PtElect()) {
@@ -957,20 +971,21 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
         }
       };
       const auto p_ready = [&]() { return wait(p_full(o_count), (o_count >> 2) & 1); };
+      // the tile's Q is in tensor memory: its ring stage is free again
       const auto q_ready = [&]() {
-        const bool ready = wait(q_full(q_count), (q_count >> 1) & 1);
+        if (!wait(q_full(q_count), (q_count >> 1) & 1)) return false;
+        PtArrive(empty(get % kStages));
         ++q_count;
-        return ready;
+        ++get;
+        return item_ready();
       };
       PtWork w = fast();
       int b = 0;
+      if (w.valid) ok = q_ready();
       while (ok && (w.valid || due)) {
-        // S = Q K^T of the next block, unless it is another tile's and O is due
-        const bool s_now = w.valid && (b != 0 || !due);
+        const bool more = w.valid;
         const int sk = get % kStages;
-        if (s_now) {
-          if (b == 0) ok = q_ready() && item_ready();
-          if (!ok) break;
+        if (more) {  // S = Q K^T of this block
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           s_part(sk, true);
           ++get;
@@ -1003,7 +1018,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
         } else if (w.valid && b != 0) {
           ok = item_ready();
         }
-        due = s_now;
+        if (more && w.valid && b == 0) ok = ok && q_ready();
+        due = more;
       }
       if (!ok) give_up();
       PtCommit(all_done);
@@ -1018,66 +1034,39 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
     const int row = v / a.group;
     const bool used = v < (kPtVectors / a.group) * a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    // q is read by fours of lanes, 64 bytes of a vector at a time (16 bytes of
-    // 32 vectors would take four times the requests), and turned over between
-    // the four
-    const int at = (row * a.in.n_heads + v % a.group) * HD;  // of the vector in the tile
-    int quad_row[4], quad_at[4];  // the four vectors: row of the tile, offset from its first
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int u = (v & ~3) + j;
-      quad_row[j] = u < (kPtVectors / a.group) * a.group ? u / a.group : kPtVectors;
-      quad_at[j] = (u / a.group * a.in.n_heads + u % a.group) * HD + 4 * (lane & 3);
-    }
     const auto first_of = [&](const PtWork& w) {  // the tile's first vector in q and out
       return (static_cast<int64_t>(w.tile.row0) * a.in.n_heads + w.head * a.group) * HD;
     };
-    // tile t's Q pieces into tensor memory, and the vectors' factors from raw
-    // scores to powers of two (without the key block's)
-    const auto write_q = [&](const PtWork& w, uint32_t t) __attribute__((always_inline)) {
-      const float* q = a.in.q + first_of(w);
-      const auto load = [&](int i) __attribute__((always_inline)) {
-        return quad_row[i & 3] < w.tile.rows
-                   ? *reinterpret_cast<const float4*>(q + quad_at[i & 3] + 16 * (i >> 2))
-                   : make_float4(0.f, 0.f, 0.f, 0.f);
-      };
+    // tile t's Q, from ring item `item`, as pieces into tensor memory, and the
+    // vectors' factors from raw scores to powers of two (without the key
+    // block's)
+    const auto write_q = [&](const PtWork& w, uint32_t t, uint32_t item)
+        __attribute__((always_inline)) {
+      constexpr int kChunks = HD / 4;
+      const uint32_t stage = item % kStages;
+      if (!warp_wait(full(stage), (item / kStages) & 1)) return false;
+      const bool live = used && row < w.tile.rows;
+      const float4* x =
+          reinterpret_cast<const float4*>(base + stage * L::kItemBytes) + v * kChunks;
       float top = 0.0f;
-      {  // of the quad's four vectors over this lane's chunks, then of this vector
-        float tops[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-        for (int c = 0; c < HD / 64; ++c) {
-          float4 x[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = load(16 * c + i);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float m =
-                fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-            // a vector with Inf (or NaN) has NaN outputs whatever its scale
-            tops[i & 3] = fmaxf(tops[i & 3], m < INFINITY ? m : 0.0f);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          tops[j] = fmaxf(tops[j], __shfl_xor_sync(0xffffffffu, tops[j], 1));
-          tops[j] = fmaxf(tops[j], __shfl_xor_sync(0xffffffffu, tops[j], 2));
-          if ((lane & 3) == j) top = tops[j];
-        }
+#pragma unroll 8
+      for (int i = 0; i < kChunks; ++i) {
+        const float4 y = x[(i + v) % kChunks];
+        const float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+        // a vector with Inf (or NaN) has NaN outputs whatever its scale
+        top = fmaxf(top, m < INFINITY ? m : 0.0f);
       }
       float down;
-      const float up = PtUp(top, down);
+      const float up = PtUp(live ? top : 0.0f, down);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {  // 32 dimensions: 16 columns of each piece
-        float4 x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = load(8 * c + i);
-        PtTurn(x[0], x[1], x[2], x[3]);
-        PtTurn(x[4], x[5], x[6], x[7]);
         uint32_t out[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          PtSplit(x[i].x * up, x[i].y * up, out[2 * i], out[16 + 2 * i]);
-          PtSplit(x[i].z * up, x[i].w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
+          float4 y = x[(8 * c + i + v) % kChunks];
+          if (!live) y = make_float4(0.f, 0.f, 0.f, 0.f);
+          PtSplit(y.x * up, y.y * up, out[2 * i], out[16 + 2 * i]);
+          PtSplit(y.z * up, y.w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
         }
         PtSt16(lanes + kPtQCol + 16 * c, out);
         PtSt16(lanes + kPtQCol + 16 * c + HD / 2, out + 16);
@@ -1086,6 +1075,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
       asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
       PtArrive(q_full(t));
+      return true;
     };
     int round = 0;
     const auto fast = [&]() {
@@ -1102,11 +1092,6 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
 #pragma unroll 1
     do {
       if (w.valid) next = fast();
-      if (next.valid && quad_row[lane & 3] < next.tile.rows) {  // its q on the way to L2
-        const float* q = a.in.q + first_of(next) + quad_at[lane & 3] - 4 * (lane & 3);
-#pragma unroll
-        for (int i = 0; i < HD; i += 32) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + i));
-      }
       uint64_t acc[HD / 2];  // pairs of dimensions
 #pragma unroll
       for (int i = 0; i < HD / 2; ++i) acc[i] = 0;
@@ -1116,11 +1101,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
 #pragma unroll 1
       for (int b = 0; b < w.nb; ++b, ++n) {
         const float fv = w.valid ? fabsf(factors[static_cast<int64_t>(b) * a.in.kv_heads].y) : 0.0f;
-        if (b + 1 == w.nb && next.valid) {  // all products with this tile's Q have run
-          ok = !w.valid || warp_wait(s_full(n), (n >> 1) & 1);
+        // The next tile's Q as soon as all products with this tile's have run:
+        // the last block's scores come before the last but one's output.
+        if (b == max(w.nb - 2, 0) && next.valid) {
+          const uint32_t last = n + w.nb - 1 - b;
+          ok = !w.valid || warp_wait(s_full(last), (last >> 1) & 1);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          write_q(next, w.valid ? t + 1 : 0);
+          ok = write_q(next, w.valid ? t + 1 : 0, w.valid ? PtQItem(t + 1, last + 1) : 0);
+          if (!ok) break;
         }
         if (!w.valid) break;
         ok = warp_wait(p_full(n), (n >> 2) & 1);
@@ -1154,13 +1143,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
       }
       if (!ok) break;
       if (w.valid && used && row < w.tile.rows) {
-        // 16 bytes a lane as they stand: turned over between lanes like q they
-        // would be fewer requests, but the code for it, run once a tile, takes
-        // longer to fetch than these take to drain
+        // 16 bytes a lane as they stand: turned over between lanes they would
+        // be fewer requests, but the code for it, run once a tile, takes longer
+        // to fetch than these take to drain (13,500 clocks against 5,800)
         const bool sees = w.tile.sees + row > 0;
         const float inv = sees ? kPtPScale / l : 0.0f;
         const uint64_t inv2 = PtPair(inv, inv);
-        float4* out = reinterpret_cast<float4*>(a.in.out + first_of(w) + at);
+        float4* out = reinterpret_cast<float4*>(
+            a.in.out + first_of(w) + (row * a.in.n_heads + v % a.group) * HD);
 #pragma unroll
         for (int i = 0; i < HD / 4; ++i) {
           float4 x;

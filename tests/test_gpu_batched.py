@@ -48,20 +48,23 @@ def attend(q, k, v, sees):
     """One head in 64 bits: q [n, hd], k, v [t, hd]; row r sees keys < sees[r].
     Returns (out, tolerance, weights)."""
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
-    hd, t = q.shape[1], k.shape[0]
-    out, tol, w = np.zeros_like(q), np.zeros_like(q), np.zeros((len(q), t))
-    for r, n in enumerate(sees):
-        n = min(int(n), t)
-        if n <= 0:
-            continue
-        s = k[:n] @ q[r] / np.sqrt(hd)
-        delta = delta_of(q[r], k[:n])
-        e = np.exp(s - s.max())
-        e /= e.sum()
-        w[r, :n] = e
-        out[r] = e @ v[:n]
-        tol[r] = (2 * delta + 2.0 ** -20 + (n / 4 + 64) * 2.0 ** -23) * (e @ np.abs(v[:n]))
-        tol[r] += 2.0 ** -37 * np.abs(v[:n]).max(1).sum()
+    n, hd, t = q.shape[0], q.shape[1], k.shape[0]
+    sees = np.clip(np.asarray(sees), 0, t)
+    out, tol, w = np.zeros_like(q), np.zeros_like(q), np.zeros((n, t))
+    some = sees > 0
+    if not some.any():
+        return out, tol, w
+    q, seen = q[some], np.arange(t)[None, :] < sees[some][:, None]
+    s = np.where(seen, q @ k.T / np.sqrt(hd), -np.inf)
+    e = np.exp(s - s.max(1, keepdims=True))
+    e /= e.sum(1, keepdims=True)
+    near = np.where(seen, np.abs(q) @ np.abs(k).T, 0).max(1) * (2.0 ** -21 + hd * 2.0 ** -23)
+    top = np.maximum.accumulate(np.abs(k).max(1))[sees[some] - 1]
+    delta = (near + 2.0 ** -38 * hd * np.abs(q).max(1) * top) / np.sqrt(hd)
+    each = np.abs(v).max(1)
+    w[some], out[some] = e, e @ np.where(e.any(0)[:, None], v, 0)
+    tol[some] = (2 * delta + 2.0 ** -20 + (sees[some] / 4 + 64) * 2.0 ** -23)[:, None] * (e @ np.abs(v))
+    tol[some] += 2.0 ** -37 * np.cumsum(each)[sees[some] - 1][:, None]
     return out, tol, w
 
 
@@ -181,6 +184,23 @@ def test_packed_attention_does_not_look_past_its_keys(cuda, hd):
     assert np.isnan(got[149]).all()
     keep = np.r_[3:149, 150:190]
     check(got[keep], want[keep], tol[keep])
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 8, 128), (8, 8, 64), (14, 2, 64)])
+@pytest.mark.parametrize("most,context", [(40, 0), (300, 0), (130, 300)])
+def test_packed_attention_many_tiles(cuda, nh, nkv, hd, most, context):
+    """More query tiles than the GPU has multiprocessors, most of them of one
+    to three key blocks: each CTA goes through several, one after another."""
+    rng = np.random.default_rng(most + nh)
+    lens = rng.integers(max(1, most // 3), most, 90).tolist()
+    keys = [n + int(rng.integers(0, context + 1)) for n in lens]
+    q, k, v, qo, ko = packed_inputs(rng, lens, keys, nh, nkv, hd)
+    want, tol = packed_reference(q, k, v, qo, ko)
+    for _ in range(2):
+        got = mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(qo, cuda),
+                                   dev(ko, cuda))
+        check(got.cpu().numpy(), want, tol)
+    assert mlb.wait_timeouts() == 0
 
 
 def test_packed_attention_equals_rows_of_one_sequence(cuda):
