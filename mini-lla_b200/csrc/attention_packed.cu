@@ -4,9 +4,13 @@
 // 0 .. K - Q + r:  out = softmax(q k^T / sqrt(hd)) v, kv head h / G for query
 // head h.  Rows and keys of a sequence are found from the offsets on the
 // device.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <mutex>
 
 #include "common.cuh"
 
@@ -600,6 +604,14 @@ __device__ __forceinline__ void PtBulk(uint32_t dst, const void* src, uint32_t b
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void PtTensor(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void PtCommit(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar)
@@ -787,7 +799,8 @@ __device__ __forceinline__ PtWork PtFetch(const PtArgs& a, int64_t total, int& r
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
+__global__ void __launch_bounds__(kPtThreads, 1)
+    PkTcKernel(const PtArgs a, const __grid_constant__ CUtensorMap q_map) {
   using L = PtLayout<HD>;
   constexpr int kStages = L::kStages;
   LaunchWait();  // the previous kernel on the stream has completed
@@ -886,23 +899,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
       const uint8_t* v_due = nullptr;  // the block before's V comes after this block's K
       for (PtWork w = PtFetch(a, total, round); ok && w.valid; w = PtFetch(a, total, round)) {
         if (w.slow) continue;
-        // Q: a vector's 16-byte chunk i goes to place (i + v) mod (HD / 4) of
-        // its row, so that 8 threads that read chunk i of 8 vectors meet all
-        // banks
-        constexpr uint32_t kChunks = HD / 4;
-        const int vectors = w.tile.rows * a.group;
+        // Q: 32 dimensions of all vectors a copy, as 128-byte swizzled rows
+        // (rows of other sequences that come along are not used)
         const int sq = stage();
         if (!ok) break;
-        if (lane == 0) PtExpect(full(sq), vectors * HD * 4);
-        __syncwarp();
-        for (int v = lane; v < vectors; v += 32) {
-          const uint8_t* src = reinterpret_cast<const uint8_t*>(
-              a.in.q + ((w.tile.row0 + v / a.group) * static_cast<int64_t>(a.in.n_heads) +
-                        w.head * a.group + v % a.group) * HD);
-          const uint32_t dst = sbase + sq * L::kItemBytes + v * HD * 4;
-          const uint32_t turn = 16 * (v % kChunks);
-          PtBulk(dst + turn, src, HD * 4 - turn, full(sq));
-          if (turn != 0) PtBulk(dst, src + HD * 4 - turn, turn, full(sq));
+        if (lane == 0) {
+          PtExpect(full(sq), (kPtVectors / a.group) * a.group * HD * 4);
+          for (int c = 0; c < HD / 32; ++c)
+            PtTensor(sbase + sq * L::kItemBytes + c * (kPtVectors * 128), &q_map, 32 * c,
+                     w.head * a.group, w.tile.row0, full(sq));
         }
         __syncwarp();
         const uint8_t* image =
@@ -1046,12 +1051,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
       const uint32_t stage = item % kStages;
       if (!warp_wait(full(stage), (item / kStages) & 1)) return false;
       const bool live = used && row < w.tile.rows;
-      const float4* x =
-          reinterpret_cast<const float4*>(base + stage * L::kItemBytes) + v * kChunks;
+      const auto chunk = [&](int i) {  // 4 dimensions of the vector
+        return *reinterpret_cast<const float4*>(base + stage * L::kItemBytes +
+                                                (i >> 3) * (kPtVectors * 128) + PtSwz(v, i & 7));
+      };
       float top = 0.0f;
 #pragma unroll 8
       for (int i = 0; i < kChunks; ++i) {
-        const float4 y = x[(i + v) % kChunks];
+        const float4 y = chunk(i);
         const float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
         // a vector with Inf (or NaN) has NaN outputs whatever its scale
         top = fmaxf(top, m < INFINITY ? m : 0.0f);
@@ -1063,7 +1070,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
         uint32_t out[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float4 y = x[(8 * c + i + v) % kChunks];
+          float4 y = chunk(8 * c + i);
           if (!live) y = make_float4(0.f, 0.f, 0.f, 0.f);
           PtSplit(y.x * up, y.y * up, out[2 * i], out[16 + 2 * i]);
           PtSplit(y.z * up, y.w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
@@ -1316,6 +1323,23 @@ __global__ void __launch_bounds__(kPtThreads, 1) PkTcKernel(const PtArgs a) {
   }
 }
 
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no link
+// against the driver library); null when the driver does not offer it.
+PFN_cuTensorMapEncodeTiled_v12000 PtEncodeFn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    cudaGetLastError();
+  });
+  return fn;
+}
+
 template <int HD>
 int LaunchPkTc(const PtArgs& a, cudaStream_t s) {
   constexpr int smem = PtLayout<HD>::kSmemBytes;
@@ -1324,12 +1348,27 @@ int LaunchPkTc(const PtArgs& a, cudaStream_t s) {
     cudaGetLastError();
     return Fail(MLB_ERR_CUDA, "mlb_attention_packed_f32: shared memory opt-in");
   }
+  // q as [rows][heads][HD]; a box is 32 dimensions of a tile's vectors
+  CUtensorMap q_map;
+  const cuuint64_t dims[3] = {HD, static_cast<cuuint64_t>(a.in.n_heads),
+                              static_cast<cuuint64_t>(a.in.q_rows)};
+  const cuuint64_t strides[2] = {HD * 4, static_cast<cuuint64_t>(a.in.n_heads) * HD * 4};
+  const cuuint32_t box[3] = {32, static_cast<cuuint32_t>(a.group),
+                             static_cast<cuuint32_t>(kPtVectors / a.group)};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const auto encode = PtEncodeFn();
+  if (encode == nullptr ||
+      encode(&q_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(a.in.q), dims, strides,
+             box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return Fail(MLB_ERR_CUDA, "mlb_attention_packed_f32: tensor map");
   Launch(PkSplitKernel<HD>,
          dim3(static_cast<unsigned>(a.max_blocks + 1), static_cast<unsigned>(a.in.kv_heads), 2),
          kPtSplitThreads, 0, s, a);
   const int64_t most = a.max_tiles * a.in.kv_heads, sms = SmCount();
   Launch(PkTcKernel<HD>, dim3(static_cast<unsigned>(most < sms ? most : sms)), kPtThreads,
-         static_cast<size_t>(smem), s, a);
+         static_cast<size_t>(smem), s, a, q_map);
   return MLB_OK;
 }
 
