@@ -170,7 +170,8 @@ struct A8Smem {
   static constexpr int kKBytes = kUnit * kKPitch;
   static constexpr int kStageBytes = kKBytes + HD * kUnit + 16;  // K, V, the two scales
   static constexpr int kStages = 2;
-  static constexpr int kBytes = kA8Warps * kStages * kStageBytes;
+  static constexpr int kQBytes = (HD / 16) * 32 * 16;  // A operand of the scores
+  static constexpr int kBytes = kA8Warps * (kStages * kStageBytes + kQBytes);
   // CTAs that fit an SM's shared memory (1 KB of each is the system's)
   static constexpr int kFit = 228 * 1024 / (kBytes + 1024 + 256);
   static constexpr int kCtasPerSm = kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
@@ -185,54 +186,49 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
   extern __shared__ __align__(16) uint8_t a8_raw[];
-  __shared__ int64_t sums[kA8Warps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = lane >> 2, c = lane & 3;  // head of the group / column; quarter
-  uint8_t* ring = a8_raw + warp * kStages * S::kStageBytes;
+  uint8_t* ring = a8_raw + warp * (kStages * S::kStageBytes + S::kQBytes);
+  uint4* qf = reinterpret_cast<uint4*>(ring + kStages * S::kStageBytes) + lane;  // [k16 step][lane]
 
-  // all units, and the place where this warp's share begins
-  int64_t mine = 0;
-  for (int i = threadIdx.x; i < a.n_seqs; i += kA8Warps * 32) mine += UnitsOf(a, i);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sums[warp] = mine;
-  __syncthreads();
+  // all units, and the place where this warp's share begins (each warp on its
+  // own: the lengths come from L2 once and then from L1)
   int64_t total = 0;
+#pragma unroll 4
+  for (int i = lane; i < a.n_seqs; i += 32) total += UnitsOf(a, i);
 #pragma unroll
-  for (int w = 0; w < kA8Warps; ++w) total += sums[w];
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   total *= a.kv_heads;
-  if (total == 0) return;
   const int workers = a.workers < total ? a.workers : static_cast<int>(total);
   const int worker = warp * gridDim.x + blockIdx.x;  // few workers: one a CTA
   if (worker >= workers) return;  // nothing below waits for another warp
   const int64_t begin = ShareBegin(total, workers, worker);
   const int count = static_cast<int>(ShareBegin(total, workers, worker + 1) - begin);
   Place put{};  // next unit to copy
-  {
-    int64_t before = 0;
-    for (int base = 0; base < a.n_seqs; base += 32) {
-      const int i = base + lane;
-      const int64_t units = i < a.n_seqs ? static_cast<int64_t>(UnitsOf(a, i)) * a.kv_heads : 0;
-      int64_t upto = units;
+  int64_t before = 0;
+  for (int base = 0; base < a.n_seqs; base += 32) {
+    const int i = base + lane;
+    const int length = i < a.n_seqs ? LengthOf(a, i) : 0;
+    const int64_t units = static_cast<int64_t>(UnitsIn(length)) * a.kv_heads;
+    int64_t upto = units;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += up;
-      }
-      const bool here = begin >= before + upto - units && begin < before + upto;
-      const uint32_t found = __ballot_sync(0xffffffffu, here);
-      if (found != 0) {
-        const int src = __ffs(found) - 1;
-        put.seq = base + src;
-        put.length = LengthOf(a, put.seq);
-        put.units = UnitsIn(put.length);
-        const int64_t first = __shfl_sync(0xffffffffu, before + upto - units, src);
-        put.head = static_cast<int>((begin - first) / put.units);
-        put.unit = static_cast<int>((begin - first) % put.units);
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
     }
+    const bool here = begin >= before + upto - units && begin < before + upto;
+    const uint32_t found = __ballot_sync(0xffffffffu, here);
+    if (found != 0) {
+      const int src = __ffs(found) - 1;
+      put.seq = base + src;
+      put.length = __shfl_sync(0xffffffffu, length, src);
+      put.units = UnitsIn(put.length);
+      const int64_t first = __shfl_sync(0xffffffffu, before + upto - units, src);
+      put.head = static_cast<int>((begin - first) / put.units);
+      put.unit = static_cast<int>((begin - first) % put.units);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
   }
   Place get = put;  // next unit to compute
 
@@ -290,7 +286,6 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
   }
 
   const int64_t unit_cols = a.table_cols * a.block / kUnit;
-  uint32_t qf[2 * DC][4];  // A operand of the scores, two k16 steps per 32 dimensions
   float acc[DT][2];
   float m = 0.0f, l = 0.0f, factor = 0.0f;
   bool bad = false, fresh = true;
@@ -336,9 +331,10 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
       for (int j = 0; j < DC; ++j)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          SplitPair(x[j][4 * s] * up, x[j][4 * s + 1] * up, qf[2 * j + s][0], qf[2 * j + s][1]);
-          SplitPair(x[j][4 * s + 2] * up, x[j][4 * s + 3] * up, qf[2 * j + s][2],
-                    qf[2 * j + s][3]);
+          uint4 a;
+          SplitPair(x[j][4 * s] * up, x[j][4 * s + 1] * up, a.x, a.y);
+          SplitPair(x[j][4 * s + 2] * up, x[j][4 * s + 3] * up, a.z, a.w);
+          qf[32 * (2 * j + s)] = a;  // read by this lane only
         }
     }
     CopyAsyncWait<kStages - 1>();
@@ -360,14 +356,15 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
             w[j] = *reinterpret_cast<const uint2*>(kt + (8 * j + row) * S::kKPitch + 32 * g +
                                                    8 * c);
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
+          for (int s = 0; s < 2; ++s) {
+            const uint4 q = qf[32 * (2 * g + s)];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t b0, b1;
               CodePairs(s == 0 ? w[j].x : w[j].y, b0, b1);
-              const uint32_t(&q)[4] = qf[2 * g + s];
-              Mma(d[j], q[0], q[1], q[2], q[3], b0, b1);
+              Mma(d[j], q.x, q.y, q.z, q.w, b0, b1);
             }
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -472,67 +469,104 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
 }
 
 // Joins the partials of a (sequence, query head): out = sum_w acc_w f_w / sum_w
-// l_w f_w, f_w = 2^(m_w - M).  Warps take partials in turn, lanes dimensions.
-constexpr int kJoinThreads = 256;
+// l_w f_w, f_w = 2^(m_w - M).  CTA = (query head, sequence); every eighth
+// partial is a warp's, which joins them to a state of its own, headers by
+// lanes, rows 16 bytes a lane, all loads under way together; the warps' states
+// meet in shared memory after the only barrier.
+constexpr int kJoinWarps = 8;
 
-__global__ void __launch_bounds__(kJoinThreads) A8JoinKernel(A8Args a) {
+template <int V>  // float4 of a row per lane
+__global__ void __launch_bounds__(kJoinWarps * 32) A8JoinKernel(A8Args a) {
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
-  __shared__ float red[3][32];
-  __shared__ float accs[kJoinThreads / 32][256];
+  __shared__ float4 accs[kJoinWarps][32 * V];
+  __shared__ float ms[kJoinWarps], ls[kJoinWarps], bads[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int h = blockIdx.x, seq = blockIdx.y;
   const int64_t at = static_cast<int64_t>(seq) * a.n_heads + h;
-  const int kv = h / a.group;
-  const int2 span = a.spans[static_cast<int64_t>(seq) * a.kv_heads + kv];
+  const int hd4 = a.hd >> 2;
+  const int2 span = a.spans[static_cast<int64_t>(seq) * a.kv_heads + h / a.group];
+  float4* out = reinterpret_cast<float4*>(a.out + at * a.hd);
   if (LengthOf(a, seq) == 0) {  // its span was not written
     if (h == 0 && threadIdx.x == 0 && a.lengths[seq] != 0 && a.status != nullptr)
       atomicOr(a.status, MLB_STATUS_BAD_LENGTH);
-    for (int d = threadIdx.x; d < a.hd; d += kJoinThreads) a.out[at * a.hd + d] = 0.0f;
+    if (threadIdx.x < hd4) out[threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (threadIdx.x == 0) a.lse[at] = make_float2(0.0f, 0.0f);
     return;
   }
-  if (span.y == 1) return;  // finished by its warp
-  const int64_t w0 = span.x;
   const int n = span.y;
-  const int stride = a.hd + kPartHead;
-  // worker w0 found the sequence's beginning (its slot 1), the others its rest
+  if (n == 1) return;  // finished by its warp
+  const int stride4 = hd4 + kPartHead / 4;
+  // worker span.x found the sequence's beginning (its slot 1), the others its
+  // rest
   const auto part = [&](int i) {
-    return a.partial + (((w0 + i) * 2 + (i == 0 ? 1 : 0)) * a.group + h % a.group) * stride;
+    return reinterpret_cast<const float4*>(a.partial) +
+           (((static_cast<int64_t>(span.x) + i) * 2 + (i == 0 ? 1 : 0)) * a.group + h % a.group) *
+               stride4;
   };
-  float m = -INFINITY, bad = 0.0f;
-  for (int i = threadIdx.x; i < n; i += kJoinThreads) {
-    const float4 x = *reinterpret_cast<const float4*>(part(i));
-    m = fmaxf(m, x.x);
-    bad = fmaxf(bad, x.z);
-  }
-  m = BlockMax(m, red[0]);
-  bad = BlockMax(bad, red[1]);
-  float l = 0.0f;
-  for (int i = threadIdx.x; i < n; i += kJoinThreads) {
-    const float4 x = *reinterpret_cast<const float4*>(part(i));
-    l += x.x == -INFINITY ? x.y : x.y * Exp2(x.x - m);
-  }
-  l = BlockSum(l, red[2]);
-  float acc[8] = {};
-#pragma unroll 4
-  for (int i = warp; i < n; i += kJoinThreads / 32) {
-    const float* x = part(i);
-    const float f = Exp2(x[0] - m);
+  float m = -INFINITY, l = 0.0f, bad = 0.0f;
+  float4 acc[V];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (32 * j < a.hd) acc[j] = fmaf(x[kPartHead + 32 * j + lane], f, acc[j]);
+  for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = warp; base < n; base += 32 * kJoinWarps) {  // 32 partials
+    const int mine = base + kJoinWarps * lane;
+    const float4 head = mine < n ? part(mine)[0] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    const float m_new = fmaxf(m, WarpMax(head.x));
+    const float keep = m == m_new ? 1.0f : Exp2(m - m_new);
+    // a partial of NaN scores alone has m = -inf and keeps its NaN
+    const float f = head.x == -INFINITY ? 0.0f : Exp2(head.x - m_new);
+    l = fmaf(l, keep, WarpSum(head.x == -INFINITY ? head.y : head.y * f));
+    bad = fmaxf(bad, WarpMax(head.z));
+    m = m_new;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      acc[v] = make_float4(acc[v].x * keep, acc[v].y * keep, acc[v].z * keep, acc[v].w * keep);
+    const int rows = min(32, (n - base + kJoinWarps - 1) / kJoinWarps);
+#pragma unroll 8
+    for (int i = 0; i < rows; ++i) {
+      const float4* x = part(base + kJoinWarps * i) + kPartHead / 4;
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float4 y =
+            lane + 32 * v < hd4 ? x[lane + 32 * v] : make_float4(0.f, 0.f, 0.f, 0.f);
+        acc[v].x = fmaf(y.x, fi, acc[v].x);
+        acc[v].y = fmaf(y.y, fi, acc[v].y);
+        acc[v].z = fmaf(y.z, fi, acc[v].z);
+        acc[v].w = fmaf(y.w, fi, acc[v].w);
+      }
+    }
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (32 * j < a.hd) accs[warp][32 * j + lane] = acc[j];
+  for (int v = 0; v < V; ++v) accs[warp][lane + 32 * v] = acc[v];
+  if (lane == 0) {
+    ms[warp] = m;
+    ls[warp] = l;
+    bads[warp] = bad;
+  }
   __syncthreads();
-  if (threadIdx.x < a.hd) {
-    float o = 0.0f;
+  if (threadIdx.x >= hd4) return;
+  m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) o += accs[w][threadIdx.x];
-    a.out[at * a.hd + threadIdx.x] = bad != 0.0f ? 0.0f : o / l;
+  for (int w = 0; w < kJoinWarps; ++w) {
+    m = fmaxf(m, ms[w]);
+    bad = fmaxf(bad, bads[w]);
   }
+  l = 0.0f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float f = ms[w] == -INFINITY ? 0.0f : Exp2(ms[w] - m);
+    l += ms[w] == -INFINITY ? ls[w] : ls[w] * f;
+    const float4 x = accs[w][threadIdx.x];
+    o.x = fmaf(x.x, f, o.x);
+    o.y = fmaf(x.y, f, o.y);
+    o.z = fmaf(x.z, f, o.z);
+    o.w = fmaf(x.w, f, o.w);
+  }
+  const float inv = 1.0f / l;
+  out[threadIdx.x] = bad != 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                 : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   if (threadIdx.x == 0) a.lse[at] = bad != 0.0f ? make_float2(0.0f, 0.0f) : make_float2(m, l);
 }
 
@@ -547,21 +581,18 @@ __global__ void __launch_bounds__(256) A8MassKernel(A8Args a, const float* mass_
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int64_t seq = blockIdx.y;
   if (c >= a.table_cols) return;
-  const int64_t length = a.lengths[seq];
-  const int64_t unit_cols = a.table_cols * a.block / kUnit;
-  const int64_t units = (length + kUnit - 1) / kUnit;
+  const int per = a.block / kUnit;
+  const int64_t unit_cols = a.table_cols * per;
   const float2* lse = a.lse + seq * a.n_heads;
+  const float2* of = a.units + (seq * unit_cols + c * per) * a.n_heads;
+  const int units = UnitsOf(a, seq);  // (a sequence with a bad length has none)
   float sum = 0.0f;
-  if (length > 0 && length <= a.table_cols * a.block) {
-    const int64_t u0 = c * (a.block / kUnit);
-    const int64_t u1 = min(u0 + a.block / kUnit, units);
-    for (int64_t u = u0; u < u1; ++u)
-      for (int h = lane; h < a.n_heads; h += 32) {
-        const float2 total = lse[h];  // L = 0: a bad block, nothing was collected
-        const float2 x = a.units[(seq * unit_cols + u) * a.n_heads + h];
-        if (total.y != 0.0f) sum += x.y * Exp2(x.x - total.x) / total.y;
-      }
-  }
+  for (int u = 0; u < per; ++u)
+    for (int h = lane; h < a.n_heads; h += 32) {
+      const float2 total = lse[h];  // L = 0: a bad block, nothing was collected
+      const float2 x = of[static_cast<int64_t>(u) * a.n_heads + h];
+      if (c * per + u < units && total.y != 0.0f) sum += x.y * Exp2(x.x - total.x) / total.y;
+    }
   sum = WarpSum(sum);
   if (lane == 0) {
     const int64_t i = seq * a.table_cols + c;
@@ -696,8 +727,9 @@ extern "C" int mlb_attention_kv8_f32(const float* q, const int8_t* k_codes, cons
     }
     if (rc != MLB_OK) return rc;
   }
-  Launch(A8JoinKernel, dim3(static_cast<unsigned>(n_heads), static_cast<unsigned>(n_seqs)),
-         kJoinThreads, 0, s, a);
+  Launch(head_dim <= 128 ? A8JoinKernel<1> : A8JoinKernel<2>,
+         dim3(static_cast<unsigned>(n_heads), static_cast<unsigned>(n_seqs)), kJoinWarps * 32, 0, s,
+         a);
   if (mass_out != nullptr && table_cols > 0)
     Launch(A8MassKernel, dim3(static_cast<unsigned>((table_cols + 7) / 8),
                               static_cast<unsigned>(n_seqs)),
