@@ -16,6 +16,7 @@ namespace mlb {
 namespace {
 
 constexpr int kKv8Threads = 256;
+constexpr int kKv8Warps = kKv8Threads / 32;
 
 // What a CTA works on: columns of the table that the rows of packed
 // sequences touch, counted through all sequences.
@@ -25,10 +26,12 @@ struct Kv8Rows {
   const int32_t* positions;
   int64_t table_cols;
   int64_t n_blocks;
-  int64_t rows;
+  int rows;
   int n_seqs;
   int block;   // tokens per block
+  int shift;   // its log2
   int kv_heads;
+  int heads;   // kv heads that a CTA takes one after another
   int hd;
   int32_t* status;
 };
@@ -44,223 +47,305 @@ __device__ __forceinline__ void Raise(int32_t* status, int bits) {
   if (status != nullptr) atomicOr(status, bits);
 }
 
-// The index-th touched block over all sequences.  All threads of the CTA
-// call it; every thread receives the span.  Sequences are scanned
-// kKv8Threads at a time.
-__device__ Kv8Span FindSpan(const Kv8Rows& a, int64_t index) {
-  __shared__ int64_t warp_sum[kKv8Threads / 32];
-  __shared__ Kv8Span found;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) found = Kv8Span{0, -1, 0, 0};
-  int64_t before = 0;
-  for (int base = 0; base < a.n_seqs; base += kKv8Threads) {
-    const int i = base + static_cast<int>(threadIdx.x);
-    int64_t touched = 0, begin = 0, end = 0, position = 0;
+// The index-th touched block over all sequences, for all lanes of the warp
+// that calls it (32 sequences a step, no barrier: the warps of a CTA all do it
+// and find the offsets in L1).  Sums wrap at 32 bits where bad ranges overlap;
+// a found span lies in its own sequence's range whatever they are.
+__device__ __forceinline__ Kv8Span FindSpan(const Kv8Rows& a, uint32_t index) {
+  const int lane = threadIdx.x & 31;
+  Kv8Span s{0, -1, 0, 0};
+  uint32_t before = 0;
+  for (int base = 0; base < a.n_seqs; base += 32) {
+    const int i = base + lane;
+    uint32_t touched = 0, position = 0, count = 0;
+    int begin = 0;
     bool lost = false;
     if (i < a.n_seqs) {
       begin = a.offsets[i];
-      end = a.offsets[i + 1];
-      position = a.positions[i];
-      lost = position < 0;  // its rows have no place: counted from 0, in no block
-      if (lost) position = 0;
+      const int end = a.offsets[i + 1], p = a.positions[i];
+      lost = p < 0;  // its rows have no place: counted from 0, in no block
+      position = lost ? 0 : p;
       if (begin < 0 || end < begin || end > a.rows) {
         if (index == 0) Raise(a.status, MLB_STATUS_BAD_LENGTH);
       } else if (end > begin) {
-        touched = (position + end - begin - 1) / a.block - position / a.block + 1;
+        count = end - begin;
+        touched = ((position + count - 1) >> a.shift) - (position >> a.shift) + 1;
         if (lost && index == 0) Raise(a.status, MLB_STATUS_BAD_POSITION);
       }
     }
-    int64_t sum = touched;  // inclusive scan over the CTA
+    uint32_t upto = touched;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
+      const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
     }
-    if (lane == 31) warp_sum[warp] = sum;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kKv8Threads / 32; ++w) {
-      if (w < warp) sum += warp_sum[w];
-      total += warp_sum[w];
-    }
-    const int64_t local = index - (before + sum - touched);
-    if (touched > 0 && local >= 0 && local < touched) {
-      const int64_t col = position / a.block + local;
-      const int64_t t0 = local == 0 ? position : col * a.block;
-      const int64_t t1 = min(position + end - begin, (col + 1) * a.block);
-      Kv8Span s;
-      s.row = begin + t0 - position;
-      s.first = static_cast<int>(t0 - col * a.block);
+    const uint32_t local = index - (before + upto - touched);
+    const uint32_t found = __ballot_sync(0xffffffffu, local < touched);
+    if (found != 0 && s.count == 0) {
+      const int src = __ffs(found) - 1;
+      const uint32_t mine = __shfl_sync(0xffffffffu, local, src);
+      position = __shfl_sync(0xffffffffu, position, src);
+      count = __shfl_sync(0xffffffffu, count, src);
+      begin = __shfl_sync(0xffffffffu, begin, src);
+      lost = __shfl_sync(0xffffffffu, lost ? 1 : 0, src) != 0;
+      const uint32_t col = (position >> a.shift) + mine;
+      const uint32_t t0 = mine == 0 ? position : col << a.shift;
+      const uint32_t t1 = min(position + count, (col + 1) << a.shift);
+      s.row = static_cast<int64_t>(begin) + (t0 - position);
+      s.first = static_cast<int>(t0 & (a.block - 1));
       s.count = static_cast<int>(t1 - t0);
-      s.block = -1;
       if (col >= a.table_cols) {
-        Raise(a.status, MLB_STATUS_BAD_POSITION);
+        if (threadIdx.x == 0) Raise(a.status, MLB_STATUS_BAD_POSITION);
       } else if (!lost) {
-        const int32_t id = a.table[i * a.table_cols + col];
-        if (id < 0 || id >= a.n_blocks)
-          Raise(a.status, MLB_STATUS_BAD_BLOCK);
-        else
-          s.block = id;
+        const int32_t id = a.table[(base + src) * a.table_cols + col];
+        if (id >= 0 && id < a.n_blocks) s.block = id;
+        else if (threadIdx.x == 0) Raise(a.status, MLB_STATUS_BAD_BLOCK);
       }
-      found = s;
     }
-    before += total;
-    __syncthreads();
-    if (index < before && index != 0) break;  // index 0 looks at every sequence's range
+    before += __shfl_sync(0xffffffffu, upto, 31);
+    if (s.count != 0 && index != 0) break;  // index 0 looks at every sequence's range
   }
-  return found;
+  return s;
 }
 
-// round(x / s) as if the quotient were exact, clamped to [-127, 127]; inv is
-// 1 / s.  r, the rounded approximate quotient, is off by at most one; the
-// remainder x - r s is a multiple of the last place of s (or of x, for
-// |r| <= 1) below 2 s, so the fused multiply-add gives it without error.
-__device__ __forceinline__ int Quantise(float x, float s, float inv) {
-  // 1 / s of a scale below 2^-100 may overflow: divide instead
-  float r = rintf(s >= 7.9e-31f ? x * inv : __fdiv_rn(x, s));
+// 1.5 * 2^23: adding it leaves a value of up to 2^22 rounded (half to even) in
+// the low mantissa bits, in two's complement.
+constexpr float kRound = 12582912.0f;
+
+// kRound + round(x / s) as if the quotient were exact; inv is about 1 / s, hs
+// is s / 2.  The first rounding is off by at most one; the remainder x - r s
+// is a multiple of the last place of s (or of x, for |r| <= 1) below 2 s, so
+// the fused multiply-add gives it without error.
+__device__ __forceinline__ float Quantise(float x, float s, float inv, float hs) {
+  float t = fmaf(x, inv, kRound);
+  const float r = t - kRound;
   const float e = fmaf(-r, s, x);
-  const float twice = fabsf(e) + fabsf(e);
-  const bool odd = (static_cast<int>(r) & 1) != 0;
-  if (twice > s || (twice == s && odd)) r += copysignf(1.0f, e);
-  return static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
+  if (fabsf(e) >= hs) {  // rare: on a half or past it
+    const bool odd = (__float_as_uint(t) & 1u) != 0;
+    if (fabsf(e) > hs || odd) t += copysignf(1.0f, e);
+  }
+  return t;
+}
+// The same where 1 / s may overflow or s / 2 be inexact (s below 2^-100).
+__device__ __forceinline__ float QuantiseTiny(float x, float s) {
+  float r = rintf(__fdiv_rn(x, s));
+  const float e = fmaf(-r, s, x), twice = fabsf(e) + fabsf(e);
+  if (twice > s || (twice == s && (static_cast<int>(r) & 1) != 0)) r += copysignf(1.0f, e);
+  return fminf(fmaxf(r, -127.0f), 127.0f) + kRound;
+}
+// An earlier code c under a larger scale: kRound + round(c from / to).  c from
+// is taken as a sum of two fp32 numbers, its remainder by r to is then exact
+// in two parts, and the sign of their sum against a half is what rounds.
+__device__ __forceinline__ float Requantise(float c, float from, float to, float ratio) {
+  const float p = c * from, p_low = fmaf(c, from, -p);
+  const float r = rintf(c * ratio);
+  const float e = fmaf(-r, to, p);
+  const float side = copysignf(1.0f, e);
+  const float past = (fabsf(e) + fabsf(e) - to) + 2.0f * side * p_low;  // its sign is exact
+  float t = r + kRound;
+  if (past > 0.0f || (past == 0.0f && (__float_as_uint(t) & 1u) != 0)) t += side;
+  return t;
 }
 
-// An earlier code under a larger scale: c s / s' has at most 31 significant
-// bits above and 24 below the line, so a quotient that is no tie is further
-// from one than a double's rounding.
-__device__ __forceinline__ int Requantise(int c, double from, double to) {
-  return static_cast<int>(rint(static_cast<double>(c) * from / to));
+// Low bytes of four words.
+__device__ __forceinline__ uint32_t LowBytes(float a, float b, float c, float d) {
+  const uint32_t x = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+  const uint32_t y = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+  return __byte_perm(x, y, 0x5410);
+}
+// Code e (0..3) of a word as a float: the sign bit flipped makes it code + 128,
+// 0x4b0000 above it the number 2^23 + code + 128.
+__device__ __forceinline__ float CodeOf(uint32_t flipped, int e) {
+  return __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7540 + e)) - 8388736.0f;
+}
+
+// 16 earlier codes under a larger scale (kept out of line: few blocks need it).
+__device__ __noinline__ uint4 Moved(uint4 old, float from, float to, float ratio) {
+  const auto word = [&](uint32_t c) {
+    const uint32_t f = c ^ 0x80808080u;
+    return LowBytes(
+        Requantise(CodeOf(f, 0), from, to, ratio), Requantise(CodeOf(f, 1), from, to, ratio),
+        Requantise(CodeOf(f, 2), from, to, ratio), Requantise(CodeOf(f, 3), from, to, ratio));
+  };
+  return make_uint4(word(old.x), word(old.y), word(old.z), word(old.w));
+}
+// The first n bytes (of 4) of `old`, the rest of `fresh`.
+__device__ __forceinline__ uint32_t Merge(uint32_t old, uint32_t fresh, int n) {
+  const uint32_t mask = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+  return (old & mask) | (fresh & ~mask);
 }
 
 struct Kv8WriteArgs {
   Kv8Rows at;
-  int8_t* codes[2];
-  float* scales[2];
-  const float* x[2];
+  int8_t *k_codes, *v_codes;
+  float *k_scales, *v_scales;
+  const float *k, *v;
 };
 
-// CTA = (touched block, kv head, K or V).  The new rows pass through shared
-// memory once (their maximum, then their codes).
-__global__ void __launch_bounds__(kKv8Threads) Kv8WriteKernel(Kv8WriteArgs a) {
+// CTA = (touched block, some kv heads, K or V).  An item is 16 codes that lie
+// side by side: 16 dimensions of a token in K, 16 tokens of a dimension in V
+// (neighbouring lanes neighbouring dimensions, so that a row of new values is
+// read in full lines); a thread holds NI items in registers from the maximum
+// to the codes.
+template <int NI>
+__global__ void __launch_bounds__(kKv8Threads, NI == 1 ? 4 : NI == 2 ? 3 : 1) Kv8WriteKernel(Kv8WriteArgs a) {
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
-  extern __shared__ __align__(16) float rows[];  // [count][hd]
-  __shared__ uint32_t top_of[kKv8Threads / 32];
+  __shared__ uint32_t top_of[2][kKv8Warps];
   const Kv8Span s = FindSpan(a.at, blockIdx.x);
   if (s.block < 0 || s.count == 0) return;
-  const int which = blockIdx.z, head = blockIdx.y;
-  const int hd = a.at.hd, B = a.at.block, hd4 = hd >> 2;
-  const float* x = a.x[which] + (s.row * a.at.kv_heads + head) * hd;
+  const int which = blockIdx.z;
+  const float* rows = which == 0 ? a.k : a.v;
+  int8_t* pool = which == 0 ? a.k_codes : a.v_codes;
+  float* scales = which == 0 ? a.k_scales : a.v_scales;
+  const int hd = a.at.hd, B = a.at.block;
+  const int per = which == 0 ? hd >> 4 : hd;  // items of a token, or dimensions
+  const int items = (hd >> 4) * B;
   const int64_t row_stride = static_cast<int64_t>(a.at.kv_heads) * hd;
-  // magnitudes as integers: NaN above Inf above every number
-  uint32_t top = 0;
-  for (int i = threadIdx.x; i < s.count * hd4; i += kKv8Threads) {
-    const int t = i / hd4, c = i - t * hd4;
-    const float4 v = LoadStream(reinterpret_cast<const float4*>(x + t * row_stride) + c);
-    reinterpret_cast<float4*>(rows)[i] = v;
-    top = max(max(top, __float_as_uint(v.x) & 0x7fffffffu),
-              max(__float_as_uint(v.y) & 0x7fffffffu,
-                  max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) top_of[threadIdx.x >> 5] = top;
-  float* scale_at = a.scales[which] + s.block * a.at.kv_heads + head;
-  const float had = s.first > 0 ? *scale_at : 0.0f;
-  __syncthreads();
+  const int last = min((static_cast<int>(blockIdx.y) + 1) * a.at.heads, a.at.kv_heads);
+  for (int head = blockIdx.y * a.at.heads, turn = 0; head < last; ++head, turn ^= 1) {
+    const float* x = rows + s.row * row_stride + head * hd;
+    const int64_t at = s.block * a.at.kv_heads + head;
+    uint4* codes = reinterpret_cast<uint4*>(pool + at * B * hd);
+    float* scale_at = scales + at;
+    const float had = s.first > 0 ? *scale_at : 0.0f;
+    float v[NI][16];
+    // magnitudes as integers: NaN above Inf above every number
+    uint32_t top = 0;
+    const bool whole = s.count == B;
 #pragma unroll
-  for (int w = 0; w < kKv8Threads / 32; ++w) top = max(top, top_of[w]);
-  const float fresh = __fdiv_rn(__uint_as_float(top), 127.0f);
-  const float scale =
-      __float_as_uint(fresh) > (__float_as_uint(had) & 0x7fffffffu) ? fresh : had;
-  if (threadIdx.x == 0) *scale_at = scale;  // every thread has read it
-  const bool usable = scale > 0.0f && scale < INFINITY;
-  const float inv = 1.0f / scale;
-  const bool moved = scale != had;
-  int8_t* codes = a.codes[which] + (s.block * a.at.kv_heads + head) * static_cast<int64_t>(B) * hd;
-  const auto code = [&](int t, int d, int old) -> int {  // token t of the block, dimension d
-    if (!usable) return 0;
-    if (t < s.first) return moved ? Requantise(old, had, scale) : old;
-    if (t >= s.first + s.count) return 0;
-    return Quantise(rows[(t - s.first) * hd + d], scale, inv);
-  };
-  if (which == 0) {  // [B][hd]: 4 dimensions of a token
-    for (int i = threadIdx.x; i < B * hd4; i += kKv8Threads) {
-      const int t = i / hd4, d = 4 * (i - t * hd4);
-      char4 c = t < s.first ? reinterpret_cast<char4*>(codes)[i] : make_char4(0, 0, 0, 0);
-      c = make_char4(code(t, d, c.x), code(t, d + 1, c.y), code(t, d + 2, c.z),
-                     code(t, d + 3, c.w));
-      reinterpret_cast<char4*>(codes)[i] = c;
-    }
-  } else {  // [hd][B]: 16 tokens of a dimension, neighbouring lanes neighbouring dimensions
-    for (int i = threadIdx.x; i < hd * (B >> 4); i += kKv8Threads) {
-      const int d = i % hd, t0 = 16 * (i / hd);
-      uint4* at = reinterpret_cast<uint4*>(codes + d * B + t0);
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (t0 < s.first) {
-        const uint4 old = *at;
-        w[0] = old.x; w[1] = old.y; w[2] = old.z; w[3] = old.w;
-      }
+    for (int n = 0; n < NI; ++n) {
+      const int i = n * kKv8Threads + threadIdx.x;
+      const int q = i / per, r = i - q * per;
+      if (which == 0) {
+        const int t = q - s.first;
+        const bool in = i < items && t >= 0 && t < s.count;
+        const float4* from = reinterpret_cast<const float4*>(x + t * row_stride + 16 * r);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t packed = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int old = static_cast<int8_t>(w[j] >> (8 * e));
-          packed |= (static_cast<uint32_t>(code(t0 + 4 * j + e, d, old)) & 0xffu) << (8 * e);
+        for (int j = 0; j < 4; ++j) {
+          const float4 y = in ? LoadStream(from + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[n][4 * j] = y.x;
+          v[n][4 * j + 1] = y.y;
+          v[n][4 * j + 2] = y.z;
+          v[n][4 * j + 3] = y.w;
         }
-        w[j] = packed;
+      } else {
+        const int t = 16 * q - s.first;
+        const float* from = x + t * row_stride + r;
+        if (whole && i < items) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j, from += row_stride) v[n][j] = __ldcs(from);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j, from += row_stride)
+            v[n][j] = i < items && t + j >= 0 && t + j < s.count ? __ldcs(from) : 0.0f;
+        }
       }
-      *at = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[n][j]) & 0x7fffffffu);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) top_of[turn][threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kKv8Warps; ++w) top = max(top, top_of[turn][w]);
+    const float fresh = __fdiv_rn(__uint_as_float(top), 127.0f);
+    const float scale =
+        __float_as_uint(fresh) > (__float_as_uint(had) & 0x7fffffffu) ? fresh : had;
+    if (threadIdx.x == 0) *scale_at = scale;  // every thread has read it
+    const bool usable = scale > 0.0f && scale < INFINITY;
+    const bool tiny = scale < 7.9e-31f;
+    const bool moved = scale != had;
+    const float inv = 1.0f / scale, hs = 0.5f * scale, ratio = had / scale;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const int i = n * kKv8Threads + threadIdx.x;
+      if (i >= items) break;
+      const int q = i / per, r = i - q * per;
+      // places of the item's tokens: the same for all in K, 16 in a row in V
+      const int t0 = which == 0 ? q : 16 * q, t1 = which == 0 ? q : 16 * q + 15;
+      if (t1 < s.first && !moved && usable) continue;  // earlier codes under the same scale
+      uint4* to = codes + (which == 0 ? i : r * (B >> 4) + q);
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (usable) {
+        // (0 where there is no new value)
+        float worst = 0.0f;
+        float t[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          t[j] = fmaf(v[n][j], inv, kRound);
+          worst = fmaxf(worst, fabsf(fmaf(kRound - t[j], scale, v[n][j])));
+        }
+        if (worst >= hs || tiny) {  // rare: a value on a half or past it
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            t[j] = tiny ? QuantiseTiny(v[n][j], scale) : Quantise(v[n][j], scale, inv, hs);
+        }
+        w = make_uint4(LowBytes(t[0], t[1], t[2], t[3]), LowBytes(t[4], t[5], t[6], t[7]),
+                       LowBytes(t[8], t[9], t[10], t[11]), LowBytes(t[12], t[13], t[14], t[15]));
+        if (t0 < s.first) {
+          uint4 old = *to;
+          if (moved) old = Moved(old, had, scale, ratio);
+          // bytes of the places before the first new one: all of them in K
+          const int n_old = which == 0 ? 16 : s.first - t0;
+          w = make_uint4(Merge(old.x, w.x, n_old), Merge(old.y, w.y, n_old - 4),
+                         Merge(old.z, w.z, n_old - 8), Merge(old.w, w.w, n_old - 12));
+        }
+      }
+      *to = w;
     }
   }
 }
 
 struct Kv8ReadArgs {
   Kv8Rows at;
-  const int8_t* codes[2];
-  const float* scales[2];
-  float* x[2];
+  const int8_t *k_codes, *v_codes;
+  const float *k_scales, *v_scales;
+  float *k, *v;
 };
 
-// CTA = (touched block, kv head, K or V).
+// CTA = (touched block, some kv heads, K or V); items as in the write.
 __global__ void __launch_bounds__(kKv8Threads) Kv8ReadKernel(Kv8ReadArgs a) {
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
+  const int which = blockIdx.z;
+  float* rows = which == 0 ? a.k : a.v;
+  const int8_t* pool = which == 0 ? a.k_codes : a.v_codes;
+  const float* scales = which == 0 ? a.k_scales : a.v_scales;
+  if (rows == nullptr) return;
   const Kv8Span s = FindSpan(a.at, blockIdx.x);
-  const int which = blockIdx.z, head = blockIdx.y;
-  if (s.count == 0 || a.x[which] == nullptr) return;
-  const int hd = a.at.hd, B = a.at.block, hd4 = hd >> 2;
-  float* x = a.x[which] + (s.row * a.at.kv_heads + head) * hd;
+  if (s.count == 0) return;
+  const int hd = a.at.hd, B = a.at.block;
+  const int per = which == 0 ? hd >> 4 : hd;
+  const int items = (hd >> 4) * B;
   const int64_t row_stride = static_cast<int64_t>(a.at.kv_heads) * hd;
-  if (s.block < 0) {
-    for (int i = threadIdx.x; i < s.count * hd4; i += kKv8Threads)
-      reinterpret_cast<float4*>(x + (i / hd4) * row_stride)[i % hd4] =
-          make_float4(0.f, 0.f, 0.f, 0.f);
-    return;
-  }
-  const float scale = a.scales[which][s.block * a.at.kv_heads + head];
-  const int8_t* codes =
-      a.codes[which] + (s.block * a.at.kv_heads + head) * static_cast<int64_t>(B) * hd;
-  if (which == 0) {
-    for (int i = threadIdx.x; i < s.count * hd4; i += kKv8Threads) {
-      const int t = i / hd4, c = i - t * hd4;
-      const char4 v = reinterpret_cast<const char4*>(codes + (s.first + t) * hd)[c];
-      StoreStream(reinterpret_cast<float4*>(x + t * row_stride) + c,
-                  make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale));
-    }
-  } else {
-    for (int i = threadIdx.x; i < hd * (B >> 4); i += kKv8Threads) {
-      const int d = i % hd, t0 = 16 * (i / hd);
-      if (t0 + 16 <= s.first || t0 >= s.first + s.count) continue;
-      const uint4 v = *reinterpret_cast<const uint4*>(codes + d * B + t0);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  const int last = min((static_cast<int>(blockIdx.y) + 1) * a.at.heads, a.at.kv_heads);
+  for (int head = blockIdx.y * a.at.heads; head < last; ++head) {
+    float* x = rows + s.row * row_stride + head * hd;
+    const int64_t at = s.block * a.at.kv_heads + head;
+    const uint4* codes = reinterpret_cast<const uint4*>(pool + at * B * hd);
+    const float scale = s.block >= 0 ? scales[at] : 0.0f;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < items; i += kKv8Threads) {
+      const int q = i / per, r = i - q * per;
+      const int t0 = (which == 0 ? q : 16 * q) - s.first;
+      if (t0 >= s.count || t0 + (which == 0 ? 0 : 15) < 0) continue;
+      uint4 y = make_uint4(0, 0, 0, 0);
+      if (s.block >= 0) y = codes[which == 0 ? i : r * (B >> 4) + q];
+      const uint32_t w[4] = {y.x ^ 0x80808080u, y.y ^ 0x80808080u, y.z ^ 0x80808080u,
+                             y.w ^ 0x80808080u};
+      float v[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int t = t0 + j - s.first;
-        if (t >= 0 && t < s.count)
-          x[t * row_stride + d] =
-              static_cast<float>(static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3)))) * scale;
+      for (int j = 0; j < 16; ++j) v[j] = CodeOf(w[j >> 2], j & 3) * scale;
+      if (which == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          StoreStream(reinterpret_cast<float4*>(x + t0 * row_stride + 16 * r) + j,
+                      make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (t0 + j >= 0 && t0 + j < s.count) __stcs(x + (t0 + j) * row_stride + r, v[j]);
       }
     }
   }
@@ -284,6 +369,23 @@ const char* Kv8Shape(int64_t n_blocks, int block_tokens, int64_t table_cols, int
 int64_t MostTouched(int64_t rows, int64_t n_seqs, int block) {
   const int64_t by_seq = rows / block + 2 * n_seqs;
   return rows < by_seq ? rows : by_seq;
+}
+
+Kv8Rows RowsOf(const int32_t* table, const int32_t* offsets, const int32_t* positions,
+               int64_t table_cols, int64_t n_blocks, int64_t rows, int64_t n_seqs, int block,
+               int kv_heads, int hd, int32_t* status) {
+  Kv8Rows a{table, offsets, positions, table_cols, n_blocks, static_cast<int>(rows),
+            static_cast<int>(n_seqs), block, block == 32 ? 5 : block == 64 ? 6 : 7, kv_heads,
+            1, hd, status};
+  // A CTA finds its block once for several heads where the grid stays above
+  // 16 CTAs per SM: in a decode step each head has its own CTA.
+  const int64_t ctas = 2 * MostTouched(rows, n_seqs, block) * kv_heads;
+  while (a.heads < kv_heads && ctas / (2 * a.heads) >= 16 * SmCount()) a.heads *= 2;
+  return a;
+}
+dim3 GridOf(const Kv8Rows& a) {
+  return dim3(static_cast<unsigned>(MostTouched(a.rows, a.n_seqs, a.block)),
+              static_cast<unsigned>((a.kv_heads + a.heads - 1) / a.heads), 2);
 }
 
 int Kv8Check(const char* op, bool null, bool aligned, int64_t n_blocks, int block_tokens,
@@ -452,24 +554,21 @@ extern "C" int mlb_kv8_write_f32(int8_t* k_codes, int8_t* v_codes, float* k_scal
       block_tokens, table_cols, n_seqs, rows, n_kv_heads, head_dim);
   if (rc != MLB_OK || rows == 0 || n_seqs == 0) return rc;
   Kv8WriteArgs a{};
-  a.at = Kv8Rows{table, offsets, positions, table_cols, n_blocks, rows,
-                 static_cast<int>(n_seqs), block_tokens, n_kv_heads, head_dim, status};
-  a.codes[0] = k_codes;
-  a.codes[1] = v_codes;
-  a.scales[0] = k_scales;
-  a.scales[1] = v_scales;
-  a.x[0] = k;
-  a.x[1] = v;
-  const int shm = block_tokens * head_dim * 4;
-  if (shm > 48 * 1024 &&
-      cudaFuncSetAttribute(Kv8WriteKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shm) !=
-          cudaSuccess) {
-    cudaGetLastError();
-    return Fail(MLB_ERR_CUDA, "mlb_kv8_write_f32: shared memory opt-in");
-  }
-  const dim3 grid(static_cast<unsigned>(MostTouched(rows, n_seqs, block_tokens)),
-                  static_cast<unsigned>(n_kv_heads), 2);
-  Launch(Kv8WriteKernel, grid, kKv8Threads, static_cast<size_t>(shm), AsStream(stream), a);
+  a.at = RowsOf(table, offsets, positions, table_cols, n_blocks, rows, n_seqs, block_tokens,
+                n_kv_heads, head_dim, status);
+  a.k_codes = k_codes;
+  a.v_codes = v_codes;
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  a.k = k;
+  a.v = v;
+  const dim3 grid = GridOf(a.at);
+  const int items = (block_tokens * head_dim / 16 + kKv8Threads - 1) / kKv8Threads;
+  Launch(items <= 1   ? Kv8WriteKernel<1>
+         : items <= 2 ? Kv8WriteKernel<2>
+         : items <= 4 ? Kv8WriteKernel<4>
+                      : Kv8WriteKernel<8>,
+         grid, kKv8Threads, 0, AsStream(stream), a);
   return CheckLaunch("mlb_kv8_write_f32");
 }
 
@@ -489,17 +588,15 @@ extern "C" int mlb_kv8_read_f32(const int8_t* k_codes, const int8_t* v_codes,
       block_tokens, table_cols, n_seqs, rows, n_kv_heads, head_dim);
   if (rc != MLB_OK || rows == 0 || n_seqs == 0) return rc;
   Kv8ReadArgs a{};
-  a.at = Kv8Rows{table, offsets, positions, table_cols, n_blocks, rows,
-                 static_cast<int>(n_seqs), block_tokens, n_kv_heads, head_dim, status};
-  a.codes[0] = k_codes;
-  a.codes[1] = v_codes;
-  a.scales[0] = k_scales;
-  a.scales[1] = v_scales;
-  a.x[0] = k;
-  a.x[1] = v;
-  const dim3 grid(static_cast<unsigned>(MostTouched(rows, n_seqs, block_tokens)),
-                  static_cast<unsigned>(n_kv_heads), 2);
-  Launch(Kv8ReadKernel, grid, kKv8Threads, 0, AsStream(stream), a);
+  a.at = RowsOf(table, offsets, positions, table_cols, n_blocks, rows, n_seqs, block_tokens,
+                n_kv_heads, head_dim, status);
+  a.k_codes = k_codes;
+  a.v_codes = v_codes;
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  a.k = k;
+  a.v = v;
+  Launch(Kv8ReadKernel, GridOf(a.at), kKv8Threads, 0, AsStream(stream), a);
   return CheckLaunch("mlb_kv8_read_f32");
 }
 
