@@ -403,8 +403,6 @@ int Kv8Check(const char* op, bool null, bool aligned, int64_t n_blocks, int bloc
 // ---------------------------------------------------------------------------
 // Eviction.
 
-constexpr int kEvictThreads = 1024;
-
 struct EvictArgs {
   const int32_t* table;
   const int32_t* lengths;
@@ -426,44 +424,72 @@ __device__ __forceinline__ uint32_t MassKey(float m) {
   return (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
 }
 
-// CTA = one sequence.  The g-th smallest key of the candidates is found digit
-// by digit (four 8-bit histograms); everything below it leaves, and of the
-// keys equal to it the first ones that are still wanted.  A prefix count
-// then closes up ids and masses.
-__global__ void __launch_bounds__(kEvictThreads) EvictKernel(EvictArgs a) {
+// CTA = one sequence, T threads.  The g-th smallest key of the candidates is
+// found digit by digit (8-bit histograms); everything below it leaves, and of
+// the keys equal to it the first ones that are still wanted.  A prefix count
+// then closes up ids and masses.  T is the power of two from 128 to 1024 that
+// covers the table's columns: a table of 90 blocks is done by 4 warps, whose
+// barriers are cheap, and every pass over its keys is one step; the first
+// kHeld steps' keys stay in registers.
+template <int T>
+__global__ void __launch_bounds__(T) EvictKernel(EvictArgs a) {
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
-  __shared__ int hist[256];
+  constexpr int kHeld = 2, W = T / 32;
+  __shared__ int hist[2][256];
   __shared__ int digit_of, below_digit;
-  __shared__ int warp_eq[kEvictThreads / 32], warp_leave[kEvictThreads / 32];
+  __shared__ int warp_eq[W], warp_leave[W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * a.cols;
   const int32_t length = a.lengths[blockIdx.x];
+  float held[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int64_t i = k * T + threadIdx.x;
+    held[k] = i < a.cols ? a.mass[row + i] : 0.0f;
+  }
+  for (int i = threadIdx.x; i < 512; i += T) hist[i >> 8][i & 255] = 0;
   int64_t blocks = (static_cast<int64_t>(length) + a.block - 1) / a.block;
   const bool bad = length < 0 || blocks > a.cols;
   if (bad) {
     if (threadIdx.x == 0) Raise(a.status, MLB_STATUS_BAD_LENGTH);
     blocks = a.cols;
   }
-  const int64_t gone = bad || blocks <= a.keep ? 0 : blocks - a.keep;
-  const int64_t lo = a.sink, hi = blocks - a.recent;  // candidates (when gone > 0)
+  const int gone = bad || blocks <= a.keep ? 0 : static_cast<int>(blocks - a.keep);
+  const int n = static_cast<int>(blocks), cols = static_cast<int>(a.cols);
+  const int lo = static_cast<int>(min(a.sink, blocks));
+  const int hi = static_cast<int>(blocks - min(a.recent, blocks));  // candidates, if gone > 0
   uint32_t threshold = 0;
-  int64_t equal = 0;  // keys equal to the threshold that leave
+  int equal = 0;  // keys equal to the threshold that leave
   if (gone > 0) {
-    int64_t want = gone;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = threadIdx.x; i < 256; i += kEvictThreads) hist[i] = 0;
-      __syncthreads();
-      const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int64_t i = lo + threadIdx.x; i < hi; i += kEvictThreads) {
-        const uint32_t key = MassKey(a.mass[row + i]);
-        if ((key & mask) == (threshold & mask)) atomicAdd(&hist[(key >> shift) & 255], 1);
+    int want = gone;
+#pragma unroll 1
+    for (int shift = 24, turn = 0; shift >= 0; shift -= 8, turn ^= 1) {
+      __syncthreads();  // this turn's counters are zero, the last digit is known
+      if (shift != 24) {
+        threshold |= static_cast<uint32_t>(digit_of) << (shift + 8);
+        want -= below_digit;
       }
+      const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+      const auto count = [&](float m) {
+        const uint32_t key = MassKey(m);
+        if ((key & mask) == threshold) atomicAdd(&hist[turn][(key >> shift) & 255], 1);
+      };
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        const int i = k * T + threadIdx.x;
+        if (i >= lo && i < hi) count(held[k]);
+      }
+      for (int i = kHeld * T + threadIdx.x; i < hi; i += T)
+        if (i >= lo) count(a.mass[row + i]);
       __syncthreads();
       if (warp == 0) {  // the digit at which the count reaches want
         int each[8], sum = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += each[j] = hist[8 * lane + j];
+        for (int j = 0; j < 8; ++j) {
+          sum += each[j] = hist[turn][8 * lane + j];
+          hist[turn][8 * lane + j] = 0;  // for the turn after next
+        }
         int upto = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -482,29 +508,27 @@ __global__ void __launch_bounds__(kEvictThreads) EvictKernel(EvictArgs a) {
           }
         }
       }
-      __syncthreads();
-      threshold |= static_cast<uint32_t>(digit_of) << shift;
-      want -= below_digit;
     }
-    equal = want;
+    __syncthreads();
+    threshold |= static_cast<uint32_t>(digit_of);
+    equal = want - below_digit;
   }
-  // close up, kEvictThreads places at a time: a place is read before any
-  // place at or before it is written, so outputs may be the inputs
-  int64_t seen_eq = 0, left = 0;
-  for (int64_t base = 0; base < blocks; base += kEvictThreads) {
-    const int64_t i = base + threadIdx.x;
-    const bool in = i < blocks;
+  // close up, T places at a time: a place is read before any place at or
+  // before it is written, so outputs may be the inputs
+  int seen_eq = 0, left = 0;
+  for (int base = 0; base < n; base += T) {
+    const int i = base + threadIdx.x;
+    const bool in = i < n;
     const int32_t id = in ? a.table[row + i] : -1;
-    const float m = in ? a.mass[row + i] : 0.0f;
+    const float m = in ? (base == 0 ? held[0] : base == T ? held[1] : a.mass[row + i]) : 0.0f;
     const bool open = gone > 0 && i >= lo && i < hi;
     const uint32_t key = MassKey(m);
     const bool eq = open && key == threshold;
     const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
     if (lane == 0) warp_eq[warp] = __popc(eqs);
     __syncthreads();
-    int64_t my_eq = seen_eq + __popc(eqs & ((1u << lane) - 1));
-#pragma unroll 4
-    for (int w = 0; w < kEvictThreads / 32; ++w) {
+    int my_eq = seen_eq + __popc(eqs & ((1u << lane) - 1));
+    for (int w = 0; w < W; ++w) {
       if (w < warp) my_eq += warp_eq[w];
       seen_eq += warp_eq[w];
     }
@@ -512,9 +536,8 @@ __global__ void __launch_bounds__(kEvictThreads) EvictKernel(EvictArgs a) {
     const uint32_t leave = __ballot_sync(0xffffffffu, leaves);
     if (lane == 0) warp_leave[warp] = __popc(leave);
     __syncthreads();
-    int64_t my_left = left + __popc(leave & ((1u << lane) - 1));
-#pragma unroll 4
-    for (int w = 0; w < kEvictThreads / 32; ++w) {
+    int my_left = left + __popc(leave & ((1u << lane) - 1));
+    for (int w = 0; w < W; ++w) {
       if (w < warp) my_left += warp_leave[w];
       left += warp_leave[w];
     }
@@ -523,16 +546,16 @@ __global__ void __launch_bounds__(kEvictThreads) EvictKernel(EvictArgs a) {
       a.table_out[row + i - my_left] = id;
       a.mass_out[row + i - my_left] = m;
     }
-    __syncthreads();  // the counters are read before they are filled again
+    if (base + T < n) __syncthreads();  // the counters are read before they are filled again
   }
   if (!bad)
-    for (int64_t i = blocks - left + threadIdx.x; i < a.cols; i += kEvictThreads) {
+    for (int i = n - left + threadIdx.x; i < cols; i += T) {
       a.table_out[row + i] = -1;
       a.mass_out[row + i] = 0.0f;
     }
   if (a.freed != nullptr)
-    for (int64_t i = left + threadIdx.x; i < a.cols; i += kEvictThreads) a.freed[row + i] = -1;
-  if (threadIdx.x == 0) a.lengths_out[blockIdx.x] = length - static_cast<int32_t>(left) * a.block;
+    for (int i = left + threadIdx.x; i < cols; i += T) a.freed[row + i] = -1;
+  if (threadIdx.x == 0) a.lengths_out[blockIdx.x] = length - left * a.block;
 }
 
 }  // namespace
@@ -619,6 +642,10 @@ extern "C" int mlb_kv8_evict(const int32_t* table, int64_t table_cols, const int
     return Fail(MLB_ERR_ARG, "mlb_kv8_evict: null pointer");
   const EvictArgs a{table, lengths,    mass,        table_out,   lengths_out,   mass_out, freed,
                     table_cols, keep_blocks, sink_blocks, recent_blocks, block_tokens, status};
-  Launch(EvictKernel, static_cast<unsigned>(n_seqs), kEvictThreads, 0, AsStream(stream), a);
+  const unsigned grid = static_cast<unsigned>(n_seqs);
+  if (table_cols <= 128) Launch(EvictKernel<128>, grid, 128, 0, AsStream(stream), a);
+  else if (table_cols <= 256) Launch(EvictKernel<256>, grid, 256, 0, AsStream(stream), a);
+  else if (table_cols <= 512) Launch(EvictKernel<512>, grid, 512, 0, AsStream(stream), a);
+  else Launch(EvictKernel<1024>, grid, 1024, 0, AsStream(stream), a);
   return CheckLaunch("mlb_kv8_evict");
 }
