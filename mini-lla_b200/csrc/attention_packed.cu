@@ -52,19 +52,34 @@ __device__ __forceinline__ bool PkRange(const PkArgs& a, int i, PkSeq& s) {
          s.k1 <= a.k_rows;
 }
 
-// Any head size up to 256 and any alignment of the sequences: CTA = (query
-// row, kv head), 4 warps share the row's keys, each with an online softmax
-// for the G heads of the group; the warps' states are merged at the end.
+// 2^x; results below fp32's normal range are 0.
+__device__ __forceinline__ float PtExp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// On the CUDA cores, any head size up to 256: CTA = (query row, kv head), 4
+// warps share the row's keys, 32 at a step.  A lane scores one key against
+// the G heads of the group (q broadcast from shared memory, the key's row in
+// 16-byte pieces, all under way together), the online softmax runs over the
+// lanes, and then the lanes take the dimensions of the 32 values.  The warps'
+// states are merged at the end.
 template <int G, int NV>
 __global__ void __launch_bounds__(kPkWarps * 32) PkRowKernel(PkArgs a) {
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
+  __shared__ float4 qs[G][32 * NV];
+  __shared__ float ps[kPkWarps][32][G];
   __shared__ float sm_m[kPkWarps][G];
   __shared__ float sm_l[kPkWarps][G];
   __shared__ float4 sm_acc[kPkWarps][G][32 * NV];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x;
   const int g = blockIdx.y, hd4 = a.hd >> 2;
+  const int64_t q_at = (row * a.n_heads + static_cast<int64_t>(g) * G) * hd4;
+  for (int i = threadIdx.x; i < G * hd4; i += kPkWarps * 32)
+    qs[i / hd4][i % hd4] = reinterpret_cast<const float4*>(a.q)[q_at + i];
   // the sequence that holds the row: its ranges, or none
   PkSeq s{};
   bool have = false;
@@ -90,10 +105,9 @@ __global__ void __launch_bounds__(kPkWarps * 32) PkRowKernel(PkArgs a) {
     if (have && row != 0) break;  // row 0 looks at every sequence's ranges
   }
   if (!have) return;
+  __syncthreads();
   const int64_t visible = (s.k1 - s.k0) - (s.q1 - row) + 1;  // keys the row sees
-  const int64_t q_at = (row * a.n_heads + static_cast<int64_t>(g) * G) * hd4;
-  const float4* q4 = reinterpret_cast<const float4*>(a.q) + q_at;
-  float4 q[G][NV];
+  const float scale = a.scale * 1.4426950408889634f;
   float m[G], l[G];
   float4 acc[G][NV];
 #pragma unroll
@@ -101,53 +115,70 @@ __global__ void __launch_bounds__(kPkWarps * 32) PkRowKernel(PkArgs a) {
     m[h] = -INFINITY;
     l[h] = 0.0f;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = lane + 32 * v;
-      q[h][v] = i < hd4 ? q4[h * hd4 + i] : make_float4(0.f, 0.f, 0.f, 0.f);
-      acc[h][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+    for (int v = 0; v < NV; ++v) acc[h][v] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const int64_t stride4 = static_cast<int64_t>(a.kv_heads) * hd4;
   const float4* k4 = reinterpret_cast<const float4*>(a.k) + s.k0 * stride4 + g * hd4;
   const float4* v4 = reinterpret_cast<const float4*>(a.v) + s.k0 * stride4 + g * hd4;
-  for (int64_t t = warp; t < visible; t += kPkWarps) {
-    float4 kk[NV], vv[NV];
+  for (int64_t base = 32 * warp; base < visible; base += 32 * kPkWarps) {
+    const int n = visible - base < 32 ? static_cast<int>(visible - base) : 32;
+    const float4* key = k4 + (base + (lane < n ? lane : n - 1)) * stride4;
+    float dot[G];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = lane + 32 * v;
-      kk[v] = i < hd4 ? k4[t * stride4 + i] : make_float4(0.f, 0.f, 0.f, 0.f);
-      vv[v] = i < hd4 ? v4[t * stride4 + i] : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int h = 0; h < G; ++h) dot[h] = 0.0f;
+#pragma unroll 8
+    for (int j = 0; j < hd4; ++j) {
+      const float4 x = key[j];
+#pragma unroll
+      for (int h = 0; h < G; ++h) {
+        const float4 q = qs[h][j];
+        dot[h] = fmaf(q.x, x.x, fmaf(q.y, x.y, fmaf(q.z, x.z, fmaf(q.w, x.w, dot[h]))));
+      }
     }
 #pragma unroll
     for (int h = 0; h < G; ++h) {
-      float dot = 0.0f;
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        dot = fmaf(q[h][v].x, kk[v].x, dot);
-        dot = fmaf(q[h][v].y, kk[v].y, dot);
-        dot = fmaf(q[h][v].z, kk[v].z, dot);
-        dot = fmaf(q[h][v].w, kk[v].w, dot);
-      }
-      const float score = WarpSum(dot) * a.scale;
-      const float m_new = fmaxf(m[h], score);
-      const float alpha = m[h] == -INFINITY ? 0.0f : expf(m[h] - m_new);
-      const float p = expf(score - m_new);
-      l[h] = fmaf(l[h], alpha, p);
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        acc[h][v].x = fmaf(acc[h][v].x, alpha, p * vv[v].x);
-        acc[h][v].y = fmaf(acc[h][v].y, alpha, p * vv[v].y);
-        acc[h][v].z = fmaf(acc[h][v].z, alpha, p * vv[v].z);
-        acc[h][v].w = fmaf(acc[h][v].w, alpha, p * vv[v].w);
-      }
+      const float x = lane < n ? dot[h] * scale : -INFINITY;
+      const float m_new = fmaxf(m[h], WarpMax(x));
+      const float alpha = m[h] == m_new ? 1.0f : PtExp2(m[h] - m_new);
+      const float p = lane < n ? PtExp2(x - m_new) : 0.0f;
+      l[h] = fmaf(l[h], alpha, p);  // this lane's keys
       m[h] = m_new;
+      ps[warp][lane][h] = p;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        acc[h][v].x *= alpha;
+        acc[h][v].y *= alpha;
+        acc[h][v].z *= alpha;
+        acc[h][v].w *= alpha;
+      }
     }
+    __syncwarp();
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int d = lane + 32 * v;
+      if (d >= hd4) break;
+      const float4* val = v4 + base * stride4 + d;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float4 x = val[i * stride4];
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          const float p = ps[warp][i][h];
+          acc[h][v].x = fmaf(x.x, p, acc[h][v].x);
+          acc[h][v].y = fmaf(x.y, p, acc[h][v].y);
+          acc[h][v].z = fmaf(x.z, p, acc[h][v].z);
+          acc[h][v].w = fmaf(x.w, p, acc[h][v].w);
+        }
+      }
+    }
+    __syncwarp();  // the weights are read before they are written again
   }
 #pragma unroll
   for (int h = 0; h < G; ++h) {
+    const float sum = WarpSum(l[h]);
     if (lane == 0) {
       sm_m[warp][h] = m[h];
-      sm_l[warp][h] = l[h];
+      sm_l[warp][h] = sum;
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) sm_acc[warp][h][lane + 32 * v] = acc[h][v];
@@ -159,7 +190,7 @@ __global__ void __launch_bounds__(kPkWarps * 32) PkRowKernel(PkArgs a) {
     float f[kPkWarps];
 #pragma unroll
     for (int w = 0; w < kPkWarps; ++w) {
-      f[w] = sm_m[w][h] == -INFINITY ? 0.0f : expf(sm_m[w][h] - mm);
+      f[w] = sm_m[w][h] == -INFINITY ? 0.0f : PtExp2(sm_m[w][h] - mm);
       // a warp whose scores are NaN keeps them visible
       if (sm_l[w][h] != sm_l[w][h]) f[w] = NAN;
       ll = fmaf(sm_l[w][h], f[w], ll);
@@ -303,12 +334,6 @@ __device__ __forceinline__ float PtUp(float top, float& down) {
   e = top == 0.0f ? 14 : max(e, -100);
   down = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
   return __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
-}
-
-__device__ __forceinline__ float PtExp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Two values -> their high fp16 pieces and what is left, again in fp16.
