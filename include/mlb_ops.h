@@ -351,8 +351,9 @@ int mlb_attention_rows_f32(const float* q, const float* keys,
 
 /*
  * Kernel choice of mlb_attention_rows_f32 for prompt chunks (two rows or
- * more): 0 = automatic (the default: the tensor cores from 512 rows),
- * 1 = always the CUDA-core
+ * more) and of mlb_attention_packed_f32: 0 = automatic (the default: the
+ * tensor cores from 512 rows; for packed sequences where their sizes make
+ * them the faster), 1 = always the CUDA-core
  * kernels, 2 = the tensor cores wherever the shape allows (group 1 .. 8,
  * head_dim 64 or 128, 16-byte aligned tensors).  Process-wide; for benchmarks
  * and tests.  Returns MLB_OK, or MLB_ERR_ARG for another value;
@@ -422,9 +423,13 @@ int64_t mlb_attention_packed_scratch_floats(int64_t q_rows, int64_t k_rows,
  *   head_dim]; group n_heads / n_kv_heads <= 8; head_dim % 4 == 0, <= 256;
  *   q, k, v, out 16-byte aligned; q_rows, k_rows, n_seqs < 2^31 / 8.
  *   scratch: caller-owned device memory of at least
- *   mlb_attention_packed_scratch_floats(...) floats, 16-byte aligned.
+ *   mlb_attention_packed_scratch_floats(...) floats, 16-byte aligned (0 where
+ *   the CUDA cores take the call; mlb_set_attention_path changes the need).
  * Within 1e-5 * sum_t w_t |v_t| of the exact result for scores of ordinary
- * spread.  out must not overlap q, k or v.
+ * spread.  out must not overlap q, k or v.  Keys, values and rows that a row
+ * does not see do not reach it, whatever they hold; a row that sees an Inf or
+ * NaN gets NaN in the outputs it reaches (also where a weight of 0 would hide
+ * it).
  */
 int mlb_attention_packed_f32(const float* q, const float* k, const float* v,
                              float* out, const int32_t* q_offsets,

@@ -742,9 +742,9 @@ def set_gemv_path(path: int) -> int:
 
 
 def set_attention_path(path: int) -> int:
-    """Kernel choice of attention_rows() for prompt chunks: 0 automatic, 1
-    CUDA-core kernels, 2 tensor cores wherever the shape allows.  Returns the
-    previous setting."""
+    """Kernel choice of attention_rows() for prompt chunks and of
+    attention_packed(): 0 automatic, 1 CUDA-core kernels, 2 tensor cores
+    wherever the shape allows.  Returns the previous setting."""
     previous = load().mlb_attention_path()
     _check(load().mlb_set_attention_path(int(path)), "set_attention_path")
     return previous

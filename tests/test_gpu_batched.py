@@ -98,6 +98,14 @@ def packed_inputs(rng, lens, keys, nh, nkv, hd, spread=1.0):
     return q, k, v, qo, ko
 
 
+@pytest.fixture(params=[1, 2], ids=["cuda cores", "tensor cores"])
+def path(request):
+    """Both kernels (head sizes other than 64 and 128 have one)."""
+    previous = mlb.set_attention_path(request.param)
+    yield request.param
+    mlb.set_attention_path(previous)
+
+
 PACKED = [
     # heads, kv heads, head size, query rows, keys (None: the same)
     (4, 2, 64, [1], None),
@@ -119,7 +127,7 @@ PACKED = [
 
 
 @pytest.mark.parametrize("nh,nkv,hd,lens,keys", PACKED)
-def test_packed_attention(cuda, nh, nkv, hd, lens, keys):
+def test_packed_attention(cuda, path, nh, nkv, hd, lens, keys):
     rng = np.random.default_rng(nh * 100 + hd)
     q, k, v, qo, ko = packed_inputs(rng, lens, lens if keys is None else keys, nh, nkv, hd)
     want, tol = packed_reference(q, k, v, qo, ko)
@@ -131,7 +139,7 @@ def test_packed_attention(cuda, nh, nkv, hd, lens, keys):
 
 @pytest.mark.parametrize("spread", [0.0, 6.0, 12.0])
 @pytest.mark.parametrize("scale", [1.0, 1e-18, 1e12])
-def test_packed_attention_wide_values(cuda, spread, scale):
+def test_packed_attention_wide_values(cuda, path, spread, scale):
     """Peaked softmax rows, and values far from 1 (q small where k is large:
     the scores stay, the pieces' scales do not)."""
     rng = np.random.default_rng(int(spread) + 5)
@@ -144,7 +152,7 @@ def test_packed_attention_wide_values(cuda, spread, scale):
     check(got.cpu().numpy(), want, tol)
 
 
-def test_packed_attention_values_of_different_size(cuda):
+def test_packed_attention_values_of_different_size(cuda, path):
     """Neighbouring keys whose values differ by powers of ten: an output's
     tolerance follows the weights, so no key may be lost beside a larger one."""
     rng = np.random.default_rng(3)
@@ -158,7 +166,7 @@ def test_packed_attention_values_of_different_size(cuda):
 
 
 @pytest.mark.parametrize("hd", [64, 128, 96])
-def test_packed_attention_does_not_look_past_its_keys(cuda, hd):
+def test_packed_attention_does_not_look_past_its_keys(cuda, path, hd):
     """NaN and Inf in later keys, in other sequences' keys and in rows between
     the sequences reach no row that does not see them; rows outside every
     sequence stay as they were."""
@@ -188,7 +196,7 @@ def test_packed_attention_does_not_look_past_its_keys(cuda, hd):
 
 @pytest.mark.parametrize("nh,nkv,hd", [(16, 8, 128), (8, 8, 64), (14, 2, 64)])
 @pytest.mark.parametrize("most,context", [(40, 0), (300, 0), (130, 300)])
-def test_packed_attention_many_tiles(cuda, nh, nkv, hd, most, context):
+def test_packed_attention_many_tiles(cuda, path, nh, nkv, hd, most, context):
     """More query tiles than the GPU has multiprocessors, most of them of one
     to three key blocks: each CTA goes through several, one after another."""
     rng = np.random.default_rng(most + nh)
@@ -203,7 +211,7 @@ def test_packed_attention_many_tiles(cuda, nh, nkv, hd, most, context):
     assert mlb.wait_timeouts() == 0
 
 
-def test_packed_attention_equals_rows_of_one_sequence(cuda):
+def test_packed_attention_equals_rows_of_one_sequence(cuda, path):
     """One sequence is mlb_attention_rows_f32 over its cache."""
     rng = np.random.default_rng(9)
     q, k, v, qo, ko = packed_inputs(rng, [160], [400], 16, 4, 128)
@@ -214,12 +222,25 @@ def test_packed_attention_equals_rows_of_one_sequence(cuda):
     check(got, one.astype(np.float64), 2 * tol)
 
 
+@pytest.mark.parametrize("nh,nkv,hd,seqs,longest", [(14, 2, 64, 3, 40), (32, 8, 128, 5, 400)])
+def test_packed_attention_chooses_its_kernel(cuda, nh, nkv, hd, seqs, longest):
+    """The automatic choice, on sizes where it falls on either side."""
+    rng = np.random.default_rng(longest)
+    lens = rng.integers(1, longest, seqs).tolist()
+    q, k, v, qo, ko = packed_inputs(rng, lens, lens, nh, nkv, hd)
+    want, tol = packed_reference(q, k, v, qo, ko)
+    got = mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(qo, cuda))
+    check(got.cpu().numpy(), want, tol)
+    need = mlb.load().mlb_attention_packed_scratch_floats(len(q), len(k), seqs, nh, nkv, hd)
+    assert (need == 0) == (longest == 40)
+
+
 @pytest.mark.parametrize("qo,ko", [
     ([0, 50, 40, 60], [0, 50, 60, 60]),      # runs backwards
     ([0, 20, 70, 60], [0, 20, 60, 60]),      # leaves the rows
     ([-4, 20, 40, 60], [0, 20, 40, 60]),
     ([0, 20, 40, 60], [0, 20, 90, 60])])     # leaves the keys
-def test_packed_attention_bad_ranges(cuda, qo, ko):
+def test_packed_attention_bad_ranges(cuda, path, qo, ko):
     """Sequences with a bad range are left out and reported; the others are
     computed.  (Ranges that run backwards let two sequences claim a row: what
     such a row gets is not said.)"""
@@ -686,7 +707,7 @@ def test_evict_bad_length(cuda):
 
 # --- together ---------------------------------------------------------------------------------
 
-def test_serving_loop(cuda):
+def test_serving_loop(cuda, path):
     """Prompts of several sequences, then decode steps with collected weights,
     an eviction and more steps: as a server would call them, against the same
     run in 64 bits on a cache of the same codes."""
@@ -755,7 +776,7 @@ def test_serving_loop(cuda):
     assert mlb.status_check(status) == 0
 
 
-def test_batched_calls_on_a_stream_and_in_a_graph(cuda):
+def test_batched_calls_on_a_stream_and_in_a_graph(cuda, path):
     """Another stream than the current one; and a decode step captured once and
     replayed with new inputs in the same buffers, beside a second graph."""
     import torch
