@@ -13,6 +13,7 @@ IndexError (std::out_of_range), a CUDA failure raises RuntimeError
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from collections import namedtuple
 from ctypes import c_float, c_int, c_int64, c_void_p
@@ -513,18 +514,25 @@ class _On:
             g.__exit__(*exc)
 
 
-def _like(t, dtype, device, op, name, shape=None):
-    if t.dtype is not dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{op}: {name} must be a contiguous {dtype} tensor on {device}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{op}: {name} must be {list(shape)}, got {list(t.shape)}")
+# The entries below look at their arguments in one expression (a decode step's
+# calls are a few microseconds each); where it fails, _refuse finds the words.
+
+def _refuse(op, device, *tensors):
+    """Raises for the first of (name, tensor, dtype, shape) that is not a
+    contiguous tensor of that type (and shape, None: any) on `device`."""
+    _require(device >= 0, op, f"{tensors[0][0]} must be a CUDA tensor")
+    for name, t, dtype, shape in tensors:
+        if t is None:
+            continue
+        if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+            raise ValueError(f"{op}: {name} must be a contiguous {dtype} tensor on cuda:{device}")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{op}: {name} must be {list(shape)}, got {list(t.shape)}")
+    raise ValueError(f"{op}: bad arguments")
 
 
-def _status_word(status, device, op):
-    import torch
-    if status is not None:
-        _require(status.dtype == torch.int32 and status.device == device and
-                 status.numel() >= 1, op, f"status must be int32 on {device}")
+def _plain(t, dtype, device):
+    return t.dtype is dtype and t.get_device() == device and t.is_contiguous()
 
 
 def attention_packed(q, k, v, q_offsets, k_offsets=None, out=None, scratch=None, status=None,
@@ -537,39 +545,41 @@ def attention_packed(q, k, v, q_offsets, k_offsets=None, out=None, scratch=None,
     are not written."""
     import torch
     op = "attention_packed"
-    device = q.device
-    _require(q.is_cuda and q.dim() == 3 and k.dim() == 3, op,
+    f32, i32 = torch.float32, torch.int32
+    device = q.get_device()
+    _require(q.dim() == 3 and k.dim() == 3, op,
              "q must be [rows, heads, head_dim], k [keys, kv_heads, head_dim]")
-    _like(q, torch.float32, device, op, "q")
-    _like(k, torch.float32, device, op, "k")
-    _like(v, torch.float32, device, op, "v", k.shape)
     rows, nh, hd = q.shape
     keys, kvh, khd = k.shape
     _require(khd == hd, op, "q and k differ in head_dim")
-    _require(q_offsets.dim() == 1 and q_offsets.numel() >= 1, op, "q_offsets must be [n_seqs + 1]")
-    _like(q_offsets, torch.int32, device, op, "q_offsets")
     if k_offsets is None:
         _require(keys == rows, op, "k_offsets is needed when k has other rows than q")
         k_offsets = q_offsets
-    else:
-        _like(k_offsets, torch.int32, device, op, "k_offsets", q_offsets.shape)
     n_seqs = q_offsets.numel() - 1
-    _status_word(status, device, op)
-    if out is not None:
-        _like(out, torch.float32, device, op, "out", q.shape)
+    if not (device >= 0 and _plain(q, f32, device) and _plain(k, f32, device) and
+            _plain(v, f32, device) and v.shape == k.shape and q_offsets.dim() == 1 and
+            n_seqs >= 0 and _plain(q_offsets, i32, device) and
+            _plain(k_offsets, i32, device) and k_offsets.shape == q_offsets.shape and
+            (out is None or (_plain(out, f32, device) and out.shape == q.shape)) and
+            (scratch is None or _plain(scratch, f32, device)) and
+            (status is None or _plain(status, i32, device))):
+        _refuse(op, device, ("q", q, f32, None), ("k", k, f32, None), ("v", v, f32, k.shape),
+                ("q_offsets", q_offsets, i32, (max(n_seqs, 0) + 1,)),
+                ("k_offsets", k_offsets, i32, q_offsets.shape), ("out", out, f32, q.shape),
+                ("scratch", scratch, f32, None), ("status", status, i32, None))
     lib = load()
     with _On(q, stream) as on:
         if out is None:
             out = torch.empty_like(q)
         if scratch is None:
             need = lib.mlb_attention_packed_scratch_floats(rows, keys, n_seqs, nh, kvh, hd)
-            scratch = torch.empty(max(need, 1), dtype=torch.float32, device=device)
-        else:
-            _like(scratch, torch.float32, device, op, "scratch")
+            scratch = torch.empty(need, dtype=f32, device=q.device) if need > 0 else None
         _check(lib.mlb_attention_packed_f32(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_offsets.data_ptr(),
-            k_offsets.data_ptr(), n_seqs, rows, keys, nh, kvh, hd, scratch.data_ptr(),
-            scratch.numel(), _ptr(status), on), op)
+            k_offsets.data_ptr(), n_seqs, rows, keys, nh, kvh, hd,
+            None if scratch is None else scratch.data_ptr(),
+            0 if scratch is None else scratch.numel(), None if status is None else
+            status.data_ptr(), on), op)
     return out
 
 
@@ -591,24 +601,26 @@ def kv8_cache(n_blocks: int, n_kv_heads: int, block_tokens: int, head_dim: int, 
     return Kv8Cache(*codes, *scales)
 
 
-def _pool(cache, device, op):
-    """(n_blocks, kv_heads, block_tokens, head_dim) of a pool."""
+def _pool(cache, table, op):
+    """What the cache's entries share: (k_codes, v_codes, k_scales, v_scales),
+    (n_blocks, kv_heads, block_tokens, head_dim), (n_seqs, columns), the
+    device."""
     import torch
-    k = cache.k_codes
-    _require(k.is_cuda and k.dim() == 4, op, "k_codes must be [blocks, kv_heads, block, head_dim]")
-    n, kvh, block, hd = k.shape
-    _like(k, torch.int8, device, op, "k_codes")
-    _like(cache.v_codes, torch.int8, device, op, "v_codes", (n, kvh, hd, block))
-    _like(cache.k_scales, torch.float32, device, op, "k_scales", (n, kvh))
-    _like(cache.v_scales, torch.float32, device, op, "v_scales", (n, kvh))
-    return n, kvh, block, hd
-
-
-def _table(table, device, op):
-    import torch
-    _require(table.dim() == 2, op, "table must be [n_seqs, columns]")
-    _like(table, torch.int32, device, op, "table")
-    return table.shape
+    i8, f32, i32 = torch.int8, torch.float32, torch.int32
+    kc, vc, ks, vs = cache
+    device = kc.get_device()
+    if kc.dim() != 4 or table.dim() != 2:
+        raise ValueError(f"{op}: k_codes must be [blocks, kv_heads, block, head_dim], table "
+                         "[n_seqs, columns]")
+    n, kvh, block, hd = sizes = kc.shape
+    if not (device >= 0 and _plain(kc, i8, device) and _plain(vc, i8, device) and
+            vc.shape == (n, kvh, hd, block) and _plain(ks, f32, device) and
+            ks.shape == (n, kvh) and _plain(vs, f32, device) and vs.shape == (n, kvh) and
+            _plain(table, i32, device)):
+        _refuse(op, device, ("k_codes", kc, i8, None), ("v_codes", vc, i8, (n, kvh, hd, block)),
+                ("k_scales", ks, f32, (n, kvh)), ("v_scales", vs, f32, (n, kvh)),
+                ("table", table, i32, None))
+    return (kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()), sizes, table.shape, device
 
 
 def kv8_write(cache, table, k, v, offsets, positions, status=None, stream=None):
@@ -617,21 +629,21 @@ def kv8_write(cache, table, k, v, offsets, positions, status=None, stream=None):
     positions[i] on (int32 [n_seqs + 1] and [n_seqs])."""
     import torch
     op = "kv8_write"
-    device = cache.k_codes.device
-    n_blocks, kvh, block, hd = _pool(cache, device, op)
-    n_seqs, cols = _table(table, device, op)
-    _require(k.dim() == 3 and k.shape[1:] == (kvh, hd), op, "k must be [rows, kv_heads, head_dim]")
-    _like(k, torch.float32, device, op, "k")
-    _like(v, torch.float32, device, op, "v", k.shape)
-    _like(offsets, torch.int32, device, op, "offsets", (n_seqs + 1,))
-    _like(positions, torch.int32, device, op, "positions", (n_seqs,))
-    _status_word(status, device, op)
+    f32, i32 = torch.float32, torch.int32
+    pool, (n_blocks, kvh, block, hd), (n_seqs, cols), device = _pool(cache, table, op)
+    rows = k.shape[0] if k.dim() == 3 else 0
+    if not (k.shape == (rows, kvh, hd) and _plain(k, f32, device) and _plain(v, f32, device) and
+            v.shape == k.shape and _plain(offsets, i32, device) and
+            offsets.shape == (n_seqs + 1,) and _plain(positions, i32, device) and
+            positions.shape == (n_seqs,) and (status is None or _plain(status, i32, device))):
+        _refuse(op, device, ("k", k, f32, (rows, kvh, hd)), ("v", v, f32, k.shape),
+                ("offsets", offsets, i32, (n_seqs + 1,)),
+                ("positions", positions, i32, (n_seqs,)), ("status", status, i32, None))
     with _On(k, stream) as on:
         _check(load().mlb_kv8_write_f32(
-            cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scales.data_ptr(),
-            cache.v_scales.data_ptr(), n_blocks, block, table.data_ptr(), cols, n_seqs,
-            k.data_ptr(), v.data_ptr(), offsets.data_ptr(), positions.data_ptr(), k.shape[0],
-            kvh, hd, _ptr(status), on), op)
+            *pool, n_blocks, block, table.data_ptr(), cols, n_seqs, k.data_ptr(), v.data_ptr(),
+            offsets.data_ptr(), positions.data_ptr(), rows, kvh, hd,
+            None if status is None else status.data_ptr(), on), op)
 
 
 def kv8_read(cache, table, offsets, positions, rows: int, status=None, stream=None):
@@ -640,21 +652,28 @@ def kv8_read(cache, table, offsets, positions, rows: int, status=None, stream=No
     written."""
     import torch
     op = "kv8_read"
-    device = cache.k_codes.device
-    n_blocks, kvh, block, hd = _pool(cache, device, op)
-    n_seqs, cols = _table(table, device, op)
-    _like(offsets, torch.int32, device, op, "offsets", (n_seqs + 1,))
-    _like(positions, torch.int32, device, op, "positions", (n_seqs,))
-    _status_word(status, device, op)
+    f32, i32 = torch.float32, torch.int32
+    pool, (n_blocks, kvh, block, hd), (n_seqs, cols), device = _pool(cache, table, op)
+    if not (_plain(offsets, i32, device) and offsets.shape == (n_seqs + 1,) and
+            _plain(positions, i32, device) and positions.shape == (n_seqs,) and
+            (status is None or _plain(status, i32, device))):
+        _refuse(op, device, ("offsets", offsets, i32, (n_seqs + 1,)),
+                ("positions", positions, i32, (n_seqs,)), ("status", status, i32, None))
     with _On(table, stream) as on:
-        k = torch.empty((rows, kvh, hd), dtype=torch.float32, device=device)
-        v = torch.empty((rows, kvh, hd), dtype=torch.float32, device=device)
+        k = torch.empty((rows, kvh, hd), dtype=f32, device=table.device)
+        v = torch.empty_like(k)
         _check(load().mlb_kv8_read_f32(
-            cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scales.data_ptr(),
-            cache.v_scales.data_ptr(), n_blocks, block, table.data_ptr(), cols, n_seqs,
-            k.data_ptr(), v.data_ptr(), offsets.data_ptr(), positions.data_ptr(), rows, kvh, hd,
-            _ptr(status), on), op)
+            *pool, n_blocks, block, table.data_ptr(), cols, n_seqs, k.data_ptr(), v.data_ptr(),
+            offsets.data_ptr(), positions.data_ptr(), rows, kvh, hd,
+            None if status is None else status.data_ptr(), on), op)
     return k, v
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_kv8_scratch(device, n_seqs, cols, block, nh, kvh, hd, with_mass):
+    """Floats of scratch; they go by the sizes and the device alone."""
+    return max(int(load().mlb_attention_kv8_scratch_floats(n_seqs, cols, block, nh, kvh, hd,
+                                                           with_mass)), 1)
 
 
 def attention_kv8(q, cache, table, lengths, out=None, mass_in=None, mass_out=None, scratch=None,
@@ -665,36 +684,34 @@ def attention_kv8(q, cache, table, lengths, out=None, mass_in=None, mass_out=Non
     collected, added to mass_in (None: zeros; may be mass_out)."""
     import torch
     op = "attention_kv8"
-    device = q.device
-    n_blocks, kvh, block, hd = _pool(cache, device, op)
-    n_seqs, cols = _table(table, device, op)
-    _require(q.dim() == 3 and q.shape[0] == n_seqs and q.shape[2] == hd, op,
-             "q must be [n_seqs, heads, head_dim]")
-    _like(q, torch.float32, device, op, "q")
-    _like(lengths, torch.int32, device, op, "lengths", (n_seqs,))
-    nh = q.shape[1]
-    for m, name in ((mass_in, "mass_in"), (mass_out, "mass_out")):
-        if m is not None:
-            _like(m, torch.float32, device, op, name, table.shape)
-    _status_word(status, device, op)
-    if out is not None:
-        _like(out, torch.float32, device, op, "out", q.shape)
-    lib = load()
+    f32, i32 = torch.float32, torch.int32
+    pool, (n_blocks, kvh, block, hd), (n_seqs, cols), device = _pool(cache, table, op)
+    nh = q.shape[1] if q.dim() == 3 else 0
+    if not (q.shape == (n_seqs, nh, hd) and _plain(q, f32, device) and
+            _plain(lengths, i32, device) and lengths.shape == (n_seqs,) and
+            (mass_in is None or (_plain(mass_in, f32, device) and
+                                 mass_in.shape == table.shape)) and
+            (mass_out is None or (_plain(mass_out, f32, device) and
+                                  mass_out.shape == table.shape)) and
+            (out is None or (_plain(out, f32, device) and out.shape == q.shape)) and
+            (scratch is None or _plain(scratch, f32, device)) and
+            (status is None or _plain(status, i32, device))):
+        _refuse(op, device, ("q", q, f32, (n_seqs, nh, hd)), ("lengths", lengths, i32, (n_seqs,)),
+                ("mass_in", mass_in, f32, table.shape), ("mass_out", mass_out, f32, table.shape),
+                ("out", out, f32, q.shape), ("scratch", scratch, f32, None),
+                ("status", status, i32, None))
     with _On(q, stream) as on:
         if out is None:
             out = torch.empty_like(q)
         if scratch is None:
-            need = lib.mlb_attention_kv8_scratch_floats(n_seqs, cols, block, nh, kvh, hd,
-                                                        0 if mass_out is None else 1)
-            scratch = torch.empty(max(need, 1), dtype=torch.float32, device=device)
-        else:
-            _like(scratch, torch.float32, device, op, "scratch")
-        _check(lib.mlb_attention_kv8_f32(
-            q.data_ptr(), cache.k_codes.data_ptr(), cache.v_codes.data_ptr(),
-            cache.k_scales.data_ptr(), cache.v_scales.data_ptr(), n_blocks, block,
-            table.data_ptr(), cols, lengths.data_ptr(), n_seqs, nh, kvh, hd, out.data_ptr(),
-            _ptr(mass_in), _ptr(mass_out), scratch.data_ptr(), scratch.numel(), _ptr(status),
-            on), op)
+            scratch = torch.empty(_attention_kv8_scratch(device, n_seqs, cols, block, nh, kvh, hd,
+                                                         0 if mass_out is None else 1),
+                                  dtype=f32, device=q.device)
+        _check(load().mlb_attention_kv8_f32(
+            q.data_ptr(), *pool, n_blocks, block, table.data_ptr(), cols, lengths.data_ptr(),
+            n_seqs, nh, kvh, hd, out.data_ptr(), None if mass_in is None else mass_in.data_ptr(),
+            None if mass_out is None else mass_out.data_ptr(), scratch.data_ptr(),
+            scratch.numel(), None if status is None else status.data_ptr(), on), op)
     return out
 
 
@@ -706,19 +723,23 @@ def kv8_evict(table, lengths, mass, block_tokens: int, keep_blocks: int, sink_bl
     the ids of the blocks that left, -1 behind them."""
     import torch
     op = "kv8_evict"
-    device = table.device
-    _require(table.is_cuda, op, "table must be a CUDA tensor")
-    n_seqs, cols = _table(table, device, op)
-    _like(lengths, torch.int32, device, op, "lengths", (n_seqs,))
-    _like(mass, torch.float32, device, op, "mass", table.shape)
-    _status_word(status, device, op)
+    f32, i32 = torch.float32, torch.int32
+    device = table.get_device()
+    _require(table.dim() == 2, op, "table must be [n_seqs, columns]")
+    n_seqs, cols = table.shape
+    if not (device >= 0 and _plain(table, i32, device) and _plain(lengths, i32, device) and
+            lengths.shape == (n_seqs,) and _plain(mass, f32, device) and
+            mass.shape == table.shape and (status is None or _plain(status, i32, device))):
+        _refuse(op, device, ("table", table, i32, None), ("lengths", lengths, i32, (n_seqs,)),
+                ("mass", mass, f32, table.shape), ("status", status, i32, None))
     with _On(table, stream) as on:
         table_out, freed = torch.empty_like(table), torch.empty_like(table)
         lengths_out, mass_out = torch.empty_like(lengths), torch.empty_like(mass)
         _check(load().mlb_kv8_evict(
             table.data_ptr(), cols, lengths.data_ptr(), mass.data_ptr(), n_seqs, block_tokens,
             keep_blocks, sink_blocks, recent_blocks, table_out.data_ptr(),
-            lengths_out.data_ptr(), mass_out.data_ptr(), freed.data_ptr(), _ptr(status), on), op)
+            lengths_out.data_ptr(), mass_out.data_ptr(), freed.data_ptr(),
+            None if status is None else status.data_ptr(), on), op)
     return table_out, lengths_out, mass_out, freed
 
 
