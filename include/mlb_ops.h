@@ -425,6 +425,7 @@ int64_t mlb_attention_packed_scratch_floats(int64_t q_rows, int64_t k_rows,
  *   scratch: caller-owned device memory of at least
  *   mlb_attention_packed_scratch_floats(...) floats, 16-byte aligned (0 where
  *   the CUDA cores take the call; mlb_set_attention_path changes the need).
+ *   Calls that may overlap on the GPU need scratch of their own.
  * Within 1e-5 * sum_t w_t |v_t| of the exact result for scores of ordinary
  * spread.  out must not overlap q, k or v.  Keys, values and rows that a row
  * does not see do not reach it, whatever they hold; a row that sees an Inf or
@@ -521,7 +522,8 @@ int64_t mlb_attention_kv8_scratch_floats(int64_t n_seqs, int64_t table_cols,
  * (mass_in NULL reads as zeros and may be mass_out itself; sequences with an
  * error and places behind the last block get mass_in unchanged).
  * scratch: at least mlb_attention_kv8_scratch_floats(...) floats, 16-byte
- * aligned.  Deterministic.  Queries are taken in 22 bits, the weights in 22
+ * aligned; calls that may overlap on the GPU need scratch of their own.  out
+ * overlaps neither q nor the pool.  Deterministic.  Queries are taken in 22 bits, the weights in 22
  * bits, all sums in fp32: within 1e-5 * sum_t w_t |v_t| of the exact result
  * over the cache's values for scores of ordinary spread.
  */

@@ -382,48 +382,39 @@ __device__ __forceinline__ uint32_t PtQItem(uint32_t t, uint32_t n) {
   return t + n + (n == 0 ? 0 : n - 1);
 }
 
-constexpr int kPtSplitThreads = 256;
+constexpr int kPtSplitThreads = 512;
 
-// First image of every sequence, scanned kPtSplitThreads at a time; calls
-// each(i, range, first image, blocks) for the sequences that take part.  All
-// threads of the CTA call it; each thread sees its own sequences.
+// Walks the sequences 32 at a time and calls each(i, range, first image,
+// blocks) on the lane that has sequence i; it returns whether to stop, which
+// the warp does together.  First image -1: left out.
 template <typename Each>
-__device__ int64_t PtScan(const PtArgs& a, bool report, Each each) {
-  __shared__ int64_t warp_sum[kPtSplitThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ void PtScan(const PtArgs& a, bool report, Each each) {
+  const int lane = threadIdx.x & 31;
   int64_t before = 0;
-  for (int base = 0; base < a.in.n_seqs; base += kPtSplitThreads) {
-    const int i = base + static_cast<int>(threadIdx.x);
+  for (int base = 0; base < a.in.n_seqs; base += 32) {
+    const int i = base + lane;
     PkSeq s{};
-    int64_t blocks = 0;
+    int blocks = 0;
     bool good = false;
     if (i < a.in.n_seqs) {
       good = PkRange(a.in, i, s);
       if (!good && report && a.in.status != nullptr) atomicOr(a.in.status, MLB_STATUS_BAD_LENGTH);
-      if (good) blocks = (s.k1 - s.k0 + kPtKeys - 1) / kPtKeys;
+      if (good) blocks = static_cast<int>((s.k1 - s.k0 + kPtKeys - 1) / kPtKeys);
     }
-    int64_t upto = blocks;
+    int upto = blocks;  // at most 32 * 2^28 / 128
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += up;
-    }
-    if (lane == 31) warp_sum[warp] = upto;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kPtSplitThreads / 32; ++w) {
-      if (w < warp) upto += warp_sum[w];
-      total += warp_sum[w];
     }
     // ranges that run backwards can let others overlap and claim more blocks
     // than there are: those are left out too (the status is raised already)
     const int64_t first = before + upto - blocks;
-    if (i < a.in.n_seqs) each(i, s, good && first + blocks <= a.max_blocks ? first : -1, blocks);
-    before += total;
-    __syncthreads();
+    const bool stop =
+        i < a.in.n_seqs && each(i, s, good && first + blocks <= a.max_blocks ? first : -1, blocks);
+    if (__any_sync(0xffffffffu, stop)) return;
+    before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  return before;
 }
 
 // The list of query tiles, in falling order of their key blocks (counting
@@ -434,9 +425,11 @@ __device__ void PtListTiles(const PtArgs& a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int qr = kPtVectors / a.group;
   for (int i = threadIdx.x; i < 1024; i += kPtSplitThreads) bins[i] = 0;
-  PtScan(a, true, [&](int i, const PkSeq&, int64_t first, int64_t) {
-    a.blocks[i] = static_cast<int32_t>(first);
-  });
+  if (warp == 0)
+    PtScan(a, true, [&](int i, const PkSeq&, int64_t first, int) {
+      a.blocks[i] = static_cast<int32_t>(first);
+      return false;
+    });
   __syncthreads();  // also the block's own global writes
   int shift = 0;
   while ((a.in.k_rows / kPtKeys + 1) >> shift >= 1024) ++shift;
@@ -461,10 +454,11 @@ __device__ void PtListTiles(const PtArgs& a) {
   };
   tiles([&](const PtTile&, int bin) { atomicAdd(&bins[bin], 1); });
   __syncthreads();
-  // exclusive scan: 4 bins a thread
-  int each[4], sum = 0;
+  // exclusive scan, the same number of bins a thread
+  constexpr int kPer = 1024 / kPtSplitThreads;
+  int each[kPer], sum = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) sum += each[j] = bins[4 * threadIdx.x + j];
+  for (int j = 0; j < kPer; ++j) sum += each[j] = bins[kPer * threadIdx.x + j];
   int upto = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -476,8 +470,8 @@ __device__ void PtListTiles(const PtArgs& a) {
   for (int w = 0; w < warp; ++w) upto += bin_sum[w];
   int at = upto - sum;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    bins[4 * threadIdx.x + j] = at;
+  for (int j = 0; j < kPer; ++j) {
+    bins[kPer * threadIdx.x + j] = at;
     at += each[j];
   }
   if (threadIdx.x == kPtSplitThreads - 1)
@@ -490,38 +484,40 @@ __device__ void PtListTiles(const PtArgs& a) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kPtSplitThreads) PkSplitKernel(PtArgs a) {
+__global__ void __launch_bounds__(kPtSplitThreads, 2) PkSplitKernel(PtArgs a) {
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
-  if (static_cast<int64_t>(blockIdx.x) == a.max_blocks) {
+  if (blockIdx.x == 0) {  // first, as it takes longest
     if (blockIdx.y == 0 && blockIdx.z == 0) PtListTiles(a);
     return;
   }
-  __shared__ int64_t key0_of;
-  __shared__ int keys_of;
   __shared__ float top_of[kPtSplitThreads / 32];
   __shared__ int odd_of[kPtSplitThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t image = blockIdx.x;
+  const int64_t image = blockIdx.x - 1;
   const int head = blockIdx.y;
   const bool is_v = blockIdx.z != 0;
-  if (threadIdx.x == 0) keys_of = 0;
-  __syncthreads();
-  PtScan(a, false, [&](int, const PkSeq& s, int64_t first, int64_t blocks) {
-    if (first >= 0 && image >= first && image < first + blocks) {
-      key0_of = s.k0 + (image - first) * kPtKeys;
-      keys_of = static_cast<int>(min(s.k1 - key0_of, static_cast<int64_t>(kPtKeys)));
+  int64_t key0 = 0;  // the image's first key
+  int keys = 0;
+  PtScan(a, false, [&](int, const PkSeq& s, int64_t first, int blocks) {
+    const bool here = first >= 0 && image >= first && image < first + blocks;
+    if (here) {
+      key0 = s.k0 + (image - first) * kPtKeys;
+      keys = static_cast<int>(min(s.k1 - key0, static_cast<int64_t>(kPtKeys)));
     }
+    return here;
   });
-  __syncthreads();
-  const int keys = keys_of;
-  if (keys == 0) return;
+  const uint32_t found = __ballot_sync(0xffffffffu, keys != 0);
+  if (found == 0) return;
+  key0 = __shfl_sync(0xffffffffu, key0, __ffs(found) - 1);
+  keys = __shfl_sync(0xffffffffu, keys, __ffs(found) - 1);
   const int64_t stride = static_cast<int64_t>(a.in.kv_heads) * HD;
-  const float* x = (is_v ? a.in.v : a.in.k) + key0_of * stride + head * HD;
+  const float* x = (is_v ? a.in.v : a.in.k) + key0 * stride + head * HD;
   uint8_t* hi = a.images + (image * a.in.kv_heads + head) * (int64_t{8} * kPtKeys * HD) +
                 (is_v ? 4 * kPtKeys * HD : 0);
   uint8_t* lo = hi + 2 * kPtKeys * HD;
-  // 8 values a step: of one key (K) or of one dimension (V)
+  // 8 values a step: of one key (K) or of one dimension (V).  (512 threads of
+  // four steps: the code of 256 with eight took longer to fetch than to run.)
   constexpr int kSteps = kPtKeys * HD / 8 / kPtSplitThreads;
   float val[kSteps][8];
   float top = 0.0f;
@@ -533,15 +529,22 @@ __global__ void __launch_bounds__(kPtSplitThreads) PkSplitKernel(PtArgs a) {
       const int key = n / (HD / 8), c = n % (HD / 8);
       float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
       if (key < keys) {
-        u = *reinterpret_cast<const float4*>(x + key * stride + 8 * c);
-        w = *reinterpret_cast<const float4*>(x + key * stride + 8 * c + 4);
+        const float* from = x + key * stride + 8 * c;
+        u = *reinterpret_cast<const float4*>(from);
+        w = *reinterpret_cast<const float4*>(from + 4);
       }
       val[i][0] = u.x; val[i][1] = u.y; val[i][2] = u.z; val[i][3] = u.w;
       val[i][4] = w.x; val[i][5] = w.y; val[i][6] = w.z; val[i][7] = w.w;
     } else {
       const int d = n % HD, k0 = n / HD * 8;
+      const float* from = x + k0 * stride + d;
+      if (k0 + 8 <= keys) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) val[i][e] = k0 + e < keys ? x[(k0 + e) * stride + d] : 0.0f;
+        for (int e = 0; e < 8; ++e, from += stride) val[i][e] = *from;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e, from += stride) val[i][e] = k0 + e < keys ? *from : 0.0f;
+      }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -1182,7 +1185,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const float inv = sees ? kPtPScale / l : 0.0f;
         const uint64_t inv2 = PtPair(inv, inv);
         float4* out = reinterpret_cast<float4*>(
-            a.in.out + first_of(w) + (row * a.in.n_heads + v % a.group) * HD);
+            a.in.out + first_of(w) +
+            (static_cast<int64_t>(row) * a.in.n_heads + v % a.group) * HD);
 #pragma unroll
         for (int i = 0; i < HD / 4; ++i) {
           float4 x;
@@ -1373,6 +1377,14 @@ int LaunchPkTc(const PtArgs& a, cudaStream_t s) {
     cudaGetLastError();
     return Fail(MLB_ERR_CUDA, "mlb_attention_packed_f32: shared memory opt-in");
   }
+  // The split of registers between the kernel's roles draws on what a launch
+  // has; with fewer a role would wait for registers forever.
+  static const int regs = [] {
+    cudaFuncAttributes f{};
+    return cudaFuncGetAttributes(&f, PkTcKernel<HD>) == cudaSuccess ? f.numRegs : 0;
+  }();
+  if (regs * kPtThreads < 256 * regs + 128 * kPtRegsOutput + 128 * kPtRegsIssue)
+    return Fail(MLB_ERR_CUDA, "mlb_attention_packed_f32: built with too few registers");
   // q as [rows][heads][HD]; a box is 32 dimensions of a tile's vectors
   CUtensorMap q_map;
   const cuuint64_t dims[3] = {HD, static_cast<cuuint64_t>(a.in.n_heads),

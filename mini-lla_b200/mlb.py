@@ -535,6 +535,11 @@ def _plain(t, dtype, device):
     return t.dtype is dtype and t.get_device() == device and t.is_contiguous()
 
 
+def _word(t, device):
+    import torch
+    return _plain(t, torch.int32, device) and t.numel() >= 1
+
+
 def attention_packed(q, k, v, q_offsets, k_offsets=None, out=None, scratch=None, status=None,
                      stream=None):
     """Causal attention over packed sequences: q [rows, n_heads, hd], k and v
@@ -562,7 +567,7 @@ def attention_packed(q, k, v, q_offsets, k_offsets=None, out=None, scratch=None,
             _plain(k_offsets, i32, device) and k_offsets.shape == q_offsets.shape and
             (out is None or (_plain(out, f32, device) and out.shape == q.shape)) and
             (scratch is None or _plain(scratch, f32, device)) and
-            (status is None or _plain(status, i32, device))):
+            (status is None or _word(status, device))):
         _refuse(op, device, ("q", q, f32, None), ("k", k, f32, None), ("v", v, f32, k.shape),
                 ("q_offsets", q_offsets, i32, (max(n_seqs, 0) + 1,)),
                 ("k_offsets", k_offsets, i32, q_offsets.shape), ("out", out, f32, q.shape),
@@ -635,7 +640,7 @@ def kv8_write(cache, table, k, v, offsets, positions, status=None, stream=None):
     if not (k.shape == (rows, kvh, hd) and _plain(k, f32, device) and _plain(v, f32, device) and
             v.shape == k.shape and _plain(offsets, i32, device) and
             offsets.shape == (n_seqs + 1,) and _plain(positions, i32, device) and
-            positions.shape == (n_seqs,) and (status is None or _plain(status, i32, device))):
+            positions.shape == (n_seqs,) and (status is None or _word(status, device))):
         _refuse(op, device, ("k", k, f32, (rows, kvh, hd)), ("v", v, f32, k.shape),
                 ("offsets", offsets, i32, (n_seqs + 1,)),
                 ("positions", positions, i32, (n_seqs,)), ("status", status, i32, None))
@@ -656,7 +661,7 @@ def kv8_read(cache, table, offsets, positions, rows: int, status=None, stream=No
     pool, (n_blocks, kvh, block, hd), (n_seqs, cols), device = _pool(cache, table, op)
     if not (_plain(offsets, i32, device) and offsets.shape == (n_seqs + 1,) and
             _plain(positions, i32, device) and positions.shape == (n_seqs,) and
-            (status is None or _plain(status, i32, device))):
+            (status is None or _word(status, device))):
         _refuse(op, device, ("offsets", offsets, i32, (n_seqs + 1,)),
                 ("positions", positions, i32, (n_seqs,)), ("status", status, i32, None))
     with _On(table, stream) as on:
@@ -695,7 +700,7 @@ def attention_kv8(q, cache, table, lengths, out=None, mass_in=None, mass_out=Non
                                   mass_out.shape == table.shape)) and
             (out is None or (_plain(out, f32, device) and out.shape == q.shape)) and
             (scratch is None or _plain(scratch, f32, device)) and
-            (status is None or _plain(status, i32, device))):
+            (status is None or _word(status, device))):
         _refuse(op, device, ("q", q, f32, (n_seqs, nh, hd)), ("lengths", lengths, i32, (n_seqs,)),
                 ("mass_in", mass_in, f32, table.shape), ("mass_out", mass_out, f32, table.shape),
                 ("out", out, f32, q.shape), ("scratch", scratch, f32, None),
@@ -729,7 +734,7 @@ def kv8_evict(table, lengths, mass, block_tokens: int, keep_blocks: int, sink_bl
     n_seqs, cols = table.shape
     if not (device >= 0 and _plain(table, i32, device) and _plain(lengths, i32, device) and
             lengths.shape == (n_seqs,) and _plain(mass, f32, device) and
-            mass.shape == table.shape and (status is None or _plain(status, i32, device))):
+            mass.shape == table.shape and (status is None or _word(status, device))):
         _refuse(op, device, ("table", table, i32, None), ("lengths", lengths, i32, (n_seqs,)),
                 ("mass", mass, f32, table.shape), ("status", status, i32, None))
     with _On(table, stream) as on:
