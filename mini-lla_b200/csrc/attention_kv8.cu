@@ -27,8 +27,9 @@
 // n % 2: a thread (lane = 4 row + c) then holds the scores of tokens 8 c ..
 // 8 c + 7 of its head, which are its part of the second product's A operand as
 // they stand, and its V codes are 8 consecutive bytes of V's [hd][token]
-// rows.  K rows are stored in that column order, their 32-byte groups turned
-// by row: the 8-byte reads of both products are free of bank conflicts.  Codes travel by cp.async, kStages - 1 units ahead of the
+// rows.  K rows are stored in that column order with an odd pitch in units
+// of 32 bytes: the 8-byte reads of both products are free of bank
+// conflicts.  Codes travel by cp.async, kStages - 1 units ahead of the
 // products, each warp on its own.
 //
 // Bound: HBM reads of 2 hd bytes per token and kv head.
@@ -162,34 +163,23 @@ __device__ __forceinline__ void Next(const A8Args& a, Place& p) {
   } while (p.units == 0);
 }
 
-// Shared memory of a warp: kStages of (K, V, the two scales), then q's pieces
-// for up to GQ heads.
-template <int HD, int GQ>
+template <int HD>
 struct A8Smem {
-  static constexpr int kKBytes = kUnit * HD;
-  static constexpr int kStageBytes = kKBytes + HD * kUnit + 16;
+  // an odd number of 32-byte groups per K row
+  static constexpr int kKPitch = (HD / 32) % 2 == 0 ? HD + 32 : HD;
+  static constexpr int kKBytes = kUnit * kKPitch;
+  static constexpr int kStageBytes = kKBytes + HD * kUnit + 16;  // K, V, the two scales
   static constexpr int kStages = 2;
-  static constexpr int kQBytes = (HD / 16) * GQ * 4 * 16;  // A operand of the scores
-  static constexpr int kWarpBytes = kStages * kStageBytes + kQBytes;
-  static constexpr int kBytes = kA8Warps * kWarpBytes;
+  static constexpr int kQBytes = (HD / 16) * 32 * 16;  // A operand of the scores
+  static constexpr int kBytes = kA8Warps * (kStages * kStageBytes + kQBytes);
   // CTAs that fit an SM's shared memory (1 KB of each is the system's)
-  static constexpr int kFit = 228 * 1024 / (kBytes + 1024);
-  static constexpr int kCtasPerSm = kFit < 1 ? 1 : kFit > 2 ? 2 : kFit;
+  static constexpr int kFit = 228 * 1024 / (kBytes + 1024 + 256);
+  static constexpr int kCtasPerSm = kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
 };
 
-// Where the 32-byte group g of K row r is kept: turned so that group g of four
-// consecutive rows falls on four different groups of banks.
 template <int HD>
-__device__ __forceinline__ int TurnedGroup(int r, int g) {
-  constexpr int groups = HD / 32;
-  if (groups % 4 == 0) return g ^ (r & 3);
-  if (groups % 2 == 0) return g ^ ((r >> 1) & 1);
-  return g;
-}
-
-template <int HD, int GQ>
-__global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD, GQ>::kCtasPerSm) A8Kernel(A8Args a) {
-  using S = A8Smem<HD, GQ>;
+__global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kernel(A8Args a) {
+  using S = A8Smem<HD>;
   constexpr int kStages = S::kStages;
   constexpr int DC = HD / 32;  // groups of 32 dimensions
   constexpr int DT = HD / 8;   // output tiles
@@ -198,10 +188,8 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD, GQ>::kCtasPerSm) A8K
   extern __shared__ __align__(16) uint8_t a8_raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = lane >> 2, c = lane & 3;  // head of the group / column; quarter
-  uint8_t* ring = a8_raw + warp * S::kWarpBytes;
-  // q's pieces, [k16 step][lane of the first GQ rows]; with GQ = 4 the rows
-  // behind repeat them, and nobody looks at their results
-  uint4* qf = reinterpret_cast<uint4*>(ring + kStages * S::kStageBytes) + (lane & (4 * GQ - 1));
+  uint8_t* ring = a8_raw + warp * (kStages * S::kStageBytes + S::kQBytes);
+  uint4* qf = reinterpret_cast<uint4*>(ring + kStages * S::kStageBytes) + lane;  // [k16 step][lane]
 
   // all units, and the place where this warp's share begins (each warp on its
   // own: the lengths come from L2 once and then from L1)
@@ -244,9 +232,6 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD, GQ>::kCtasPerSm) A8K
   }
   Place get = put;  // next unit to compute
 
-  // (HD = 128) this lane's offset in a K stage for its rows with i = 0
-  const int k_to = (8 * (lane >> 4) + ((lane >> 3) & 1)) * 128 +
-                   32 * (((lane & 7) >> 1) ^ ((lane >> 3) & 1)) + 16 * (lane & 1);
   // block ids of 32 columns of the sequence that is being copied, one a lane
   int window = -1;
   int window_seq = -1;
@@ -269,23 +254,11 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD, GQ>::kCtasPerSm) A8K
       const int8_t* v = a.v_codes + at * a.block * HD + place;
       // K: 16-byte chunks in memory order; token r goes to the row of its
       // score column
-      if constexpr (HD == 128) {
-        // r = 4 i + lane / 8: its row is 16 (i % 2) + 2 (i / 2) plus a part
-        // that only the lane sets, and turns by 2 (i / 2 % 2) besides
-        uint8_t* row0 = to + k_to;
-        uint8_t* row2 = to + (k_to ^ 64);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          CopyAsync16(((i >> 1) & 1 ? row2 : row0) + (16 * (i & 1) + 2 * (i >> 1)) * HD,
-                      k + 16 * lane + 512 * i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-          const int x = 32 * i + lane, r = x / (HD / 16), ch = x % (HD / 16);
-          const int dst = 8 * ((r & 7) >> 1) + 2 * (r >> 3) + (r & 1);
-          CopyAsync16(to + dst * HD + 32 * TurnedGroup<HD>(dst, ch >> 1) + 16 * (ch & 1),
-                      k + r * HD + 16 * ch);
-        }
+      for (int i = 0; i < HD / 16; ++i) {
+        const int x = 32 * i + lane, r = x / (HD / 16), ch = x % (HD / 16);
+        const int dst = 8 * ((r & 7) >> 1) + 2 * (r >> 3) + (r & 1);
+        CopyAsync16(to + dst * S::kKPitch + 16 * ch, k + r * HD + 16 * ch);
       }
       uint8_t* vt = to + S::kKBytes;
       if (a.block == kUnit) {
@@ -361,11 +334,11 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD, GQ>::kCtasPerSm) A8K
           uint4 a;
           SplitPair(x[j][4 * s] * up, x[j][4 * s + 1] * up, a.x, a.y);
           SplitPair(x[j][4 * s + 2] * up, x[j][4 * s + 3] * up, a.z, a.w);
-          if (row < GQ) qf[4 * GQ * (2 * j + s)] = a;
+          qf[32 * (2 * j + s)] = a;  // read by this lane only
         }
     }
     CopyAsyncWait<kStages - 1>();
-    __syncwarp();  // all lanes' copies of this unit have landed (and q's pieces)
+    __syncwarp();  // all lanes' copies of this unit have landed
     if ((usable >> stage & 1u) != 0) {
       const uint8_t* kt = ring + stage * S::kStageBytes;
       const uint8_t* vt = kt + S::kKBytes;
@@ -380,11 +353,11 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD, GQ>::kCtasPerSm) A8K
           uint2 w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            w[j] = *reinterpret_cast<const uint2*>(
-                kt + (8 * j + row) * HD + 32 * TurnedGroup<HD>(8 * j + row, g) + 8 * c);
+            w[j] = *reinterpret_cast<const uint2*>(kt + (8 * j + row) * S::kKPitch + 32 * g +
+                                                   8 * c);
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            const uint4 q = qf[4 * GQ * (2 * g + s)];
+            const uint4 q = qf[32 * (2 * g + s)];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t b0, b1;
@@ -640,22 +613,19 @@ const char* A8Shape(int64_t n_seqs, int64_t table_cols, int block, int n_heads, 
 
 // Warps of the grid: as many as run at once, but not more than there can be
 // units.
-template <int GQ>
-int CtasPerSm(int hd) {
+int Workers(int64_t n_seqs, int64_t unit_cols, int kv_heads, int hd) {
+  int per_sm = 1;
   switch (hd / 32) {
-    case 1: return A8Smem<32, GQ>::kCtasPerSm;
-    case 2: return A8Smem<64, GQ>::kCtasPerSm;
-    case 3: return A8Smem<96, GQ>::kCtasPerSm;
-    case 4: return A8Smem<128, GQ>::kCtasPerSm;
-    case 5: return A8Smem<160, GQ>::kCtasPerSm;
-    case 6: return A8Smem<192, GQ>::kCtasPerSm;
-    case 7: return A8Smem<224, GQ>::kCtasPerSm;
-    default: return A8Smem<256, GQ>::kCtasPerSm;
+    case 1: per_sm = A8Smem<32>::kCtasPerSm; break;
+    case 2: per_sm = A8Smem<64>::kCtasPerSm; break;
+    case 3: per_sm = A8Smem<96>::kCtasPerSm; break;
+    case 4: per_sm = A8Smem<128>::kCtasPerSm; break;
+    case 5: per_sm = A8Smem<160>::kCtasPerSm; break;
+    case 6: per_sm = A8Smem<192>::kCtasPerSm; break;
+    case 7: per_sm = A8Smem<224>::kCtasPerSm; break;
+    default: per_sm = A8Smem<256>::kCtasPerSm; break;
   }
-}
-int Workers(int64_t n_seqs, int64_t unit_cols, int kv_heads, int group, int hd) {
-  const int64_t ctas =
-      static_cast<int64_t>(group <= 4 ? CtasPerSm<4>(hd) : CtasPerSm<8>(hd)) * SmCount();
+  const int64_t ctas = static_cast<int64_t>(per_sm) * SmCount();
   const int64_t most = n_seqs * unit_cols * kv_heads;
   const int64_t need = (most + kA8Warps - 1) / kA8Warps;
   return static_cast<int>(need < ctas ? need : ctas) * kA8Warps;
@@ -670,7 +640,7 @@ A8Scratch ScratchOf(int64_t n_seqs, int64_t table_cols, int block, int n_heads, 
                     int hd, bool with_mass) {
   A8Scratch s;
   const int64_t unit_cols = table_cols * block / kUnit;
-  s.workers = Workers(n_seqs, unit_cols, kv_heads, n_heads / kv_heads, hd);
+  s.workers = Workers(n_seqs, unit_cols, kv_heads, hd);
   s.lse = 0;
   s.units = (2 * n_seqs * n_heads + 3) & ~int64_t{3};
   s.spans = s.units + (with_mass ? (2 * n_seqs * unit_cols * n_heads + 3) & ~int64_t{3} : 0);
@@ -679,23 +649,18 @@ A8Scratch ScratchOf(int64_t n_seqs, int64_t table_cols, int block, int n_heads, 
   return s;
 }
 
-template <int HD, int GQ>
+template <int HD>
 int LaunchA8(const A8Args& a, cudaStream_t s) {
-  constexpr int shm = A8Smem<HD, GQ>::kBytes;
+  constexpr int shm = A8Smem<HD>::kBytes;
   if (shm > 48 * 1024 &&
-      cudaFuncSetAttribute(A8Kernel<HD, GQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, shm) !=
+      cudaFuncSetAttribute(A8Kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, shm) !=
           cudaSuccess) {
     cudaGetLastError();
     return Fail(MLB_ERR_CUDA, "mlb_attention_kv8_f32: shared memory opt-in");
   }
-  Launch(A8Kernel<HD, GQ>, dim3(static_cast<unsigned>(a.workers / kA8Warps)), kA8Warps * 32,
+  Launch(A8Kernel<HD>, dim3(static_cast<unsigned>(a.workers / kA8Warps)), kA8Warps * 32,
          static_cast<size_t>(shm), s, a);
   return MLB_OK;
-}
-
-template <int HD>
-int LaunchA8(const A8Args& a, cudaStream_t s) {
-  return a.group <= 4 ? LaunchA8<HD, 4>(a, s) : LaunchA8<HD, 8>(a, s);
 }
 
 }  // namespace
