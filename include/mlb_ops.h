@@ -428,9 +428,9 @@ int64_t mlb_attention_packed_scratch_floats(int64_t q_rows, int64_t k_rows,
  *   Calls that may overlap on the GPU need scratch of their own.
  * Within 1e-5 * sum_t w_t |v_t| of the exact result for scores of ordinary
  * spread.  out must not overlap q, k or v.  Keys, values and rows that a row
- * does not see do not reach it, whatever they hold; a row that sees an Inf or
- * NaN gets NaN in the outputs it reaches (also where a weight of 0 would hide
- * it).
+ * does not see do not reach it, whatever they hold.  A row that sees an Inf or
+ * NaN may get NaN where a weight of 0 would hide it; finite keys whose scores
+ * overflow to -inf have a weight of 0.
  */
 int mlb_attention_packed_f32(const float* q, const float* k, const float* v,
                              float* out, const int32_t* q_offsets,
@@ -523,9 +523,9 @@ int64_t mlb_attention_kv8_scratch_floats(int64_t n_seqs, int64_t table_cols,
  * error and places behind the last block get mass_in unchanged).
  * scratch: at least mlb_attention_kv8_scratch_floats(...) floats, 16-byte
  * aligned; calls that may overlap on the GPU need scratch of their own.  out
- * overlaps neither q nor the pool.  Deterministic.  Queries are taken in 22 bits, the weights in 22
- * bits, all sums in fp32: within 1e-5 * sum_t w_t |v_t| of the exact result
- * over the cache's values for scores of ordinary spread.
+ * overlaps neither q nor the pool.  Deterministic.  Queries and weights are
+ * taken in 22 bits, all sums in fp32: within 1e-5 * sum_t w_t |v_t| of the
+ * exact result over the cache's values for scores of ordinary spread.
  */
 int mlb_attention_kv8_f32(const float* q, const int8_t* k_codes,
                           const int8_t* v_codes, const float* k_scales,

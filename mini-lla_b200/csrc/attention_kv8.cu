@@ -33,6 +33,7 @@
 // products, each warp on its own.
 //
 // Bound: HBM reads of 2 hd bytes per token and kv head.
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
       fresh = false;
       bad = false;
       first_unit = get.unit;
-      m = -INFINITY;
+      m = -FLT_MAX;  // finite: a unit of scores of -inf has weights of 0
       l = 0.0f;
 #pragma unroll
       for (int i = 0; i < DT; ++i) acc[i][0] = acc[i][1] = 0.0f;
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const float m_new = fmaxf(m, top);
-      const float alpha = Exp2(m - m_new);  // 0 for the first unit
+      const float alpha = Exp2(m - m_new);
       m = m_new;
       float sum = 0.0f;
       uint32_t ph[4], pl[4];
@@ -504,18 +505,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) A8JoinKernel(A8Args a) {
            (((static_cast<int64_t>(span.x) + i) * 2 + (i == 0 ? 1 : 0)) * a.group + h % a.group) *
                stride4;
   };
-  float m = -INFINITY, l = 0.0f, bad = 0.0f;
+  float m = -FLT_MAX, l = 0.0f, bad = 0.0f;
   float4 acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int base = warp; base < n; base += 32 * kJoinWarps) {  // 32 partials
     const int mine = base + kJoinWarps * lane;
-    const float4 head = mine < n ? part(mine)[0] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    const float4 head = mine < n ? part(mine)[0] : make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
     const float m_new = fmaxf(m, WarpMax(head.x));
-    const float keep = m == m_new ? 1.0f : Exp2(m - m_new);
-    // a partial of NaN scores alone has m = -inf and keeps its NaN
-    const float f = head.x == -INFINITY ? 0.0f : Exp2(head.x - m_new);
-    l = fmaf(l, keep, WarpSum(head.x == -INFINITY ? head.y : head.y * f));
+    const float keep = Exp2(m - m_new), f = Exp2(head.x - m_new);
+    l = fmaf(l, keep, WarpSum(head.y * f));
     bad = fmaxf(bad, WarpMax(head.z));
     m = m_new;
 #pragma unroll
@@ -546,7 +545,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) A8JoinKernel(A8Args a) {
   }
   __syncthreads();
   if (threadIdx.x >= hd4) return;
-  m = -INFINITY;
+  m = -FLT_MAX;
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) {
     m = fmaxf(m, ms[w]);
@@ -556,8 +555,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) A8JoinKernel(A8Args a) {
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) {
-    const float f = ms[w] == -INFINITY ? 0.0f : Exp2(ms[w] - m);
-    l += ms[w] == -INFINITY ? ls[w] : ls[w] * f;
+    const float f = Exp2(ms[w] - m);
+    l = fmaf(ls[w], f, l);
     const float4 x = accs[w][threadIdx.x];
     o.x = fmaf(x.x, f, o.x);
     o.y = fmaf(x.y, f, o.y);

@@ -7,6 +7,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kPkWarps * 32) PkRowKernel(PkArgs a) {
   float4 acc[G][NV];
 #pragma unroll
   for (int h = 0; h < G; ++h) {
-    m[h] = -INFINITY;
+    m[h] = -FLT_MAX;  // finite: scores of -inf alone have weights of 0
     l[h] = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) acc[h][v] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kPkWarps * 32) PkRowKernel(PkArgs a) {
     for (int h = 0; h < G; ++h) {
       const float x = lane < n ? dot[h] * scale : -INFINITY;
       const float m_new = fmaxf(m[h], WarpMax(x));
-      const float alpha = m[h] == m_new ? 1.0f : PtExp2(m[h] - m_new);
+      const float alpha = PtExp2(m[h] - m_new);
       const float p = lane < n ? PtExp2(x - m_new) : 0.0f;
       l[h] = fmaf(l[h], alpha, p);  // this lane's keys
       m[h] = m_new;
@@ -185,15 +186,13 @@ __global__ void __launch_bounds__(kPkWarps * 32) PkRowKernel(PkArgs a) {
   }
   __syncthreads();
   for (int h = warp; h < G; h += kPkWarps) {
-    float mm = -INFINITY, ll = 0.0f;
+    float mm = -FLT_MAX, ll = 0.0f;
     for (int w = 0; w < kPkWarps; ++w) mm = fmaxf(mm, sm_m[w][h]);
     float f[kPkWarps];
 #pragma unroll
     for (int w = 0; w < kPkWarps; ++w) {
-      f[w] = sm_m[w][h] == -INFINITY ? 0.0f : PtExp2(sm_m[w][h] - mm);
-      // a warp whose scores are NaN keeps them visible
-      if (sm_l[w][h] != sm_l[w][h]) f[w] = NAN;
-      ll = fmaf(sm_l[w][h], f[w], ll);
+      f[w] = PtExp2(sm_m[w][h] - mm);
+      ll = fmaf(sm_l[w][h], f[w], ll);  // a NaN stays one at f = 0 too
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -768,7 +767,7 @@ __device__ void PtSlowTile(const PtArgs& a, const PtTile& tile, int head) {
     const int64_t at =
         ((tile.row0 + i / a.group) * static_cast<int64_t>(a.in.n_heads) + head * a.group +
          i % a.group) * HD;
-    float q[E], acc[E], m = -INFINITY, l = 0.0f;
+    float q[E], acc[E], m = -FLT_MAX, l = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       q[e] = a.in.q[at + 32 * e + lane];
@@ -780,7 +779,7 @@ __device__ void PtSlowTile(const PtArgs& a, const PtTile& tile, int head) {
       for (int e = 0; e < E; ++e) dot = fmaf(q[e], k[t * stride + 32 * e + lane], dot);
       const float s = WarpSum(dot) * a.in.scale;
       const float m_new = fmaxf(m, s);
-      const float alpha = m == -INFINITY ? 0.0f : expf(m - m_new);
+      const float alpha = expf(m - m_new);
       const float p = expf(s - m_new);
       l = fmaf(l, alpha, p);
 #pragma unroll

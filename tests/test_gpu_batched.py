@@ -211,6 +211,28 @@ def test_packed_attention_many_tiles(cuda, path, nh, nkv, hd, most, context):
     assert mlb.wait_timeouts() == 0
 
 
+@pytest.mark.parametrize("hd", [64, 128, 96])
+@pytest.mark.parametrize("first,last", [(32, 64), (0, 32), (0, 128), (128, 200), (60, 199)])
+def test_packed_attention_scores_below_the_range(cuda, path, hd, first, last):
+    """Keys whose scores overflow to -inf have no weight, wherever they stand;
+    the others' scores are 0 here, so their weights are the same."""
+    rng = np.random.default_rng(first + last)
+    q, k, v, qo, ko = packed_inputs(rng, [1, 30], [200, 200], 4, 2, hd)
+    q, k = np.full_like(q, 1e20), np.zeros_like(k)
+    k[first:last] = k[200 + first:200 + last] = -1e20
+    got = mlb.attention_packed(dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(qo, cuda),
+                               dev(ko, cuda)).cpu().numpy()
+    for row in range(31):
+        base, sees = (0, 200) if row == 0 else (200, 200 - 30 + row)
+        t = np.setdiff1d(np.arange(sees), np.arange(first, last))
+        x = np.repeat(v[base + t].astype(np.float64), 2, axis=1)
+        if len(t):
+            check(got[row], x.mean(0), (2.0 ** -20 + (50 + 64) * 2.0 ** -23) * np.abs(x).mean(0) +
+                  2.0 ** -37 * np.abs(x).max(2, keepdims=True).sum(0), row)
+        else:
+            assert np.isnan(got[row]).all()
+
+
 def test_packed_attention_equals_rows_of_one_sequence(cuda, path):
     """One sequence is mlb_attention_rows_f32 over its cache."""
     rng = np.random.default_rng(9)
@@ -598,6 +620,39 @@ def test_attention_kv8_not_finite(cuda):
     lost[2, 3] = lost[2, 5] = True
     assert not np.isfinite(got[lost]).any()
     check(got[~lost], want[~lost], tol[~lost])
+
+
+@pytest.mark.parametrize("lengths", [[100, 33, 9000], [9000, 9000, 40]])
+def test_attention_kv8_scores_below_the_range(cuda, lengths):
+    """Blocks whose scores overflow to -inf have no weight and collect none; the
+    others' scores are 0 here, so their tokens' weights are the same."""
+    import torch
+    rng = np.random.default_rng(24)
+    nh, nkv, hd, block = 16, 8, 128, 32
+    needed = [-(-n // block) for n in lengths]
+    n_blocks = sum(needed)
+    pool, table = make_pool(rng, n_blocks, nkv, block, hd), make_table(rng, needed, n_blocks)
+    low = rng.random(n_blocks) < 0.5
+    for i, n in enumerate(needed):  # the first and the last in turn
+        low[table[i, 0]], low[table[i, n - 1]] = i % 2 == 0, i % 2 == 1
+    pool[0][low], pool[0][~low], pool[2][low] = -127, 0, 1e18
+    q = np.full((3, nh, hd), 1e20, np.float32)
+    mass_out = torch.empty(table.shape, device=cuda)
+    got = mlb.attention_kv8(dev(q, cuda), to_device(pool, cuda), dev(table, cuda),
+                            dev(np.array(lengths, np.int32), cuda),
+                            mass_out=mass_out).cpu().numpy()
+    mass_out = mass_out.cpu().numpy()
+    for i, length in enumerate(lengths):
+        t = np.arange(length)
+        t = t[~low[table[i, t // block]]]
+        ids = table[i, t // block]
+        x = pool[1][ids, :, :, t % block] * pool[3][ids].astype(np.float64)[:, :, None]
+        x = np.repeat(x, nh // nkv, axis=1)
+        rel = 2.0 ** -20 + (length / 4 + 64) * 2.0 ** -23
+        check(got[i], x.mean(0), rel * np.abs(x).mean(0) +
+              2.0 ** -37 * np.abs(x).max(2, keepdims=True).sum(0), f"out {i}")
+        each = np.bincount(t // block, np.full(len(t), nh / len(t)), table.shape[1])
+        check(mass_out[i], each, each * (rel + (nh + 4) * 2.0 ** -23), f"mass {i}")
 
 
 def test_attention_kv8_bad_lengths_and_blocks(cuda):
