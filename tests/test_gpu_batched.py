@@ -886,3 +886,82 @@ def test_batched_calls_on_a_stream_and_in_a_graph(cuda, path):
         want = evict_reference(table, lengths, masses[turn % 2].cpu().numpy(), block, 4, 1, 1)
         for g, w in zip(evicted, want):
             assert np.array_equal(g.cpu().numpy(), w)
+
+
+def test_batched_calls_on_two_streams_at_once(cuda, path):
+    """Calls that overlap on the GPU give what each gives alone."""
+    import torch
+    rng = np.random.default_rng(42)
+    nh, nkv, hd, block, lengths = 16, 4, 128, 32, [900, 40, 333, 2000]
+    needed = [-(-n // block) for n in lengths]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    jobs = []
+    for _ in streams:
+        pool, table = make_pool(rng, 120, nkv, block, hd), make_table(rng, needed, 120)
+        lens = [300, 17, 450, 130]
+        q, k, v, qo, _ = packed_inputs(rng, lens, lens, nh, nkv, hd)
+        args = (dev(q, cuda), dev(k, cuda), dev(v, cuda), dev(qo, cuda))
+        decode = (dev(q[:4], cuda), to_device(pool, cuda), dev(table, cuda),
+                  dev(np.array(lengths, np.int32), cuda))
+        jobs.append((args, decode, torch.empty(table.shape, device=cuda)))
+    alone = []
+    for args, decode, mass in jobs:
+        alone.append((mlb.attention_packed(*args), mlb.attention_kv8(*decode, mass_out=mass),
+                      mass.clone()))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for stream, (args, decode, mass) in zip(streams, jobs):
+            got.append((mlb.attention_packed(*args, stream=stream),
+                        mlb.attention_kv8(*decode, mass_out=mass, stream=stream)))
+        torch.cuda.synchronize()
+        for (packed, out), (_, _, mass), want in zip(got, jobs, alone):
+            assert torch.equal(packed, want[0]) and torch.equal(out, want[1])
+            assert torch.equal(mass, want[2])
+    assert mlb.wait_timeouts() == 0
+
+
+def test_packed_attention_rows_past_32_bits(cuda, path):
+    """Rows whose elements lie past 2^31 (9 GB a tensor)."""
+    import torch
+    rng = np.random.default_rng(43)
+    nh, nkv, hd, n = 32, 32, 128, 150
+    rows = 2 ** 31 // (nh * hd) + 200
+    q, k, v, _, _ = packed_inputs(rng, [n], [n], nh, nkv, hd)
+    want, tol = packed_reference(q, k, v, [0, n], [0, n])
+    big = [torch.empty((rows, nh, hd), device=cuda) for _ in range(4)]
+    for b, x in zip(big, (q, k, v)):
+        b[rows - n:] = dev(x, cuda)
+    mlb.attention_packed(*big[:3], dev(np.array([rows - n, rows], np.int32), cuda), out=big[3])
+    check(big[3][rows - n:].cpu().numpy(), want, tol)
+
+
+def test_kv8_blocks_past_32_bits(cuda):
+    """Blocks whose codes lie past 2^32 (4.5 GB of codes for K and for V)."""
+    import torch
+    rng = np.random.default_rng(44)
+    nh, nkv, hd, block, n = 16, 8, 128, 32, 200
+    n_blocks = 2 ** 32 // (nkv * block * hd) + 100
+    cache = mlb.kv8_cache(n_blocks, nkv, block, hd, cuda)
+    table = np.arange(n_blocks - 1, n_blocks - 9, -1, dtype=np.int32)[None]
+    q, k, v, _, _ = packed_inputs(rng, [n], [n], nh, nkv, hd)
+    offsets, zero = np.array([0, n], np.int32), np.zeros(1, np.int32)
+    mlb.kv8_write(cache, dev(table, cuda), dev(k, cuda), dev(v, cuda), dev(offsets, cuda),
+                  dev(zero, cuda))
+    small = [np.zeros(x.shape, x.dtype) for x in make_pool(rng, 8, nkv, block, hd)]
+    own = np.arange(7, -1, -1, dtype=np.int32)[None]  # the same blocks, counted from the last 8
+    small = write_reference(small, own, k, v, offsets, zero, block)
+    for got, x in zip(cache, small):
+        assert np.array_equal(got[n_blocks - 8:].cpu().numpy(), x)
+        assert not bool(got[:n_blocks - 8].any())
+    out = mlb.attention_kv8(dev(q[:1], cuda), cache, dev(table, cuda),
+                            dev(np.array([n], np.int32), cuda))
+    want, tol, _, _ = decode_reference(q[:1], small, own, [n], block)
+    check(out.cpu().numpy(), want, tol)
+    kr, vr = mlb.kv8_read(cache, dev(table, cuda), dev(offsets, cuda), dev(zero, cuda), n)
+    t = np.arange(n)
+    ids = own[0, t // block]
+    assert np.array_equal(kr.cpu().numpy(),
+                          small[0][ids, :, t % block] * small[2][ids][:, :, None])
+    assert np.array_equal(vr.cpu().numpy(),
+                          small[1][ids, :, :, t % block] * small[3][ids][:, :, None])
