@@ -140,7 +140,9 @@ __global__ void __launch_bounds__(kPkWarps * 32) PkRowKernel(PkArgs a) {
     for (int h = 0; h < G; ++h) {
       const float x = lane < n ? dot[h] * scale : -INFINITY;
       const float m_new = fmaxf(m[h], WarpMax(x));
-      const float alpha = PtExp2(m[h] - m_new);
+      // (without the choice the compiler keeps fewer of the loads under way:
+      // 7.8 us instead of 6.1 for one short prompt)
+      const float alpha = m[h] == m_new ? 1.0f : PtExp2(m[h] - m_new);
       const float p = lane < n ? PtExp2(x - m_new) : 0.0f;
       l[h] = fmaf(l[h], alpha, p);  // this lane's keys
       m[h] = m_new;
