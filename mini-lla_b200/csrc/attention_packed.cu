@@ -371,6 +371,18 @@ __device__ __forceinline__ uint64_t PtAdd2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// Four such pairs to 32 bytes of global memory (aligned to them).
+__device__ __forceinline__ void PtStore32(float* to, uint64_t a, uint64_t b, uint64_t c,
+                                          uint64_t d) {
+  float x[8];
+  PtUnpair(a, x[0], x[1]);
+  PtUnpair(b, x[2], x[3]);
+  PtUnpair(c, x[4], x[5]);
+  PtUnpair(d, x[6], x[7]);
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to), "f"(x[0]),
+               "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
+}
 __device__ __forceinline__ float PtMax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -1068,6 +1080,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const int row = v / a.group;
     const bool used = v < (kPtVectors / a.group) * a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const bool wide_out = (reinterpret_cast<uintptr_t>(a.in.out) & 31) == 0;
     const auto first_of = [&](const PtWork& w) {  // the tile's first vector in q and out
       return (static_cast<int64_t>(w.tile.row0) * a.in.n_heads + w.head * a.group) * HD;
     };
@@ -1179,24 +1192,31 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
       if (!ok) break;
       if (w.valid && used && row < w.tile.rows) {
-        // 16 bytes a lane as they stand: turned over between lanes they would
-        // be fewer requests, but the code for it, run once a tile, takes longer
-        // to fetch than these take to drain (13,500 clocks against 5,800)
+        // 32 bytes a lane as they stand, a whole sector: turned over between
+        // lanes they would be fewer requests, but the code for it, run once a
+        // tile, takes longer to fetch than these take to drain
         const bool sees = w.tile.sees + row > 0;
         const float inv = sees ? kPtPScale / l : 0.0f;
         const uint64_t inv2 = PtPair(inv, inv);
-        float4* out = reinterpret_cast<float4*>(
-            a.in.out + first_of(w) +
-            (static_cast<int64_t>(row) * a.in.n_heads + v % a.group) * HD);
+        float* out = a.in.out + first_of(w) +
+                     (static_cast<int64_t>(row) * a.in.n_heads + v % a.group) * HD;
+        if (!sees) {
+          for (int i = 0; i < HD / 4; ++i)
+            reinterpret_cast<float4*>(out)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else if (wide_out) {
 #pragma unroll
-        for (int i = 0; i < HD / 4; ++i) {
-          float4 x;
-          PtUnpair(PtMul2(acc[2 * i], inv2), x.x, x.y);
-          PtUnpair(PtMul2(acc[2 * i + 1], inv2), x.z, x.w);
-          out[i] = x;
+          for (int i = 0; i < HD / 8; ++i)
+            PtStore32(out + 8 * i, PtMul2(acc[4 * i], inv2), PtMul2(acc[4 * i + 1], inv2),
+                      PtMul2(acc[4 * i + 2], inv2), PtMul2(acc[4 * i + 3], inv2));
+        } else {
+#pragma unroll
+          for (int i = 0; i < HD / 4; ++i) {
+            float4 x;
+            PtUnpair(PtMul2(acc[2 * i], inv2), x.x, x.y);
+            PtUnpair(PtMul2(acc[2 * i + 1], inv2), x.z, x.w);
+            reinterpret_cast<float4*>(out)[i] = x;
+          }
         }
-        if (!sees)
-          for (int i = 0; i < HD / 4; ++i) out[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
       if (w.valid) ++t;
       w = next;

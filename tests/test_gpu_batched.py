@@ -211,6 +211,26 @@ def test_packed_attention_many_tiles(cuda, path, nh, nkv, hd, most, context):
     assert mlb.wait_timeouts() == 0
 
 
+@pytest.mark.parametrize("skip", [4, 8, 12])
+def test_packed_attention_tensors_inside_a_buffer(cuda, path, skip):
+    """Tensors that begin at any multiple of 16 bytes."""
+    import torch
+    rng = np.random.default_rng(skip)
+    q, k, v, qo, ko = packed_inputs(rng, [70, 33], [70, 200], 8, 2, 128)
+    want, tol = packed_reference(q, k, v, qo, ko)
+
+    def inside(shape):
+        return torch.full((skip + int(np.prod(shape)) + 4,), 7.0, device=cuda)
+
+    bufs = [inside(x.shape) for x in (q, k, v, q)]
+    views = [b[skip:-4].view(x.shape) for b, x in zip(bufs, (q, k, v, q))]
+    for view, x in zip(views, (q, k, v)):
+        view.copy_(dev(x, cuda))
+    mlb.attention_packed(*views[:3], dev(qo, cuda), dev(ko, cuda), out=views[3])
+    check(views[3].cpu().numpy(), want, tol)
+    assert bool((bufs[3][:skip] == 7.0).all()) and bool((bufs[3][-4:] == 7.0).all())
+
+
 @pytest.mark.parametrize("hd", [64, 128, 96])
 @pytest.mark.parametrize("first,last", [(32, 64), (0, 32), (0, 128), (128, 200), (60, 199)])
 def test_packed_attention_scores_below_the_range(cuda, path, hd, first, last):
