@@ -371,18 +371,6 @@ __device__ __forceinline__ uint64_t PtAdd2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// Four such pairs to 32 bytes of global memory (aligned to them).
-__device__ __forceinline__ void PtStore32(float* to, uint64_t a, uint64_t b, uint64_t c,
-                                          uint64_t d) {
-  float x[8];
-  PtUnpair(a, x[0], x[1]);
-  PtUnpair(b, x[2], x[3]);
-  PtUnpair(c, x[4], x[5]);
-  PtUnpair(d, x[6], x[7]);
-  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to), "f"(x[0]),
-               "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
-               : "memory");
-}
 __device__ __forceinline__ float PtMax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -744,8 +732,9 @@ __device__ __forceinline__ bool PtElect() {
 }
 
 // Shared memory from a 1024-byte aligned base: the ring (an item is the hi and
-// lo images of one block's K or V, or a tile's Q in fp32), blocks' references and sums, queries' scales,
-// the halves' exchange, barriers.
+// lo images of one block's K or V, or a tile's Q in fp32), blocks' references
+// and sums, queries' scales, the halves' exchange, outputs on their way to
+// memory, barriers.
 template <int HD>
 struct PtLayout {
   static constexpr int kItemBytes = 4 * kPtKeys * HD;  // hi and lo
@@ -753,7 +742,8 @@ struct PtLayout {
   static constexpr int kStat = kStages * kItemBytes;         // float [4][3][128]
   static constexpr int kScale = kStat + 12 * kPtVectors * 4;  // float [2][128]
   static constexpr int kSwap = kScale + 2 * kPtVectors * 4;   // float [2][2][128]
-  static constexpr int kBars = kSwap + 4 * kPtVectors * 4;
+  static constexpr int kTurn = (kSwap + 4 * kPtVectors * 4 + 127) / 128 * 128;  // outputs, 4 KB a warp
+  static constexpr int kBars = kTurn + 4 * 4096;
   // full / empty per stage, q_full[2], s_full[2], p_full[4], o_full, o_empty,
   // swap[4], done
   static constexpr int kBarriers = 2 * kStages + 15;
@@ -816,18 +806,19 @@ struct PtWork {
   bool slow;     // computed on the CUDA cores (also: nothing to see)
 };
 
-__device__ __forceinline__ PtWork PtFetch(const PtArgs& a, int64_t total, int& round) {
+__device__ __forceinline__ PtWork PtFetch(const PtArgs& a, uint32_t total, int& round) {
   PtWork w;
   w.valid = false;
   for (;; ++round) {
-    const int64_t base = static_cast<int64_t>(round) * gridDim.x;
+    const uint32_t base = static_cast<uint32_t>(round) * gridDim.x;  // below 2^31 + the grid
     if (base >= total) return w;
-    const int64_t n = base + ((round & 1) == 0 ? blockIdx.x : gridDim.x - 1 - blockIdx.x);
+    const uint32_t n = base + ((round & 1) == 0 ? blockIdx.x : gridDim.x - 1 - blockIdx.x);
     if (n >= total) continue;
     ++round;
     w.valid = true;
-    w.tile = a.tiles[n / a.in.kv_heads];
-    w.head = static_cast<int>(n % a.in.kv_heads);
+    const uint32_t tile = n / static_cast<uint32_t>(a.in.kv_heads);
+    w.tile = a.tiles[tile];
+    w.head = static_cast<int>(n - tile * static_cast<uint32_t>(a.in.kv_heads));
     const int last = w.tile.sees + w.tile.rows - 1;  // keys that the last row sees
     w.nb = last <= 0 ? 0 : (last + kPtKeys - 1) / kPtKeys;
     w.partial0 = w.tile.sees <= 0 ? 0 : w.tile.sees / kPtKeys;
@@ -847,7 +838,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
   extern __shared__ __align__(16) uint8_t pt_raw[];
-  const int64_t total = static_cast<int64_t>(a.blocks[a.in.n_seqs]) * a.in.kv_heads;
+  // (query tile, kv head) pairs: at most 2^31 - 1, as the host checks
+  const uint32_t total = static_cast<uint32_t>(a.blocks[a.in.n_seqs]) * a.in.kv_heads;
   const uint32_t raw_addr = PtSmem(pt_raw);
   uint8_t* base = pt_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   const uint32_t sbase = PtSmem(base);
@@ -1080,7 +1072,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const int row = v / a.group;
     const bool used = v < (kPtVectors / a.group) * a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const bool wide_out = (reinterpret_cast<uintptr_t>(a.in.out) & 31) == 0;
+    // the vector's place in out behind the tile's first, in units of 16 bytes
+    const uint32_t place = (static_cast<uint32_t>(row) * a.in.n_heads + v % a.group) * (HD / 4);
+    uint8_t* turn = base + L::kTurn + (warp & 3) * 4096;
     const auto first_of = [&](const PtWork& w) {  // the tile's first vector in q and out
       return (static_cast<int64_t>(w.tile.row0) * a.in.n_heads + w.head * a.group) * HD;
     };
@@ -1097,16 +1091,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         return *reinterpret_cast<const float4*>(base + stage * L::kItemBytes +
                                                 (i >> 3) * (kPtVectors * 128) + PtSwz(v, i & 7));
       };
-      float top = 0.0f;
+      float top = 0.0f, other = 0.0f;
 #pragma unroll 8
       for (int i = 0; i < kChunks; ++i) {
         const float4 y = chunk(i);
-        const float m = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
-        // a vector with Inf (or NaN) has NaN outputs whatever its scale
-        top = fmaxf(top, m < INFINITY ? m : 0.0f);
+        top = PtMax3(top, fabsf(y.x), fabsf(y.y));
+        other = PtMax3(other, fabsf(y.z), fabsf(y.w));
       }
+      top = fmaxf(top, other);
       float down;
-      const float up = PtUp(live ? top : 0.0f, down);
+      // (a vector with Inf or NaN has NaN outputs whatever its scale)
+      const float up = PtUp(live && top < INFINITY ? top : 0.0f, down);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {  // 32 dimensions: 16 columns of each piece
         uint32_t out[32];
@@ -1191,30 +1186,32 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
       }
       if (!ok) break;
-      if (w.valid && used && row < w.tile.rows) {
-        // 32 bytes a lane as they stand, a whole sector: turned over between
-        // lanes they would be fewer requests, but the code for it, run once a
-        // tile, takes longer to fetch than these take to drain
-        const bool sees = w.tile.sees + row > 0;
-        const float inv = sees ? kPtPScale / l : 0.0f;
+      if (w.valid) {
+        // Through shared memory, 32 dimensions at a time, so that a store
+        // writes whole lines: 32 bytes of its own row a lane kept the memory
+        // path busy for 4,000 clocks, and the next tile's V behind them.
+        const bool live = used && row < w.tile.rows;
+        const uint32_t rows = __ballot_sync(0xffffffffu, live);
+        const float inv = live && w.tile.sees + row > 0 ? kPtPScale / l : 0.0f;
         const uint64_t inv2 = PtPair(inv, inv);
-        float* out = a.in.out + first_of(w) +
-                     (static_cast<int64_t>(row) * a.in.n_heads + v % a.group) * HD;
-        if (!sees) {
-          for (int i = 0; i < HD / 4; ++i)
-            reinterpret_cast<float4*>(out)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        } else if (wide_out) {
+        float4* out = reinterpret_cast<float4*>(a.in.out + first_of(w)) + (lane & 7);
 #pragma unroll
-          for (int i = 0; i < HD / 8; ++i)
-            PtStore32(out + 8 * i, PtMul2(acc[4 * i], inv2), PtMul2(acc[4 * i + 1], inv2),
-                      PtMul2(acc[4 * i + 2], inv2), PtMul2(acc[4 * i + 3], inv2));
-        } else {
+        for (int c = 0; c < HD / 32; ++c) {
+          __syncwarp();  // the last 32 have been read
 #pragma unroll
-          for (int i = 0; i < HD / 4; ++i) {
+          for (int i = 0; i < 8; ++i) {
             float4 x;
-            PtUnpair(PtMul2(acc[2 * i], inv2), x.x, x.y);
-            PtUnpair(PtMul2(acc[2 * i + 1], inv2), x.z, x.w);
-            reinterpret_cast<float4*>(out)[i] = x;
+            PtUnpair(PtMul2(acc[16 * c + 2 * i], inv2), x.x, x.y);
+            PtUnpair(PtMul2(acc[16 * c + 2 * i + 1], inv2), x.z, x.w);
+            *reinterpret_cast<float4*>(turn + PtSwz(lane, i)) = x;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {  // 4 rows a store
+            const int r = 4 * j + (lane >> 3);
+            const uint32_t to = __shfl_sync(0xffffffffu, place, r);
+            const float4 x = *reinterpret_cast<const float4*>(turn + PtSwz(r, lane & 7));
+            if (rows >> r & 1u) out[to + 8 * c] = x;
           }
         }
       }
