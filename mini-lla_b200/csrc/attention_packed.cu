@@ -261,7 +261,8 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
 //   - warp 13: tensor memory; one lane issues S_n, then O_(n - 1), across the
 //     tiles, so that the softmax of a block runs under the products of its
 //     neighbours;
-//   - warps 14-15 only complete the warpgroup that gives up registers.
+//   - warp 14 looks up the CTA's tiles ahead of the others; warp 15 only
+//     completes the warpgroup that gives up registers.
 // Tensor memory: Q hi and lo, two S / P buffers, O.  All waits are bounded; a
 // CTA whose wait gave up writes NaN and is counted (mlb_wait_timeouts).
 //
@@ -743,10 +744,11 @@ struct PtLayout {
   static constexpr int kScale = kStat + 12 * kPtVectors * 4;  // float [2][128]
   static constexpr int kSwap = kScale + 2 * kPtVectors * 4;   // float [2][2][128]
   static constexpr int kTurn = (kSwap + 4 * kPtVectors * 4 + 127) / 128 * 128;  // outputs, 4 KB a warp
-  static constexpr int kBars = kTurn + 4 * 4096;
+  static constexpr int kList = kTurn + 4 * 4096;  // int4 [4][2]
+  static constexpr int kBars = kList + 4 * 32;
   // full / empty per stage, q_full[2], s_full[2], p_full[4], o_full, o_empty,
-  // swap[4], done
-  static constexpr int kBarriers = 2 * kStages + 15;
+  // swap[4], done, listed[4], taken[4]
+  static constexpr int kBarriers = 2 * kStages + 23;
   static constexpr int kSmemBytes = kBars + 8 * kBarriers + 16 + 1024;
 };
 
@@ -795,7 +797,7 @@ __device__ void PtSlowTile(const PtArgs& a, const PtTile& tile, int head) {
   }
 }
 
-// The tiles of a CTA, in the order in which every role walks them: rounds over
+// The tiles of a CTA, in the order in which every role takes them: rounds over
 // the sorted list, every other one backwards.
 struct PtWork {
   PtTile tile;
@@ -857,8 +859,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const uint32_t o_empty = bars + 8 * (2 * kStages + 9);
   const auto swapped = [&](int i) { return bars + 8 * (2 * kStages + 10 + i); };
   const uint32_t all_done = bars + 8 * (2 * kStages + 14);
+  const auto listed = [&](uint32_t t) { return bars + 8 * (2 * kStages + 15 + (t & 3)); };
+  const auto taken = [&](uint32_t t) { return bars + 8 * (2 * kStages + 19 + (t & 3)); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kBars + 8 * L::kBarriers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* slow_flag = abort_flag + 1;  // there are tiles for the CUDA cores
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
 
@@ -874,11 +879,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     for (int i = 0; i < 4; ++i) {
       PtBarInit(p_full(i), 256);
       PtBarInit(swapped(i), 64);
+      PtBarInit(listed(i), 1);
+      PtBarInit(taken(i), 14);  // copies, products, 4 output warps, 8 softmax warps
     }
     PtBarInit(o_full, 1);
     PtBarInit(o_empty, 128);
     PtBarInit(all_done, 1);
-    *abort_flag = 0;
+    *abort_flag = *slow_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 13) {
@@ -903,6 +910,31 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const auto warp_wait = [&](uint32_t bar, uint32_t parity) __attribute__((always_inline)) {
     return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
   };
+  // tile t of the CTA as warp 14 has listed it (not valid: no more)
+  const auto listed_tile = [&](uint32_t t) __attribute__((always_inline)) {
+    const int4* at = reinterpret_cast<const int4*>(base + L::kList) + 2 * (t & 3);
+    const int4 x = at[0], y = at[1];
+    PtWork w;
+    w.tile.row0 = x.x;
+    w.tile.rows = x.y;
+    w.tile.sees = x.z;
+    w.tile.block0 = x.w;
+    w.head = y.x;
+    w.nb = y.y;
+    w.partial0 = y.z;
+    w.valid = y.y != 0;
+    return w;
+  };
+  // the same for a whole warp; false: gave up
+  const auto next_tile = [&](uint32_t& t, PtWork& w) __attribute__((always_inline)) {
+    w.valid = false;
+    if (!warp_wait(listed(t), (t >> 2) & 1)) return false;
+    w = listed_tile(t);
+    __syncwarp();
+    if (lane == 0) PtArrive(taken(t));
+    ++t;
+    return true;
+  };
 
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kPtRegsIssue));
@@ -910,7 +942,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     // --------------------------------------------------------------- copies
       // One warp walks the ring, item by item (a wait for a stage's release
       // may only ever be for the release that comes next).
-      int put = 0, round = 0;
+      int put = 0;
+      uint32_t tiles = 0;
       bool ok = true;
       int begun[kStages];  // last item begun in each stage
       for (int i = 0; i < kStages; ++i) begun[i] = -1;
@@ -930,8 +963,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         __syncwarp();
       };
       const uint8_t* v_due = nullptr;  // the block before's V comes after this block's K
-      for (PtWork w = PtFetch(a, total, round); ok && w.valid; w = PtFetch(a, total, round)) {
-        if (w.slow) continue;
+      PtWork w;
+      while (ok && (ok = next_tile(tiles, w)) && w.valid) {
         // Q: 32 dimensions of all vectors a copy, as 128-byte swizzled rows
         // (rows of other sequences that come along are not used)
         const int sq = stage();
@@ -964,16 +997,19 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     // ------------------------------------------------------------- products
     if (PtElect()) {
       bool ok = true, due = false;  // due: O of the block before is still to come
-      int get = 0, round = 0;
-      uint32_t s_count = 0, o_count = 0, q_count = 0;
+      int get = 0;
+      uint32_t s_count = 0, o_count = 0, q_count = 0, tiles = 0;
       // The queue of products holds a few: waits for what comes next are made
       // before a group's last products are issued, so that the tensor core
       // does not run dry meanwhile.
       const auto item_ready = [&]() { return wait(full(get % kStages), (get / kStages) & 1); };
-      const auto fast = [&]() {
-        PtWork w = PtFetch(a, total, round);
-        while (w.valid && w.slow) w = PtFetch(a, total, round);
-        return w;
+      const auto next = [&](PtWork& w) {
+        w.valid = false;
+        if (!wait(listed(tiles), (tiles >> 2) & 1)) return false;
+        w = listed_tile(tiles);
+        PtArrive(taken(tiles));
+        ++tiles;
+        return true;
       };
       const auto s_part = [&](int s, bool cross) __attribute__((always_inline)) {
         const uint32_t d = tmem + kPtSCol + 128 * (s_count & 1);
@@ -1017,8 +1053,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         ++get;
         return item_ready();
       };
-      PtWork w = fast();
+      PtWork w;
       int b = 0;
+      ok = next(w);
       if (w.valid) ok = q_ready();
       while (ok && (w.valid || due)) {
         const bool more = w.valid;
@@ -1034,7 +1071,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           PtCommit(empty(sk));
           ++s_count;
           if (++b == w.nb) {
-            w = fast();
+            ok = next(w);
             b = 0;
           }
         } else {
@@ -1064,6 +1101,28 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // what was issued has read its operands before tensor memory goes back
       if (!PtWait(all_done, 0, nullptr)) give_up();
     }
+    } else if (warp == 14) {
+    // ----------------------------------------------------------------- list
+      // The CTA's tiles, up to four ahead of the roles: their look-ups take
+      // a few thousand clocks, which no other role has to wait for.
+      int round = 0;
+      bool ok = true, more = true;
+      for (uint32_t t = 0; more; ++t) {
+        PtWork w = PtFetch(a, total, round);
+        for (; w.valid && w.slow; w = PtFetch(a, total, round))
+          if (lane == 0) *slow_flag = 1;
+        if (t >= 4) ok = warp_wait(taken(t), ((t >> 2) - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) {
+          int4* at = reinterpret_cast<int4*>(base + L::kList) + 2 * (t & 3);
+          at[0] = make_int4(w.tile.row0, w.tile.rows, w.tile.sees, w.tile.block0);
+          at[1] = make_int4(w.head, w.valid ? w.nb : 0, w.partial0, 0);
+          PtArrive(listed(t));
+        }
+        __syncwarp();
+        more = w.valid;
+      }
+      if (!ok) give_up();
     }
   } else if (warp >= 8) {
     // --------------------------------------------------------------- output
@@ -1121,21 +1180,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       PtArrive(q_full(t));
       return true;
     };
-    int round = 0;
-    const auto fast = [&]() {
-      PtWork w = PtFetch(a, total, round);
-      while (w.valid && w.slow) w = PtFetch(a, total, round);
-      return w;
-    };
-    bool ok = true;
-    uint32_t n = 0, t = 0;  // blocks and tiles so far
+    uint32_t n = 0, t = 0, tiles = 0;  // blocks and tiles so far
     // (one pass before the first tile: only its Q)
-    PtWork w, next = fast();
+    PtWork w, next;
+    bool ok = next_tile(tiles, next);
     w.valid = false;
     w.nb = 1;
 #pragma unroll 1
     do {
-      if (w.valid) next = fast();
+      if (w.valid) ok = next_tile(tiles, next);
+      if (!ok) break;
       uint64_t acc[HD / 2];  // pairs of dimensions
 #pragma unroll
       for (int i = 0; i < HD / 2; ++i) acc[i] = 0;
@@ -1239,23 +1293,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const int row = v / a.group;
     const bool used = v < (kPtVectors / a.group) * a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kPtSCol + 64 * half;
-    int round = 0;
     const auto factor = [&](const PtWork& x, int block) {
       return a.factors[(static_cast<int64_t>(x.tile.block0) + block) * a.in.kv_heads + x.head].x;
     };
-    bool ok = true, some_slow = false;
-    uint32_t n = 0, t = 0;  // blocks and tiles so far
-    const auto fast = [&]() {
-      PtWork w = PtFetch(a, total, round);
-      for (; w.valid && w.slow; w = PtFetch(a, total, round)) some_slow = true;
-      return w;
-    };
-    PtWork w = fast();
+    uint32_t n = 0, t = 0, tiles = 0;  // blocks and tiles so far
+    PtWork w, next;
+    bool ok = next_tile(tiles, w);
     float f_next = w.valid ? factor(w, 0) : 0.0f;
 #pragma unroll 1
     while (w.valid) {
-      const PtWork next = fast();
-      ok = warp_wait(q_full(t), (t >> 1) & 1);
+      ok = next_tile(tiles, next) && warp_wait(q_full(t), (t >> 1) & 1);
       const float scale = scale_of[(t & 1) * kPtVectors + v];
       const int sees = used && row < w.tile.rows ? w.tile.sees + row : 0;
 #pragma unroll 1
@@ -1356,9 +1403,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       ++t;
     }
     if (!ok) give_up();
-    round = 0;
-    while (some_slow && (w = PtFetch(a, total, round)).valid)  // tiles for the CUDA cores
-      if (w.slow) PtSlowTile<HD>(a, w.tile, w.head);
+    const bool some_slow = !ok || *slow_flag != 0;
+    for (int round = 0; some_slow && (w = PtFetch(a, total, round)).valid;)
+      if (w.slow) PtSlowTile<HD>(a, w.tile, w.head);  // tiles for the CUDA cores
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
