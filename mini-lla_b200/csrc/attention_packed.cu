@@ -518,16 +518,21 @@ __global__ void __launch_bounds__(kPtSplitThreads, 2) PkSplitKernel(PtArgs a) {
   uint8_t* hi = a.images + (image * a.in.kv_heads + head) * (int64_t{8} * kPtKeys * HD) +
                 (is_v ? 4 * kPtKeys * HD : 0);
   uint8_t* lo = hi + 2 * kPtKeys * HD;
-  // 8 values a step: of one key (K) or of one dimension (V).  (512 threads of
-  // four steps: the code of 256 with eight took longer to fetch than to run.)
+  // 8 values a step, 16 bytes of an image: 8 dimensions of one key (K), 8 keys
+  // of one dimension (V: a thread's steps are neighbouring dimensions, and 8
+  // lanes side by side hold the 64 keys of an image's row, so that both the
+  // reads and the stores are whole sectors).  512 threads: the code of 256
+  // with twice the steps took longer to fetch than to run.
   constexpr int kSteps = kPtKeys * HD / 8 / kPtSplitThreads;
+  const int v_chunk = (warp & 1) * 8 + (lane & 7);                    // 8 keys
+  const int v_dim = ((warp >> 1) * 4 + (lane >> 3)) * kSteps;  // first of kSteps
   float val[kSteps][8];
   float top = 0.0f;
   int odd = 0;  // Inf or NaN
+  if (!is_v) {
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int n = i * kPtSplitThreads + threadIdx.x;
-    if (!is_v) {
+    for (int i = 0; i < kSteps; ++i) {
+      const int n = i * kPtSplitThreads + threadIdx.x;
       const int key = n / (HD / 8), c = n % (HD / 8);
       float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
       if (key < keys) {
@@ -537,24 +542,38 @@ __global__ void __launch_bounds__(kPtSplitThreads, 2) PkSplitKernel(PtArgs a) {
       }
       val[i][0] = u.x; val[i][1] = u.y; val[i][2] = u.z; val[i][3] = u.w;
       val[i][4] = w.x; val[i][5] = w.y; val[i][6] = w.z; val[i][7] = w.w;
-    } else {
-      const int d = n % HD, k0 = n / HD * 8;
-      const float* from = x + k0 * stride + d;
-      if (k0 + 8 <= keys) {
+    }
+  } else {
+    static_assert(kSteps == 2 || kSteps == 4, "one vector load a key");
+    const float* from = x + 8 * v_chunk * stride + v_dim;
 #pragma unroll
-        for (int e = 0; e < 8; ++e, from += stride) val[i][e] = *from;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e, from += stride) val[i][e] = k0 + e < keys ? *from : 0.0f;
+    for (int e = 0; e < 8; ++e, from += stride) {
+      float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (8 * v_chunk + e < keys) {
+        if constexpr (kSteps == 4) {
+          u = *reinterpret_cast<const float4*>(from);
+        } else {
+          const float2 w = *reinterpret_cast<const float2*>(from);
+          u.x = w.x;
+          u.y = w.y;
+        }
+      }
+      val[0][e] = u.x;
+      val[1][e] = u.y;
+      if constexpr (kSteps == 4) {
+        val[2][e] = u.z;
+        val[3][e] = u.w;
       }
     }
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float m = fabsf(val[i][e]);
       if (m < INFINITY) top = fmaxf(top, m);  // finite values set the scale
       else odd = 1;
     }
-  }
   top = WarpMax(top);
   odd = __any_sync(0xffffffffu, odd);
   if (lane == 0) {
@@ -584,8 +603,7 @@ __global__ void __launch_bounds__(kPtSplitThreads, 2) PkSplitKernel(PtArgs a) {
       const int key = n / (HD / 8), c = n % (HD / 8);
       at = static_cast<uint32_t>(c >> 3) * (kPtKeys * 128) + PtSwz(key, c & 7);
     } else {
-      const int d = n % HD, c = n / HD;
-      at = static_cast<uint32_t>(c >> 3) * (HD * 128) + PtSwz(d, c & 7);
+      at = static_cast<uint32_t>(v_chunk >> 3) * (HD * 128) + PtSwz(v_dim + i, v_chunk & 7);
     }
     *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
     *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -1145,7 +1163,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       constexpr int kChunks = HD / 4;
       const uint32_t stage = item % kStages;
       if (!warp_wait(full(stage), (item / kStages) & 1)) return false;
-      const bool live = used && row < w.tile.rows;
       const auto chunk = [&](int i) {  // 4 dimensions of the vector
         return *reinterpret_cast<const float4*>(base + stage * L::kItemBytes +
                                                 (i >> 3) * (kPtVectors * 128) + PtSwz(v, i & 7));
@@ -1160,14 +1177,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       top = fmaxf(top, other);
       float down;
       // (a vector with Inf or NaN has NaN outputs whatever its scale)
-      const float up = PtUp(live && top < INFINITY ? top : 0.0f, down);
+      const float up = PtUp(top < INFINITY ? top : 0.0f, down);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {  // 32 dimensions: 16 columns of each piece
         uint32_t out[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float4 y = chunk(8 * c + i);
-          if (!live) y = make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 y = chunk(8 * c + i);
           PtSplit(y.x * up, y.y * up, out[2 * i], out[16 + 2 * i]);
           PtSplit(y.z * up, y.w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
         }
@@ -1317,13 +1333,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const uint32_t s_at = lanes + 128 * (n & 1);
         const int seen = sees - b * kPtKeys - 64 * half;
         const bool whole = b < w.partial0;  // the same for every thread
-        // 32 scores; those of keys that the row does not see are -inf
-        const auto hide = [&](int c, uint32_t* s) __attribute__((always_inline)) {
-          if (!whole) {
+        // of 32 scores, those of keys that the row does not see become -inf
+        const auto hide = [&](int left, uint32_t* s) __attribute__((always_inline)) {
+          const uint32_t sees = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (32 * c + j >= seen) s[j] = 0xff800000u;
-          }
+          for (int j = 0; j < 32; ++j)
+            if ((sees & (1u << j)) == 0) s[j] = 0xff800000u;
         };
         float top;
         {
@@ -1331,8 +1346,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           PtLd32(s_at, s);
           PtLd32(s_at + 32, s + 32);
           PtLdWait(s);
-          hide(0, s);
-          hide(1, s + 32);
+          if (!whole) {  // also where they are read again below
+            hide(seen, s);
+            hide(seen - 32, s + 32);
+            PtSt32(s_at, s);
+            PtSt32(s_at + 32, s + 32);
+            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+          }
           float t0 = -INFINITY, t1 = t0, t2 = t0, t3 = t0;
 #pragma unroll
           for (int j = 0; j < 64; j += 8) {
@@ -1362,7 +1382,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         for (int c = 0; c < 2; ++c) {
           if (c != 0) PtLd32(s_at + 32, s);
           PtLdWait(s);
-          hide(c, s);
           uint32_t out[32];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
