@@ -1495,14 +1495,18 @@ int LaunchPkTc(const PtArgs& a, cudaStream_t s) {
 
 // Whether the tensor cores take a call: head size 64 or 128, and there where
 // the estimates below say that they are faster (or mlb_set_attention_path).
-// Per (row, kv head) the CUDA cores take about 2 + 1.6 G ns at head size 128,
-// once and again for every 128 keys, behind 5 us; the tensor cores take 12 us
-// (17 at head size 128) and 85 ns to split an image of 128 keys, the rest
-// being small where the two are close.  Measured on B200, tensor cores /
-// CUDA cores, us: 32 / 8 heads x 128, 1 sequence of 64 rows 20 / 11, of 128
-// 21 / 26; 64 of 8 rows 61 / 34, of 16 67 / 67, of 32 77 / 172; 32 / 32
-// heads, 64 of 16 204 / 128, of 32 232 / 427; 14 / 2 heads x 64, 1 of 128 14 /
-// 10, of 256 15 / 25, 16 of 32 16 / 15; 28 / 4 heads x 128, 4 of 64 22 / 22.
+// In us, with the average sequence's keys counted in blocks of 128: the CUDA
+// cores take 4 for each step of a row through its keys, and per thousand
+// (row, kv head) pairs 1.5 and, at head size 128, 1.2 per query head, 8 per
+// block (its K and V) and 1.8 per block and query head; the tensor cores take
+// 6 (12 at head size 128), 1.6 per block and 64 per thousand images of 128
+// keys (one kv head; split and used), the rest being small where the two are
+// close.  Over 180 shapes measured on B200 the choice is at most 10 % off the
+// faster one.  Tensor cores / CUDA cores, us, without earlier tokens: 32 / 8
+// heads x 128, 1 sequence of 64 rows 15 / 11, of 128 17 / 25; 64 of 8 rows 51 / 34, of
+// 16 53 / 67; 32 / 32 heads, 64 of 16 179 / 131; 14 / 2 heads x 64, 1 of 128 12 / 10,
+// of 256 13 / 24; after 512 tokens: 32 / 8 heads, 1 of 8 23 / 29, 14 / 2 heads x 64,
+// 64 of 8 36 / 94.
 bool TakesTc(int64_t q_rows, int64_t k_rows, int64_t n_seqs, int n_heads, int kv_heads, int hd) {
   if (hd != 64 && hd != 128) return false;
   const int group = n_heads / kv_heads;
@@ -1510,11 +1514,12 @@ bool TakesTc(int64_t q_rows, int64_t k_rows, int64_t n_seqs, int n_heads, int kv
   if (q_rows == 0 || k_rows == 0 || n_seqs == 0 || tiles * kv_heads > INT_MAX) return false;
   const int path = mlb_attention_path();
   if (path != 0) return path == 2;
-  const double images = static_cast<double>(k_rows / kPtKeys + n_seqs) * kv_heads;
-  const double tc = (hd == 128 ? 17e3 : 12e3) + images * 85.0 * hd / 128;
-  const double steps = 1.0 + static_cast<double>(k_rows) / n_seqs / 128;
-  const double rows =
-      5e3 + static_cast<double>(q_rows) * kv_heads * (2.0 + 1.6 * group) * hd / 128 * steps;
+  const double h = hd / 128.0, keys = static_cast<double>(k_rows) / n_seqs / 128;
+  const double pairs = 1e-3 * static_cast<double>(q_rows) * kv_heads;
+  const double images = 1e-3 * static_cast<double>(k_rows / kPtKeys + n_seqs) * kv_heads;
+  const double tc = 6 + 6 * h + 1.6 * (1 + keys) + 64 * images * h;
+  const double rows = 4 * (1 + keys) +
+                      pairs * (1.5 + h * (1.2 * group + 8 * keys + 1.8 * group * keys));
   return tc < rows;
 }
 
