@@ -217,28 +217,34 @@ __global__ void __launch_bounds__(kKv8Threads, NI == 1 ? 4 : NI == 2 ? 3 : 1) Kv
     for (int n = 0; n < NI; ++n) {
       const int i = n * kKv8Threads + threadIdx.x;
       const int q = i / per, r = i - q * per;
+      const int t0 = which == 0 ? q : 16 * q, t1 = which == 0 ? q : 16 * q + 15;
+      // most warps of a block that gets one token have no new value at all
+      const bool has_new = i < items && t1 >= s.first && t0 < s.first + s.count;
+      if (!has_new) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[n][j] = 0.0f;
+        continue;
+      }
+      const int t = t0 - s.first;
       if (which == 0) {
-        const int t = q - s.first;
-        const bool in = i < items && t >= 0 && t < s.count;
         const float4* from = reinterpret_cast<const float4*>(x + t * row_stride + 16 * r);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float4 y = in ? LoadStream(from + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 y = LoadStream(from + j);
           v[n][4 * j] = y.x;
           v[n][4 * j + 1] = y.y;
           v[n][4 * j + 2] = y.z;
           v[n][4 * j + 3] = y.w;
         }
       } else {
-        const int t = 16 * q - s.first;
         const float* from = x + t * row_stride + r;
-        if (whole && i < items) {
+        if (whole) {
 #pragma unroll
           for (int j = 0; j < 16; ++j, from += row_stride) v[n][j] = __ldcs(from);
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j, from += row_stride)
-            v[n][j] = i < items && t + j >= 0 && t + j < s.count ? __ldcs(from) : 0.0f;
+            v[n][j] = t + j >= 0 && t + j < s.count ? __ldcs(from) : 0.0f;
         }
       }
 #pragma unroll
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(kKv8Threads, NI == 1 ? 4 : NI == 2 ? 3 : 1) Kv
       if (t1 < s.first && !moved && usable) continue;  // earlier codes under the same scale
       uint4* to = codes + (which == 0 ? i : r * (B >> 4) + q);
       uint4 w = make_uint4(0, 0, 0, 0);
-      if (usable) {
+      if (usable && t1 >= s.first && t0 < s.first + s.count) {
         // (0 where there is no new value)
         float worst = 0.0f;
         float t[16];
@@ -283,14 +289,14 @@ __global__ void __launch_bounds__(kKv8Threads, NI == 1 ? 4 : NI == 2 ? 3 : 1) Kv
         }
         w = make_uint4(LowBytes(t[0], t[1], t[2], t[3]), LowBytes(t[4], t[5], t[6], t[7]),
                        LowBytes(t[8], t[9], t[10], t[11]), LowBytes(t[12], t[13], t[14], t[15]));
-        if (t0 < s.first) {
-          uint4 old = *to;
-          if (moved) old = Moved(old, had, scale, ratio);
-          // bytes of the places before the first new one: all of them in K
-          const int n_old = which == 0 ? 16 : s.first - t0;
-          w = make_uint4(Merge(old.x, w.x, n_old), Merge(old.y, w.y, n_old - 4),
-                         Merge(old.z, w.z, n_old - 8), Merge(old.w, w.w, n_old - 12));
-        }
+      }
+      if (usable && t0 < s.first) {
+        uint4 old = *to;
+        if (moved) old = Moved(old, had, scale, ratio);
+        // bytes of the places before the first new one: all of them in K
+        const int n_old = which == 0 ? 16 : s.first - t0;
+        w = make_uint4(Merge(old.x, w.x, n_old), Merge(old.y, w.y, n_old - 4),
+                       Merge(old.z, w.z, n_old - 8), Merge(old.w, w.w, n_old - 12));
       }
       *to = w;
     }
