@@ -383,10 +383,14 @@ Kv8Rows RowsOf(const int32_t* table, const int32_t* offsets, const int32_t* posi
   Kv8Rows a{table, offsets, positions, table_cols, n_blocks, static_cast<int>(rows),
             static_cast<int>(n_seqs), block, block == 32 ? 5 : block == 64 ? 6 : 7, kv_heads,
             1, hd, status};
-  // A CTA finds its block once for several heads where the grid stays above
-  // 16 CTAs per SM: in a decode step each head has its own CTA.
+  // A CTA finds its block once for several heads: for two where that leaves 8
+  // CTAs per SM, for more where it leaves 16.  (200 sequences' tokens written
+  // and read back 42.5 us with two heads a CTA, 48 with one; 32 prompts of up to
+  // 4,100 tokens 400 us with eight, 447 with two; 8 such prompts 86 us with four,
+  // 92 with eight.)
   const int64_t ctas = 2 * MostTouched(rows, n_seqs, block) * kv_heads;
-  while (a.heads < kv_heads && ctas / (2 * a.heads) >= 16 * SmCount()) a.heads *= 2;
+  while (a.heads < kv_heads && ctas / (2 * a.heads) >= (a.heads == 1 ? 8 : 16) * SmCount())
+    a.heads *= 2;
   return a;
 }
 dim3 GridOf(const Kv8Rows& a) {
