@@ -16,7 +16,6 @@ namespace mlb {
 namespace {
 
 constexpr int kKv8Threads = 256;
-constexpr int kKv8Warps = kKv8Threads / 32;
 
 // What a CTA works on: columns of the table that the rows of packed
 // sequences touch, counted through all sequences.
@@ -186,12 +185,13 @@ struct Kv8WriteArgs {
 // side by side: 16 dimensions of a token in K, 16 tokens of a dimension in V
 // (neighbouring lanes neighbouring dimensions, so that a row of new values is
 // read in full lines); a thread holds NI items in registers from the maximum
-// to the codes.
-template <int NI>
-__global__ void __launch_bounds__(kKv8Threads, NI == 1 ? 4 : NI == 2 ? 3 : 1) Kv8WriteKernel(Kv8WriteArgs a) {
+// to the codes.  T threads, so many that NI is 1 for all but the largest
+// blocks, and 1024 threads share an SM.
+template <int T, int NI>
+__global__ void __launch_bounds__(T, 1024 / T) Kv8WriteKernel(Kv8WriteArgs a) {
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
-  __shared__ uint32_t top_of[2][kKv8Warps];
+  __shared__ uint32_t top_of[2][T / 32];
   const Kv8Span s = FindSpan(a.at, blockIdx.x);
   if (s.block < 0 || s.count == 0) return;
   const int which = blockIdx.z;
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kKv8Threads, NI == 1 ? 4 : NI == 2 ? 3 : 1) Kv
     const bool whole = s.count == B;
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
-      const int i = n * kKv8Threads + threadIdx.x;
+      const int i = n * T + threadIdx.x;
       const int q = i / per, r = i - q * per;
       const int t0 = which == 0 ? q : 16 * q, t1 = which == 0 ? q : 16 * q + 15;
       // most warps of a block that gets one token have no new value at all
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kKv8Threads, NI == 1 ? 4 : NI == 2 ? 3 : 1) Kv
     if ((threadIdx.x & 31) == 0) top_of[turn][threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kKv8Warps; ++w) top = max(top, top_of[turn][w]);
+    for (int w = 0; w < T / 32; ++w) top = max(top, top_of[turn][w]);
     const float fresh = __fdiv_rn(__uint_as_float(top), 127.0f);
     const float scale =
         __float_as_uint(fresh) > (__float_as_uint(had) & 0x7fffffffu) ? fresh : had;
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kKv8Threads, NI == 1 ? 4 : NI == 2 ? 3 : 1) Kv
     const float inv = 1.0f / scale, hs = 0.5f * scale, ratio = had / scale;
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
-      const int i = n * kKv8Threads + threadIdx.x;
+      const int i = n * T + threadIdx.x;
       if (i >= items) break;
       const int q = i / per, r = i - q * per;
       // places of the item's tokens: the same for all in K, 16 in a row in V
@@ -596,12 +596,11 @@ extern "C" int mlb_kv8_write_f32(int8_t* k_codes, int8_t* v_codes, float* k_scal
   a.k = k;
   a.v = v;
   const dim3 grid = GridOf(a.at);
-  const int items = (block_tokens * head_dim / 16 + kKv8Threads - 1) / kKv8Threads;
-  Launch(items <= 1   ? Kv8WriteKernel<1>
-         : items <= 2 ? Kv8WriteKernel<2>
-         : items <= 4 ? Kv8WriteKernel<4>
-                      : Kv8WriteKernel<8>,
-         grid, kKv8Threads, 0, AsStream(stream), a);
+  const int items = block_tokens * head_dim / 16;
+  if (items <= 256) Launch(Kv8WriteKernel<256, 1>, grid, 256, 0, AsStream(stream), a);
+  else if (items <= 512) Launch(Kv8WriteKernel<512, 1>, grid, 512, 0, AsStream(stream), a);
+  else if (items <= 1024) Launch(Kv8WriteKernel<1024, 1>, grid, 1024, 0, AsStream(stream), a);
+  else Launch(Kv8WriteKernel<1024, 2>, grid, 1024, 0, AsStream(stream), a);
   return CheckLaunch("mlb_kv8_write_f32");
 }
 
