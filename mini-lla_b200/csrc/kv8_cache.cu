@@ -7,6 +7,11 @@
 //   new code = round(x / s'), earlier code = round(c s / s')
 // Both quotients are rounded as if they were exact, so the codes depend on
 // nothing but the definition.
+//
+// Bound: HBM for whole prompts (8 of 858 to 4,100 tokens, 8 kv heads x 128:
+// written and read back in 86 us, 403 MB, 72 % of the measured copy rate); for
+// one token of each of 64 sequences the look-ups of offsets, table and block,
+// one after another (14.5 us, of which the bytes are 2.6).
 #include <climits>
 #include <cstdint>
 
@@ -440,7 +445,8 @@ __device__ __forceinline__ uint32_t MassKey(float m) {
 // then closes up ids and masses.  T is the power of two from 128 to 1024 that
 // covers the table's columns: a table of 90 blocks is done by 4 warps, whose
 // barriers are cheap, and every pass over its keys is one step; the first
-// kHeld steps' keys stay in registers.
+// kHeld steps' keys stay in registers.  Bound: the barriers of four digits
+// and of closing up: one table of 90 columns 3.7 us, 64 of 2,000 9.8 us.
 template <int T>
 __global__ void __launch_bounds__(T) EvictKernel(EvictArgs a) {
   LaunchWait();  // the previous kernel on the stream has completed
