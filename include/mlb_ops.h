@@ -523,9 +523,10 @@ int64_t mlb_attention_kv8_scratch_floats(int64_t n_seqs, int64_t table_cols,
  * error and places behind the last block get mass_in unchanged).
  * scratch: at least mlb_attention_kv8_scratch_floats(...) floats, 16-byte
  * aligned; calls that may overlap on the GPU need scratch of their own.  out
- * overlaps neither q nor the pool.  Deterministic.  Queries and weights are
- * taken in 22 bits, all sums in fp32: within 1e-5 * sum_t w_t |v_t| of the
- * exact result over the cache's values for scores of ordinary spread.
+ * overlaps neither q nor the pool.  Deterministic.  Queries are rounded to
+ * 2^-30 of the row's largest value, weights to 22 bits, sums are fp32 or exact:
+ * within 1e-5 * sum_t w_t |v_t| of the exact result over the cache's values
+ * for scores of ordinary spread.
  */
 int mlb_attention_kv8_f32(const float* q, const int8_t* k_codes,
                           const int8_t* v_codes, const float* k_scales,

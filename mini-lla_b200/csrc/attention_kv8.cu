@@ -13,15 +13,19 @@
 // one long sequence and many short ones both keep every SM busy, whatever
 // the lengths, which only the device knows.
 //
-// Products.  Both run as mma.m16n8k16 (fp16 operands, fp32 sums) with the
-// 8-bit codes as exact fp16 numbers.  q, scaled per head by a power of two
-// that brings its largest value to [2^14, 2^15), and p, times 2^14, are split
-// into two fp16 pieces each (at most 2^-22 of the value is left, or 2^-39 of
-// the row's largest); the high pieces of up to 8 heads are the tile's rows
-// 0-7, the low ones its rows 8-15, so one MMA takes both and a thread holds
-// both sums of its (head, column).  The scales of a unit multiply its scores
-// and its weighted values in fp32; a unit's values are summed from zero and
-// then added to the running accumulator by one fp32 multiply-add.
+// Products.  q k^T runs as mma.m16n8k32 on 8-bit integers with the codes as
+// they are: q, scaled per head by a power of two that brings its largest value
+// to [2^29, 2^30) and rounded to an integer (2^-30 of the row's largest, or
+// fp32's own step), is four signed 8-bit digits.  The upper digits of a pair are
+// the tile's rows 0-7, one for each of up to 8 heads, the lower ones its rows
+// 8-15, so two MMAs take all four and a thread holds both sums of its (head,
+// column); all sums are exact.  P V runs as mma.m16n8k16 (fp16 operands, fp32
+// sums) with the codes as exact fp16 numbers and p, times 2^14, in two fp16
+// pieces (at most 2^-22 of the value is left, or 2^-39 of 1), high pieces in
+// rows 0-7, low ones in rows 8-15: a p's digits would all be of one size, where
+// the pieces follow the p.  The scales of a unit multiply its scores and its
+// weighted values in fp32; a unit's values are summed from zero and then added
+// to the running accumulator by one fp32 multiply-add.
 //
 // Layout.  Column n of score tile j is the unit's token 8 (n / 2) + 2 j +
 // n % 2: a thread (lane = 4 row + c) then holds the scores of tokens 8 c ..
@@ -33,13 +37,14 @@
 // products, each warp on its own.
 //
 // Bound: HBM reads of 2 hd bytes per token and kv head; as built the
-// instructions between them (half of the issue slots are taken, by two warps a
-// scheduler: the codes' conversion, the softmax and 16 MMAs a unit each way).
-// 64 sequences of 17 to 4,000 tokens, 32 / 8 heads x 128, with the collected
-// weights: 72 us, 3.7 TB/s of codes or 58 % of the measured copy rate (first
-// kernel 64 us, the join 6, the weights 3); the copies alone take 61 us.
-// 16 sequences, 32 / 32 heads: 48 us, 53 %.  One sequence of 16,383 tokens: 19.5
-// us; one of 511, 14 / 2 heads x 64: 7.0 us, both launch and latency.
+// instructions between them (about half of the issue slots are taken, by two
+// warps a scheduler: V's conversion, the softmax and 64 MMAs a unit).  64
+// sequences of 141 to 4,000 tokens, 32 / 8 heads x 128, with the collected
+// weights: 70 us, 3.8 TB/s of codes or 59 % of the measured copy rate (the join
+// about 6 of them, the weights 3); the copies alone take 61 us.  (With q in fp16
+// pieces and K's codes converted, too, 72 us.)  16 sequences, 32 / 32 heads: 46
+// us, 55 %.  One sequence of 16,383 tokens: 19 us; one of 511, 14 / 2 heads x
+// 64: 7.1 us, both launch and latency.
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -97,6 +102,14 @@ __device__ __forceinline__ void Mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       " {%8, %9}, {%0, %1, %2, %3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same for 32 8-bit integers a row, exact.
+__device__ __forceinline__ void MmaCodes(int (&d)[4], const uint4& a, const uint2& b) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+      " {%8, %9}, {%0, %1, %2, %3};\n"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y));
 }
 
 // Four codes -> two fp16 pairs (codes 0, 1 and 2, 3), exact: with the sign bit
@@ -178,7 +191,7 @@ struct A8Smem {
   static constexpr int kKBytes = kUnit * kKPitch;
   static constexpr int kStageBytes = kKBytes + HD * kUnit + 16;  // K, V, the two scales
   static constexpr int kStages = 2;
-  static constexpr int kQBytes = (HD / 16) * 32 * 16;  // A operand of the scores
+  static constexpr int kQBytes = (HD / 16) * 32 * 16;  // A operands of the scores
   static constexpr int kBytes = kA8Warps * (kStages * kStageBytes + kQBytes);
   // CTAs that fit an SM's shared memory (1 KB of each is the system's)
   static constexpr int kFit = 228 * 1024 / (kBytes + 1024 + 256);
@@ -197,7 +210,7 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = lane >> 2, c = lane & 3;  // head of the group / column; quarter
   uint8_t* ring = a8_raw + warp * (kStages * S::kStageBytes + S::kQBytes);
-  uint4* qf = reinterpret_cast<uint4*>(ring + kStages * S::kStageBytes) + lane;  // [k16 step][lane]
+  uint4* qf = reinterpret_cast<uint4*>(ring + kStages * S::kStageBytes) + lane;  // [32 dimensions][digits][lane]
 
   // all units, and the place where this warp's share begins (each warp on its
   // own: the lengths come from L2 once and then from L1)
@@ -303,7 +316,7 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
     const int ahead = (stage + kStages - 1) % kStages;
     if (n + kStages - 1 < count) copy(ahead);
     CopyAsyncCommit();
-    if (fresh) {  // q of a new (sequence, kv head): scaled and split
+    if (fresh) {  // q of a new (sequence, kv head): scaled and in digits
       fresh = false;
       bad = false;
       first_unit = get.unit;
@@ -312,7 +325,7 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
 #pragma unroll
       for (int i = 0; i < DT; ++i) acc[i][0] = acc[i][1] = 0.0f;
       float x[DC][8];
-      float top = 0.0f;
+      uint32_t top = 0;  // magnitudes as integers: NaN above Inf above every number
       const float4* q = reinterpret_cast<const float4*>(
           a.q + (static_cast<int64_t>(get.seq) * a.n_heads + get.head * a.group + row) * HD);
 #pragma unroll
@@ -325,25 +338,36 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
         x[j][0] = u.x; x[j][1] = u.y; x[j][2] = u.z; x[j][3] = u.w;
         x[j][4] = w.x; x[j][5] = w.y; x[j][6] = w.z; x[j][7] = w.w;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[j][e]));
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[j][e]) & 0x7fffffffu);
       }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^(14 - e) for a largest value in [2^e, 2^(e + 1)); 1 for a row of
-      // zeros or with an infinity, whose outputs are NaN whatever it is
-      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-      e = top == 0.0f || e == 128 ? 14 : max(e, -100);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
-      factor = a.scale * __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^(29 - e) for a largest value in [2^e, 2^(e + 1))
+      const int e = max(static_cast<int>(top >> 23) - 127, -97);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 29 - e) << 23);
+      factor = a.scale * __uint_as_float(static_cast<uint32_t>(127 - 29 + e) << 23);
+      if (top >= 0x7f800000u) factor = NAN;  // Inf or NaN in q
 #pragma unroll
-      for (int j = 0; j < DC; ++j)
+      for (int j = 0; j < DC; ++j) {
+        uint32_t digit[2][4];  // [dimensions 0-3, 4-7][digit, lowest first]
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          uint4 a;
-          SplitPair(x[j][4 * s] * up, x[j][4 * s + 1] * up, a.x, a.y);
-          SplitPair(x[j][4 * s + 2] * up, x[j][4 * s + 3] * up, a.z, a.w);
-          qf[32 * (2 * j + s)] = a;  // read by this lane only
+          uint32_t d[4];  // a value's four signed digits, a byte each
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            d[k] = (static_cast<uint32_t>(__float2int_rn(x[j][4 * s + k] * up)) + 0x00808080u) ^
+                   0x00808080u;
+          const uint32_t a01 = __byte_perm(d[0], d[1], 0x5140), b01 = __byte_perm(d[0], d[1], 0x7362);
+          const uint32_t a23 = __byte_perm(d[2], d[3], 0x5140), b23 = __byte_perm(d[2], d[3], 0x7362);
+          digit[s][0] = __byte_perm(a01, a23, 0x5410);
+          digit[s][1] = __byte_perm(a01, a23, 0x7632);
+          digit[s][2] = __byte_perm(b01, b23, 0x5410);
+          digit[s][3] = __byte_perm(b01, b23, 0x7632);
         }
+        // read by this lane only
+        qf[64 * j] = make_uint4(digit[0][3], digit[0][2], digit[1][3], digit[1][2]);
+        qf[64 * j + 32] = make_uint4(digit[0][1], digit[0][0], digit[1][1], digit[1][0]);
+      }
     }
     CopyAsyncWait<kStages - 1>();
     __syncwarp();  // all lanes' copies of this unit have landed
@@ -355,30 +379,26 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
       // scores of the 4 column tiles
       float sc[8];
       {
-        float d[4][4] = {};
+        int high[4][4] = {}, low[4][4] = {};  // [tile][two columns: upper digit, lower digit]
 #pragma unroll
         for (int g = 0; g < DC; ++g) {
           uint2 w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            w[j] = *reinterpret_cast<const uint2*>(kt + (8 * j + row) * S::kKPitch + 32 * g +
-                                                   8 * c);
+            w[j] = *reinterpret_cast<const uint2*>(kt + (8 * j + row) * S::kKPitch + 32 * g + 8 * c);
+          const uint4 q1 = qf[64 * g], q0 = qf[64 * g + 32];
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const uint4 q = qf[32 * (2 * g + s)];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t b0, b1;
-              CodePairs(s == 0 ? w[j].x : w[j].y, b0, b1);
-              Mma(d[j], q.x, q.y, q.z, q.w, b0, b1);
-            }
+          for (int j = 0; j < 4; ++j) {
+            MmaCodes(high[j], q1, w[j]);
+            MmaCodes(low[j], q0, w[j]);
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          sc[2 * j] = (d[j][0] + d[j][2]) * ks;
-          sc[2 * j + 1] = (d[j][1] + d[j][3]) * ks;
-        }
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            sc[2 * j + k] = fmaf(static_cast<float>(high[j][k] * 256 + high[j][2 + k]), 65536.0f,
+                                 static_cast<float>(low[j][k] * 256 + low[j][2 + k])) * ks;
       }
       const int left = get.length - get.unit * kUnit;  // tokens of the unit, if < 32
       if (left < kUnit) {

@@ -15,8 +15,12 @@ with 2^-20 for exp (2 steps), the pieces of p and v (2^-22 each) and the
 division, and one step for each addition in a row: at most n / 4 + 64 (a warp
 adds every fourth key; partial sums of tiles and slices are fewer).  The last
 term is p's 2^-39 with each key's value and v's 2^-39 with a weight of at most
-1; it also covers weights and products below fp32's range (2^-126).  Codes,
-scales, tables and lengths are exact.
+1; it also covers weights and products below fp32's range (2^-126).  The decode
+kernel takes q as integers instead, off by at most 2^-31 of the row's largest
+value, and sums them exactly: 2^-31 max|q| sum_d |k_d| is below the unused
+hd 2^-23 sum_d |q_d k_d| wherever the latter sum is at least 2^-8 / hd max|q|
+sum_d |k_d|, as with the queries here (one dimension at most a few hundred
+times the others).  Codes, scales, tables and lengths are exact.
 """
 import ctypes
 
