@@ -40,9 +40,9 @@
 // instructions between them (about half of the issue slots are taken, by two
 // warps a scheduler: V's conversion, the softmax and 64 MMAs a unit).  64
 // sequences of 141 to 4,000 tokens, 32 / 8 heads x 128, with the collected
-// weights: 70 us, 3.8 TB/s of codes or 59 % of the measured copy rate (the join
-// about 6 of them, the weights 3); the copies alone take 61 us.  (With q in fp16
-// pieces and K's codes converted, too, 72 us.)  16 sequences, 32 / 32 heads: 46
+// weights: 67.6 us, 4.0 TB/s of codes or 61 % of the measured copy rate (the
+// join about 4 of them, the weights 3); the copies alone take 61 us.  (With q in
+// fp16 pieces and K's codes converted, too, 2.2 us more.)  16 sequences, 32 / 32 heads: 46
 // us, 55 %.  One sequence of 16,383 tokens: 19 us; one of 511, 14 / 2 heads x
 // 64: 7.1 us, both launch and latency.
 #include <cfloat>
@@ -498,12 +498,10 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
 
 // Joins the partials of a (sequence, query head): out = sum_w acc_w f_w / sum_w
 // l_w f_w, f_w = 2^(m_w - M).  CTA = (query head, sequence); every eighth
-// partial is a warp's, which joins them to a state of its own, headers by
-// lanes, rows 16 bytes a lane, all loads under way together; the warps' states
-// meet in shared memory after the only barrier.
-constexpr int kJoinWarps = 8;
-
-template <int V>  // float4 of a row per lane
+// partial (fourth, for many pairs) is a warp's, which joins them to a state of
+// its own, headers by lanes, rows 16 bytes a lane, all loads under way together;
+// the warps' states meet in shared memory after the only barrier.
+template <int V, int kJoinWarps>  // float4 of a row per lane
 __global__ void __launch_bounds__(kJoinWarps * 32) A8JoinKernel(A8Args a) {
   LaunchWait();  // the previous kernel on the stream has completed
   LaunchNext();
@@ -755,9 +753,15 @@ extern "C" int mlb_attention_kv8_f32(const float* q, const int8_t* k_codes, cons
     }
     if (rc != MLB_OK) return rc;
   }
-  Launch(head_dim <= 128 ? A8JoinKernel<1> : A8JoinKernel<2>,
-         dim3(static_cast<unsigned>(n_heads), static_cast<unsigned>(n_seqs)), kJoinWarps * 32, 0, s,
-         a);
+  // Many pairs have a few partials each: four warps a CTA, so that more CTAs run
+  // at once (64 sequences, 32 heads: 67.6 us for the whole call, 70.0 with eight).
+  // Few pairs may have a hundred each: eight.
+  const bool many = n_seqs * n_heads > int64_t{8} * SmCount();
+  const dim3 pairs(static_cast<unsigned>(n_heads), static_cast<unsigned>(n_seqs));
+  if (many)
+    Launch(head_dim <= 128 ? A8JoinKernel<1, 4> : A8JoinKernel<2, 4>, pairs, 32 * 4, 0, s, a);
+  else
+    Launch(head_dim <= 128 ? A8JoinKernel<1, 8> : A8JoinKernel<2, 8>, pairs, 256, 0, s, a);
   if (mass_out != nullptr && table_cols > 0)
     Launch(A8MassKernel, dim3(static_cast<unsigned>((table_cols + 7) / 8),
                               static_cast<unsigned>(n_seqs)),
