@@ -275,7 +275,7 @@ void LaunchPkRows(const PkArgs& a, cudaStream_t s) {
 // all of such a block, a row that does not see it would still meet it as 0 *
 // NaN, so that tile is computed on the CUDA cores.
 //
-// Bound: 6 products of 2 * 128 * 128 * hd flops for 128 vectors and keys, 3072
+// Bound: 6 products of 2 * 128 * 128 * hd flops for 128 vectors and keys, 48 x 64
 // clocks at head size 128; a block takes about 3400.  Four documents of 2,462
 // to 5,000 rows (32 / 8 heads x 128): 1.44 to 1.52 ms, 563 GFLOP of attention or
 // 1.1 to 1.2 PFLOP/s of fp16 products, 80 to 84 % of the sustained rate of a
@@ -352,16 +352,6 @@ __device__ __forceinline__ float PtUp(float top, float& down) {
   return __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
 }
 
-// Two values -> their high fp16 pieces and what is left, again in fp16.
-__device__ __forceinline__ void PtSplit(float x, float y, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(hi) : "f"(y), "f"(x));
-  float hx, hy;
-  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n cvt.f32.f16 %1, b;\n}\n"
-      : "=f"(hx), "=f"(hy)
-      : "r"(hi));
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(lo) : "f"(y - hy), "f"(x - hx));
-}
-
 // Packed pairs of fp32 (one instruction each).
 __device__ __forceinline__ uint64_t PtPair(float x, float y) {
   uint64_t p;
@@ -385,6 +375,17 @@ __device__ __forceinline__ uint64_t PtAdd2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+// Two values -> their high fp16 pieces and what is left, again in fp16.
+__device__ __forceinline__ void PtSplit(uint64_t xy, uint32_t& hi, uint32_t& lo) {
+  float x, y;
+  PtUnpair(xy, x, y);
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(hi) : "f"(y), "f"(x));
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n cvt.f32.f16 %1, b;\n}\n"
+      : "=f"(x), "=f"(y)
+      : "r"(hi));
+  PtUnpair(PtFma2(PtPair(x, y), PtPair(-1.0f, -1.0f), xy), x, y);
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(lo) : "f"(y), "f"(x));
 }
 __device__ __forceinline__ float PtMax3(float a, float b, float c) {
   float d;
@@ -580,14 +581,25 @@ __global__ void __launch_bounds__(kPtSplitThreads, 2) PkSplitKernel(PtArgs a) {
       }
     }
   }
+  float zero = 0.0f;  // NaN where a value is not finite
 #pragma unroll
   for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float m = fabsf(val[i][e]);
-      if (m < INFINITY) top = fmaxf(top, m);  // finite values set the scale
-      else odd = 1;
+    for (int e = 0; e < 8; e += 2) {
+      top = PtMax3(top, fabsf(val[i][e]), fabsf(val[i][e + 1]));
+      zero = fmaf(val[i][e], 0.0f, fmaf(val[i][e + 1], 0.0f, zero));
     }
+  if (zero != zero) {  // finite values set the scale
+    odd = 1;
+    top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float m = fabsf(val[i][e]);
+        if (m < INFINITY) top = fmaxf(top, m);
+      }
+  }
   top = WarpMax(top);
   odd = __any_sync(0xffffffffu, odd);
   if (lane == 0) {
@@ -602,6 +614,7 @@ __global__ void __launch_bounds__(kPtSplitThreads, 2) PkSplitKernel(PtArgs a) {
   }
   float down;
   const float up = PtUp(top, down);
+  const uint64_t up2 = PtPair(up, up);
   if (threadIdx.x == 0) {
     float* f = reinterpret_cast<float*>(a.factors + image * a.in.kv_heads + head);
     f[is_v ? 1 : 0] = is_v && odd ? -down : down;
@@ -611,7 +624,8 @@ __global__ void __launch_bounds__(kPtSplitThreads, 2) PkSplitKernel(PtArgs a) {
     const int n = i * kPtSplitThreads + threadIdx.x;
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) PtSplit(val[i][2 * e] * up, val[i][2 * e + 1] * up, h[e], l[e]);
+    for (int e = 0; e < 4; ++e)
+      PtSplit(PtMul2(PtPair(val[i][2 * e], val[i][2 * e + 1]), up2), h[e], l[e]);
     uint32_t at;
     if (!is_v) {
       const int key = n / (HD / 8), c = n % (HD / 8);
@@ -1192,14 +1206,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       float down;
       // (a vector with Inf or NaN has NaN outputs whatever its scale)
       const float up = PtUp(top < INFINITY ? top : 0.0f, down);
+      const uint64_t up2 = PtPair(up, up);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {  // 32 dimensions: 16 columns of each piece
         uint32_t out[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float4 y = chunk(8 * c + i);
-          PtSplit(y.x * up, y.y * up, out[2 * i], out[16 + 2 * i]);
-          PtSplit(y.z * up, y.w * up, out[2 * i + 1], out[16 + 2 * i + 1]);
+          PtSplit(PtMul2(PtPair(y.x, y.y), up2), out[2 * i], out[16 + 2 * i]);
+          PtSplit(PtMul2(PtPair(y.z, y.w), up2), out[2 * i + 1], out[16 + 2 * i + 1]);
         }
         PtSt16(lanes + kPtQCol + 16 * c, out);
         PtSt16(lanes + kPtQCol + 16 * c + HD / 2, out + 16);
@@ -1408,17 +1423,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             const uint64_t p = PtPair(p0, p1);
             if ((i & 1) == 0) sum_a = PtAdd2(sum_a, p);
             else sum_b = PtAdd2(sum_b, p);
-            uint32_t hi, lo;
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(hi) : "f"(p1), "f"(p0));
-            float h0, h1;
-            asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n"
-                " cvt.f32.f16 %1, b;\n}\n"
-                : "=f"(h0), "=f"(h1)
-                : "r"(hi));
-            PtUnpair(PtFma2(PtPair(h0, h1), PtPair(-1.0f, -1.0f), p), h0, h1);
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(lo) : "f"(h1), "f"(h0));
-            out[i] = hi;
-            out[16 + i] = lo;
+            PtSplit(p, out[i], out[16 + i]);
           }
           PtSt32(s_at + 32 * c, out);
         }
