@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = lane >> 2, c = lane & 3;  // head of the group / column; quarter
   uint8_t* ring = a8_raw + warp * (kStages * S::kStageBytes + S::kQBytes);
-  uint4* qf = reinterpret_cast<uint4*>(ring + kStages * S::kStageBytes) + lane;  // [32 dimensions][digits][lane]
+  // [32 dimensions][upper, lower digits][lane]
+  uint4* qf = reinterpret_cast<uint4*>(ring + kStages * S::kStageBytes) + lane;
 
   // all units, and the place where this warp's share begins (each warp on its
   // own: the lengths come from L2 once and then from L1)
@@ -284,7 +285,8 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
       uint8_t* vt = to + S::kKBytes;
       if (a.block == kUnit) {
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) CopyAsync16(vt + 16 * (32 * i + lane), v + 16 * (32 * i + lane));
+        for (int i = 0; i < HD / 16; ++i)
+          CopyAsync16(vt + 16 * (32 * i + lane), v + 16 * (32 * i + lane));
       } else {
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
@@ -357,8 +359,10 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
           for (int k = 0; k < 4; ++k)
             d[k] = (static_cast<uint32_t>(__float2int_rn(x[j][4 * s + k] * up)) + 0x00808080u) ^
                    0x00808080u;
-          const uint32_t a01 = __byte_perm(d[0], d[1], 0x5140), b01 = __byte_perm(d[0], d[1], 0x7362);
-          const uint32_t a23 = __byte_perm(d[2], d[3], 0x5140), b23 = __byte_perm(d[2], d[3], 0x7362);
+          const uint32_t a01 = __byte_perm(d[0], d[1], 0x5140);
+          const uint32_t b01 = __byte_perm(d[0], d[1], 0x7362);
+          const uint32_t a23 = __byte_perm(d[2], d[3], 0x5140);
+          const uint32_t b23 = __byte_perm(d[2], d[3], 0x7362);
           digit[s][0] = __byte_perm(a01, a23, 0x5410);
           digit[s][1] = __byte_perm(a01, a23, 0x7632);
           digit[s][2] = __byte_perm(b01, b23, 0x5410);
@@ -385,7 +389,8 @@ __global__ void __launch_bounds__(kA8Warps * 32, A8Smem<HD>::kCtasPerSm) A8Kerne
           uint2 w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            w[j] = *reinterpret_cast<const uint2*>(kt + (8 * j + row) * S::kKPitch + 32 * g + 8 * c);
+            w[j] = *reinterpret_cast<const uint2*>(kt + (8 * j + row) * S::kKPitch + 32 * g +
+                                                   8 * c);
           const uint4 q1 = qf[64 * g], q0 = qf[64 * g + 32];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {

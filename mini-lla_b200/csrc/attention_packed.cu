@@ -789,7 +789,8 @@ struct PtLayout {
   static constexpr int kStat = kStages * kItemBytes;         // float [4][3][128]
   static constexpr int kScale = kStat + 12 * kPtVectors * 4;  // float [2][128]
   static constexpr int kSwap = kScale + 2 * kPtVectors * 4;   // float [2][2][128]
-  static constexpr int kTurn = (kSwap + 4 * kPtVectors * 4 + 127) / 128 * 128;  // outputs, 4 KB a warp
+  // outputs, 4 KB a warp
+  static constexpr int kTurn = (kSwap + 4 * kPtVectors * 4 + 127) / 128 * 128;
   static constexpr int kList = kTurn + 4 * 4096;  // int4 [4][2]
   static constexpr int kBars = kList + 4 * 32;
   // full / empty per stage, q_full[2], s_full[2], p_full[4], o_full, o_empty,
@@ -1337,7 +1338,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const int v = (warp & 3) * 32 + lane;  // query vector
     const int row = v / a.group;
     const bool used = v < (kPtVectors / a.group) * a.group;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kPtSCol + 64 * half;
+    const uint32_t lanes =
+        tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kPtSCol + 64 * half;
     const auto factor = [&](const PtWork& x, int block) {
       return a.factors[(static_cast<int64_t>(x.tile.block0) + block) * a.in.kv_heads + x.head].x;
     };
